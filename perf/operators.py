@@ -238,8 +238,7 @@ def _own(s):
         return F.fp4_ds_mla_sparse_decode_paged(s["q"], s["cache"], s["req"], s["table"], s["idx"], SM_SCALE, block_size=s["page"], return_lse=True)
     if s["op"] == "sparse":
         return F.fp4_ds_mla_sparse_decode(s["q"], s["cache"], s["idx"], SM_SCALE, return_lse=True)
-    return F.fp4_ds_mla_decode(s["q"], s["cache"], s["req"], s["table"], s["lens"], SM_SCALE, max_context_len=s["most"], block_size=s["page"],
-                               return_lse=True)
+    return F.fp4_ds_mla_decode(s["q"], s["cache"], s["req"], s["table"], s["lens"], SM_SCALE, block_size=s["page"], return_lse=True)
 
 
 # ---- what a pass cannot do without --------------------------------------------------------
