@@ -51,6 +51,18 @@ extern "C" {
 #define FP8MLA_SCALE_OFF 512
 #define FP8MLA_ROPE_OFF 528
 
+/* ---- fp4_ds_mla row geometry (416 bytes per KV slot) ----------------------
+ *     [  0:256)  512 x e2m1           NoPE latent, element 2i in the low nibble
+ *                                     of byte i, element 2i + 1 in the high one
+ *     [256:288)   32 x float8_e4m3fn  one scale per 16 latent values
+ *     [288:416)   64 x bfloat16       RoPE, stored raw
+ * A latent value is code * scale, exact in bf16 and fp16.  The format is this
+ * library's own (no reference counterpart): fp8_ds_mla with 4-bit latents. */
+#define FP8MLA_FP4_ROW_BYTES 416
+#define FP8MLA_FP4_GROUP 16
+#define FP8MLA_FP4_SCALE_OFF 256
+#define FP8MLA_FP4_ROPE_OFF 288
+
 /* Message of the last failed call on this thread ("" if none). */
 FP8MLA_API const char* fp8mla_last_error(void);
 
@@ -335,6 +347,92 @@ FP8MLA_API int fp8mla_indexer_topk(const float* logits, int64_t rows, int64_t lo
                                    int64_t next_n, const int32_t* context_lens, int32_t* out,
                                    int64_t out_stride, int64_t topk, int64_t max_model_len,
                                    void* stream);
+
+/* ======================= fp4_ds_mla: the 4-bit cache =======================
+ * No reference counterpart.  Rows as described at FP8MLA_FP4_ROW_BYTES; a
+ * pool is [num_slots, 416] uint8, 16-byte aligned, num_slots < 2^31. */
+
+/*
+ * Cache writer: bf16 latent + rope -> 416-byte rows.  Per group of 16 values
+ * scale = e4m3(amax / 6) within [2^-9, 448] and code = e2m1(x / scale), both
+ * rounded to nearest even, the code saturating at 6 (so |value| <= 2688).  A
+ * group that holds a NaN gets the NaN scale 0x7F and reads back as NaN.
+ * Arguments as fp8mla_ds_mla_write; slots < 0 or >= num_slots are skipped.
+ * A slot named twice in one call ends with either token's bytes, field by
+ * field.
+ */
+FP8MLA_API int fp8mla_fp4_write(const uint16_t* kv_c, int64_t kv_c_stride, const uint16_t* k_pe,
+                                int64_t k_pe_stride, const int64_t* slot_mapping, int64_t N,
+                                uint8_t* cache, int64_t num_slots, void* stream);
+
+/*
+ * Rows by slot -> bf16 out[n, 576] (row stride out_stride >= 576 elements,
+ * 16-byte aligned rows): latent code * scale, exact, then the raw rope.
+ * slots [n] int64; a slot < 0 or >= num_slots gives a zero row.
+ */
+FP8MLA_API int fp8mla_fp4_dequant_rows(const uint8_t* kv, int64_t num_slots, const int64_t* slots,
+                                       int64_t n, uint16_t* out, int64_t out_stride, void* stream);
+
+/*
+ * Whole sequences -> bf16 out[n, 576]: row r of sequence b (cu_seq_lens[b] <= r
+ * < cu_seq_lens[b + 1]) is position p = seq_starts[b] + r - cu_seq_lens[b] of
+ * it, at slot block_table[b, p / block_size] * block_size + p % block_size.
+ * Positions behind the table or slots outside the pool give zero rows; rows in
+ * front of cu_seq_lens[0] or from cu_seq_lens[B] on are left as they were.
+ *   cu_seq_lens [B + 1] int32, ascending; seq_starts [B] int32 or NULL (zeros).
+ */
+FP8MLA_API int fp8mla_fp4_gather(const uint8_t* kv, int64_t num_slots, const int32_t* block_table,
+                                 int64_t bt_stride, int64_t max_blocks, int64_t block_size,
+                                 const int32_t* cu_seq_lens, int64_t B, const int32_t* seq_starts,
+                                 int64_t n, uint16_t* out, int64_t out_stride, void* stream);
+
+/* Bytes of device workspace the three attention calls below need for a shape
+ * (16-byte aligned; the contents need no initialisation and carry nothing
+ * from call to call; calls that may run at once need one each). */
+FP8MLA_API int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G);
+
+/* Name of the attention kernel for H heads in G kv groups (introspection). */
+FP8MLA_API const char* fp8mla_fp4_kernel_name(int64_t H, int64_t G);
+
+/*
+ * Sparse MLA attention over fp4_ds_mla rows named by flat slots: arguments and
+ * masking as fp8mla_sparse_decode, with q, out bf16 only.  The division of the
+ * work over the SMs is the library's (no split count); results do not depend
+ * on timing.
+ */
+FP8MLA_API int fp8mla_fp4_sparse_decode(const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t,
+                                        int64_t q_stride_h, const uint8_t* kv, int64_t num_slots,
+                                        const int32_t* indices, int64_t G, int64_t topk,
+                                        int64_t idx_stride_t, int64_t idx_stride_g, float sm_scale,
+                                        uint16_t* out, int64_t out_stride_t, int64_t out_stride_h,
+                                        float* lse, int64_t lse_stride_t, void* workspace,
+                                        int64_t workspace_bytes, void* stream);
+
+/* The same over request-local positions (block table as in
+ * fp8mla_sparse_decode_paged). */
+FP8MLA_API int fp8mla_fp4_sparse_decode_paged(
+    const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* kv,
+    int64_t num_slots, const int32_t* req_id, const int32_t* block_table, int64_t bt_stride,
+    int64_t max_blocks, int64_t block_size, const int32_t* token_idx, int64_t G, int64_t topk,
+    int64_t ti_stride_t, int64_t ti_stride_g, float sm_scale, uint16_t* out, int64_t out_stride_t,
+    int64_t out_stride_h, float* lse, int64_t lse_stride_t, void* workspace, int64_t workspace_bytes,
+    void* stream);
+
+/*
+ * Attention over whole contexts: query token t attends to positions
+ * [0, context_lens[t]) of request req_id[t] through the block table (lengths
+ * below 0 count as 0, above max_blocks * block_size as that; positions whose
+ * slot is outside the pool are masked).  Lengths are read on the device, so
+ * one captured graph serves changing lengths.  With several query tokens of a
+ * request, each one's own length makes the attention causal.
+ */
+FP8MLA_API int fp8mla_fp4_decode(const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t,
+                                 int64_t q_stride_h, const uint8_t* kv, int64_t num_slots,
+                                 const int32_t* req_id, const int32_t* block_table, int64_t bt_stride,
+                                 int64_t max_blocks, int64_t block_size, const int32_t* context_lens,
+                                 float sm_scale, uint16_t* out, int64_t out_stride_t,
+                                 int64_t out_stride_h, float* lse, int64_t lse_stride_t,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

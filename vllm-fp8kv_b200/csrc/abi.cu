@@ -10,6 +10,7 @@
 
 #include "common.cuh"
 #include "decode.h"
+#include "decode_fp4.h"
 #include "wait_limit.h"
 
 namespace fp8mla {
@@ -49,16 +50,6 @@ const DevInfo* dev_info() {
     cudaDeviceGetAttribute(&g_dev[dev].minor, cudaDevAttrComputeCapabilityMinor, dev);
   });
   return &g_dev[dev];
-}
-
-int require_sm100() {
-  const DevInfo* d = dev_info();
-  if (d == nullptr) return set_error(FP8MLA_ERR_CUDA, "no current CUDA device");
-  if (d->major != 10 || d->minor != 0)
-    return set_error(FP8MLA_ERR_UNSUPPORTED,
-                     "libfp8mla is built for sm_100a (B200); current device is sm_%d%d",
-                     d->major, d->minor);
-  return FP8MLA_OK;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -109,6 +100,18 @@ int64_t ws_bytes(int64_t T, int64_t H, int S, int elem_bytes) {
 }
 }  // namespace
 
+void clear_error() { g_last_error[0] = 0; }
+
+int require_sm100() {
+  const DevInfo* d = dev_info();
+  if (d == nullptr) return set_error(FP8MLA_ERR_CUDA, "no current CUDA device");
+  if (d->major != 10 || d->minor != 0)
+    return set_error(FP8MLA_ERR_UNSUPPORTED,
+                     "libfp8mla is built for sm_100a (B200); current device is sm_%d%d",
+                     d->major, d->minor);
+  return FP8MLA_OK;
+}
+
 int device_sm_count() {
   const DevInfo* d = dev_info();
   return (d && d->sms > 0) ? d->sms : 148;
@@ -130,11 +133,12 @@ int fp8mla_device_status(unsigned int* status, int reset, void* stream) {
   *status = 0;
   if (int rc = require_sm100()) return rc;
   // each kernel file keeps its own status word
-  unsigned int v2 = 0, v3 = 0, v4 = 0;
+  unsigned int v2 = 0, v3 = 0, v4 = 0, v5 = 0;
   int rc = read_device_status_ws(&v2, reset != 0, static_cast<cudaStream_t>(stream));
   if (rc == FP8MLA_OK) rc = read_device_status_tc3(&v3, reset != 0, static_cast<cudaStream_t>(stream));
   if (rc == FP8MLA_OK) rc = read_device_status_idx(&v4, reset != 0, static_cast<cudaStream_t>(stream));
-  *status = v2 | v3 | v4;
+  if (rc == FP8MLA_OK) rc = read_device_status_fp4(&v5, reset != 0, static_cast<cudaStream_t>(stream));
+  *status = v2 | v3 | v4 | v5;
   return rc;
 }
 

@@ -1,0 +1,226 @@
+// abi_fp4.cu -- the C entry points of the 4-bit cache (include/fp8mla.h):
+// argument checks, the division of work, workspace layout and dispatch.
+#include "common.cuh"
+#include "decode_fp4.h"
+
+using namespace fp8mla;
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+struct Plan {
+  int rows, workers;
+};
+Plan plan_of(int64_t hpg) {
+  (void)hpg;
+  return Plan{16, device_sm_count()};
+}
+int64_t info_bytes(const Plan& p) { return (int64_t)p.workers * 4 * 8; }
+int64_t part_bytes(const Plan& p) { return (int64_t)2 * p.workers * p.rows * FP8MLA_NOPE * 4; }
+int64_t workspace_of(const Plan& p) {
+  return part_bytes(p) + (int64_t)2 * p.workers * p.rows * 8 + info_bytes(p);
+}
+
+int check_table(const int32_t* req_id, const int32_t* block_table, int64_t bt_stride, int64_t max_blocks,
+                int64_t block_size, int64_t T) {
+  if (block_size <= 0 || block_size > (1 << 20) || max_blocks < 0 || bt_stride < max_blocks)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "bad block table: block_size=%lld max_blocks=%lld stride=%lld",
+                     (long long)block_size, (long long)max_blocks, (long long)bt_stride);
+  if (max_blocks * block_size > INT32_MAX)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "a block-table row covers %lld positions; 2^31 - 1 at most",
+                     (long long)(max_blocks * block_size));
+  if (T > 0 && (req_id == nullptr || (max_blocks > 0 && block_table == nullptr)))
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "req_id and block_table are required");
+  return FP8MLA_OK;
+}
+
+int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, const uint8_t* kv,
+           int64_t num_slots, const int32_t* idx, int64_t G, int64_t topk, int64_t idx_st, int64_t idx_sg,
+           const int32_t* lens, const int32_t* req_id, const int32_t* block_table, int64_t bt_stride,
+           int64_t max_blocks, int64_t block_size, float sm_scale, uint16_t* out, int64_t out_st, int64_t out_sh,
+           float* lse, int64_t lse_st, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (T < 0 || H <= 0 || G <= 0 || topk < 0 || num_slots < 0 || num_slots >= (1LL << 31))
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "bad sizes T=%lld H=%lld G=%lld topk=%lld num_slots=%lld",
+                     (long long)T, (long long)H, (long long)G, (long long)topk, (long long)num_slots);
+  if (H % G != 0)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "h_q=%lld not divisible by kv_groups=%lld", (long long)H,
+                     (long long)G);
+  if (topk > (1LL << 30) || T > (1LL << 24) || H > (1 << 16))
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "topk, T or H too large");
+  if (T == 0) return FP8MLA_OK;
+  if (q == nullptr || out == nullptr || (num_slots > 0 && kv == nullptr) || (lens == nullptr && topk > 0 && idx == nullptr))
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned16(q) || q_st % 8 || q_sh % 8)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "q must be 16-byte aligned with row strides multiple of 16 bytes");
+  if (!aligned16(out) || out_st % 8 || out_sh % 8)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned with strides multiple of 8 elements");
+  if (!aligned16(kv)) return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "kv cache must be 16-byte aligned");
+  if (int rc = require_sm100()) return rc;
+
+  const int64_t hpg = H / G;
+  const Plan p = plan_of(hpg);
+  if (workspace == nullptr || workspace_bytes < workspace_of(p) || !aligned16(workspace))
+    return set_error(FP8MLA_ERR_WORKSPACE, "needs %lld bytes of 16-B aligned workspace, got %lld",
+                     (long long)workspace_of(p), (long long)workspace_bytes);
+  Fp4DecodeArgs a{};
+  a.q = q;
+  a.q_st = q_st;
+  a.q_sh = q_sh;
+  a.kv = kv;
+  a.num_slots = num_slots;
+  a.lens = lens;
+  a.idx = idx;
+  a.idx_st = idx_st;
+  a.idx_sg = idx_sg;
+  a.T = (int)T;
+  a.H = (int)H;
+  a.G = (int)G;
+  a.topk = (int)topk;
+  a.hpg = (int)hpg;
+  a.rows = p.rows;
+  a.hb_per_group = (int)((hpg + p.rows - 1) / p.rows);
+  a.scale_log2 = sm_scale * kLog2e;
+  a.out = out;
+  a.out_st = out_st;
+  a.out_sh = out_sh;
+  a.lse = lse;
+  a.lse_st = lse_st;
+  a.req_id = req_id;
+  // the kernels tell paged calls by the table: an empty one is never read, but
+  // its pointer may be null
+  a.block_table = req_id != nullptr && block_table == nullptr ? req_id : block_table;
+  a.bt_stride = bt_stride;
+  a.max_blocks = max_blocks;
+  a.block_size = (int)block_size;
+  a.block_shift = -1;
+  for (int k = 0; k < 31; ++k)
+    if (block_table != nullptr && (int64_t)1 << k == block_size) a.block_shift = k;
+  a.max_len = max_blocks * block_size;
+  char* ws = static_cast<char*>(workspace);
+  a.ws_o = reinterpret_cast<float*>(ws);
+  a.ws_info = reinterpret_cast<int64_t*>(ws + part_bytes(p));
+  a.ws_ml = reinterpret_cast<float2*>(ws + part_bytes(p) + info_bytes(p));
+
+  const int64_t chunk = decode_fp4_chunk();
+  const int64_t units = T * G * a.hb_per_group;
+  bool cuts = true;
+  if (lens == nullptr) {
+    const int64_t n = topk > chunk ? (topk + chunk - 1) / chunk : 1;
+    const int64_t total = units * n;
+    a.workers = (int)(total < p.workers ? total : p.workers);
+    a.per = (total + a.workers - 1) / a.workers;
+    // whole units where that costs a sixth more at most: no partials, no merge
+    const int64_t whole = (a.per + n - 1) / n * n;
+    if (whole * 6 <= a.per * 7) {
+      a.per = whole;
+      cuts = false;
+    }
+    a.workers = (int)((total + a.per - 1) / a.per);
+  } else {
+    const int64_t most = units * (a.max_len > chunk ? (a.max_len + chunk - 1) / chunk : 1);
+    a.workers = (int)(most < p.workers ? most : p.workers);
+    cuts = a.max_len > chunk;
+  }
+  return launch_decode_fp4(a, cuts, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp8mla_fp4_write(const uint16_t* kv_c, int64_t kv_c_stride, const uint16_t* k_pe, int64_t k_pe_stride,
+                     const int64_t* slot_mapping, int64_t N, uint8_t* cache, int64_t num_slots, void* stream) {
+  clear_error();
+  if (N < 0 || num_slots < 0 || kv_c_stride < FP8MLA_NOPE || k_pe_stride < FP8MLA_ROPE)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "bad writer sizes/strides");
+  if (N == 0) return FP8MLA_OK;
+  if (kv_c == nullptr || k_pe == nullptr || slot_mapping == nullptr || (num_slots > 0 && cache == nullptr))
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned16(cache)) return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "cache must be 16-byte aligned");
+  if (int rc = require_sm100()) return rc;
+  return launch_fp4_write(kv_c, kv_c_stride, k_pe, k_pe_stride, slot_mapping, N, cache, num_slots,
+                          static_cast<cudaStream_t>(stream));
+}
+
+int fp8mla_fp4_dequant_rows(const uint8_t* kv, int64_t num_slots, const int64_t* slots, int64_t n, uint16_t* out,
+                            int64_t out_stride, void* stream) {
+  clear_error();
+  if (n < 0 || num_slots < 0 || out_stride < kDqk)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "bad row-dequant arguments");
+  if (n == 0) return FP8MLA_OK;
+  if ((num_slots > 0 && kv == nullptr) || slots == nullptr || out == nullptr)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned16(kv) || !aligned16(out) || out_stride % 8 != 0)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "row dequant needs 16-byte aligned rows");
+  if (int rc = require_sm100()) return rc;
+  return launch_fp4_rows(kv, num_slots, slots, n, out, out_stride, static_cast<cudaStream_t>(stream));
+}
+
+int fp8mla_fp4_gather(const uint8_t* kv, int64_t num_slots, const int32_t* block_table, int64_t bt_stride,
+                      int64_t max_blocks, int64_t block_size, const int32_t* cu_seq_lens, int64_t B,
+                      const int32_t* seq_starts, int64_t n, uint16_t* out, int64_t out_stride, void* stream) {
+  clear_error();
+  if (n < 0 || num_slots < 0 || B < 0 || B > INT32_MAX || out_stride < kDqk || block_size <= 0 ||
+      block_size > (1 << 20) || max_blocks < 0 || bt_stride < max_blocks)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "bad gather sizes or strides");
+  if (n == 0 || B == 0) return FP8MLA_OK;
+  if ((num_slots > 0 && kv == nullptr) || cu_seq_lens == nullptr || out == nullptr ||
+      (max_blocks > 0 && block_table == nullptr))
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned16(kv) || !aligned16(out) || out_stride % 8 != 0)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "gather needs 16-byte aligned rows");
+  if (int rc = require_sm100()) return rc;
+  return launch_fp4_gather(kv, num_slots, block_table, bt_stride, max_blocks, (int)block_size, cu_seq_lens, (int)B,
+                           seq_starts, n, out, out_stride, static_cast<cudaStream_t>(stream));
+}
+
+int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G) {
+  if (T <= 0 || H <= 0 || G <= 0 || H % G != 0) return 0;
+  return workspace_of(plan_of(H / G));
+}
+
+const char* fp8mla_fp4_kernel_name(int64_t H, int64_t G) {
+  if (H <= 0 || G <= 0 || H % G != 0) return "";
+  return "decode_fp4_kernel";
+}
+
+int fp8mla_fp4_sparse_decode(const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t, int64_t q_stride_h,
+                             const uint8_t* kv, int64_t num_slots, const int32_t* indices, int64_t G, int64_t topk,
+                             int64_t idx_stride_t, int64_t idx_stride_g, float sm_scale, uint16_t* out,
+                             int64_t out_stride_t, int64_t out_stride_h, float* lse, int64_t lse_stride_t,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  return attend(q, T, H, q_stride_t, q_stride_h, kv, num_slots, indices, G, topk, idx_stride_t, idx_stride_g,
+                nullptr, nullptr, nullptr, 0, 0, 0, sm_scale, out, out_stride_t, out_stride_h, lse, lse_stride_t,
+                workspace, workspace_bytes, stream);
+}
+
+int fp8mla_fp4_sparse_decode_paged(const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t, int64_t q_stride_h,
+                                   const uint8_t* kv, int64_t num_slots, const int32_t* req_id,
+                                   const int32_t* block_table, int64_t bt_stride, int64_t max_blocks,
+                                   int64_t block_size, const int32_t* token_idx, int64_t G, int64_t topk,
+                                   int64_t ti_stride_t, int64_t ti_stride_g, float sm_scale, uint16_t* out,
+                                   int64_t out_stride_t, int64_t out_stride_h, float* lse, int64_t lse_stride_t,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_table(req_id, block_table, bt_stride, max_blocks, block_size, T)) return rc;
+  return attend(q, T, H, q_stride_t, q_stride_h, kv, num_slots, token_idx, G, topk, ti_stride_t, ti_stride_g,
+                nullptr, req_id, block_table, bt_stride, max_blocks, block_size, sm_scale, out, out_stride_t,
+                out_stride_h, lse, lse_stride_t, workspace, workspace_bytes, stream);
+}
+
+int fp8mla_fp4_decode(const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t, int64_t q_stride_h,
+                      const uint8_t* kv, int64_t num_slots, const int32_t* req_id, const int32_t* block_table,
+                      int64_t bt_stride, int64_t max_blocks, int64_t block_size, const int32_t* context_lens,
+                      float sm_scale, uint16_t* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                      int64_t lse_stride_t, void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_table(req_id, block_table, bt_stride, max_blocks, block_size, T)) return rc;
+  if (T > 0 && context_lens == nullptr) return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "context_lens is required");
+  return attend(q, T, H, q_stride_t, q_stride_h, kv, num_slots, nullptr, 1, 0, 0, 0, context_lens, req_id,
+                block_table, bt_stride, max_blocks, block_size, sm_scale, out, out_stride_t, out_stride_h, lse,
+                lse_stride_t, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -33,6 +33,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Records `msg` as this thread's last error and returns `code`.
 int set_error(int code, const char* fmt, ...);
 int check_cuda(cudaError_t e, const char* what);
+void clear_error();
+int require_sm100();  // FP8MLA_OK when the current device is sm_100
 int device_sm_count();
 int device_arch(int* major, int* minor);
 

@@ -1,0 +1,706 @@
+// decode_fp4.cu -- attention over fp4_ds_mla rows, 16 query heads per unit.
+//
+//   S = scale q . [latent | rope],  P = softmax(S),  O = P . latent
+//
+// A persistent CTA per SM walks its run of 64-entry chunks (decode_fp4.h).
+// The 416-byte rows stay 4-bit in shared memory; both products unpack them in
+// registers, straight into mma.sync fragments: a bf16 copy of a row in shared
+// memory would cost 1152 bytes written and twice read against 416 read twice.
+//   * latents are exact in fp16 (fp4.cuh), so the latent products are fp16
+//     MMAs: q is scaled per head by a power of two to a largest value in
+//     [2^8, 2^9) and converted (exact down to 2^-22 of that value, below it an
+//     error under 2^-33 of it), and P keeps 11 bits where bf16 keeps 8;
+//   * the rope (bf16 as stored) and q's rope (times the same power of two)
+//     go through bf16 MMAs into the same accumulators.
+//
+// Warp roles (512 threads, one of each kind per SM sub-partition but for PV):
+//   warps 0-3   S and softmax: warp w owns entries [16w, +16) of the chunk and
+//               holds all of q (16 heads x 576) as 144 registers of fragments;
+//               the four agree on the chunk's maxima through shared memory
+//   warps 4-11  O: warp w owns 64 of the 512 output dims
+//   warps 12-15 producers: entries -> slots -> TMA copies of 16 rows each
+// The registers move between the warpgroups accordingly (setmaxnreg: 232, 104,
+// 104, 64; the launch holds 128 each).
+#include "decode_fp4.h"
+#include "fp4.cuh"
+#include "tc_cluster.cuh"
+#include "tc_ptx.cuh"
+#include "tma_map.h"
+
+namespace fp8mla {
+namespace {
+using namespace fp8mla::fp4;
+using namespace fp8mla::tc;
+
+constexpr int kBH = 16;           // heads per unit
+constexpr int kBN = 64;           // entries per chunk
+constexpr int kStages = 7;
+constexpr int kStageBytes = kBN * kFp4RowBytes;  // 26624
+constexpr int kSWarps = 4, kOWarps = 8, kPWarps = 4;
+constexpr int kThreads = 32 * (kSWarps + kOWarps + kPWarps);
+constexpr int kRowsPerPWarp = kBN / kPWarps;  // 16
+constexpr float kRescale = 8.0f;  // the reference maximum lags by at most 2^8 ...
+constexpr float kBias = 6.0f;     // ... and P is stored times 2^6: below 2^14 in
+                                  // fp16, above its smallest value from 2^-30 on
+
+struct Smem {
+  uint8_t raw[kStages][kStageBytes];   // 128-B aligned TMA destinations
+  uint32_t p[2][kSWarps][32][4];       // P as A fragments of the O product
+  float smax[2][kSWarps][kBH];
+  float alpha[2][kBH];
+  float fin[2][kBH][2];                // a piece's reference maximum and sum
+  float lpart[kSWarps][kBH];
+  uint32_t live[kStages][2];           // 16 bits per producer warp
+  uint64_t raw_full[kStages], raw_empty[kStages];
+  uint64_t p_full[2], p_empty[2], fin_full[2], fin_empty[2];
+  int64_t tok_total, start_unit;
+  int start_chunk;
+  int64_t scan[kThreads / 32];
+};
+static_assert(offsetof(Smem, p) % 16 == 0 && offsetof(Smem, raw_full) % 8 == 0, "alignment");
+static_assert(sizeof(Smem) + 128 <= 227 * 1024, "shared memory budget");
+
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegs));
+}
+// Bounded wait after which every lane has acquired the phase itself.
+__device__ __forceinline__ bool acquire(uint32_t bar, uint32_t parity, uint32_t where) {
+  const bool ok = warp_wait(bar, parity, where);
+  if (ok) (void)mbar_try_wait(bar, parity);
+  return ok;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+// The chunk row that column n of an 8-column tile stands for, n even: n / 2,
+// n odd: 4 + (n / 2 + 1) % 4.  It is both the S product's B column and the O
+// product's k index, so P needs no shuffle between them; the rows of a column
+// pair differ by an odd number (S loads of two rows meet no bank twice: a row
+// is 104 words) and the rows of the even, or odd, columns are all different
+// modulo 4 (neither do the O loads of four rows).
+__device__ __forceinline__ int row_even(int pair) { return pair; }
+__device__ __forceinline__ int row_odd(int pair) { return 4 + ((pair + 1) & 3); }
+
+// Where this worker starts, and how many chunks each worker takes: from the
+// sizes, or (lengths on the device) from two passes over the lengths.
+// Returns `per`; the start goes to shared memory.
+__device__ int64_t divide_work(const Fp4DecodeArgs& a, Smem& s) {
+  const int per_tok = a.G * a.hb_per_group;
+  int64_t per = a.per;
+  if (a.lens == nullptr) {
+    if (threadIdx.x == 0) {
+      const int64_t n = fp4_chunks(a.topk, kBN), at = (int64_t)blockIdx.x * per;
+      s.tok_total = (int64_t)a.T * per_tok * n;
+      s.start_unit = at / n;
+      s.start_chunk = (int)(at - s.start_unit * n);
+    }
+    __syncthreads();
+    return per;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t sum = 0;
+  for (int t = threadIdx.x; t < a.T; t += kThreads) sum += fp4_chunks(fp4_entries(a, t), kBN);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (lane == 0) s.scan[warp] = sum;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) total += s.scan[w];
+  total *= per_tok;
+  per = (total + a.workers - 1) / a.workers;
+  const int64_t at = (int64_t)blockIdx.x * per;
+  int64_t before = 0;  // chunks of the tokens in front of this pass
+  for (int t0 = 0; t0 < a.T; t0 += kThreads) {
+    const int t = t0 + threadIdx.x;
+    const int n = t < a.T ? fp4_chunks(fp4_entries(a, t), kBN) : 0;
+    const int64_t mine = (int64_t)n * per_tok;
+    int64_t inc = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    __syncthreads();
+    if (lane == 31) s.scan[warp] = inc;
+    __syncthreads();
+    int64_t base = before;
+    for (int w = 0; w < warp; ++w) base += s.scan[w];
+    const int64_t hi = base + inc, lo = hi - mine;
+    if (t < a.T && at >= lo && at < hi) {
+      const int64_t u = (at - lo) / n;
+      s.start_unit = (int64_t)t * per_tok + u;
+      s.start_chunk = (int)(at - lo - u * n);
+    }
+    for (int w = 0; w < kThreads / 32; ++w) before += s.scan[w];
+  }
+  if (threadIdx.x == 0) s.tok_total = total;
+  __syncthreads();
+  return per;
+}
+
+// A worker's chunks in order.
+struct Walk {
+  Fp4Cursor x;
+  int64_t left;  // chunks of this worker from the current one on
+  __device__ __forceinline__ Walk(const Fp4DecodeArgs& a, const Smem& s, int64_t per) {
+    const int64_t at = (int64_t)blockIdx.x * per;
+    left = s.tok_total - at < per ? s.tok_total - at : per;
+    if (left > 0) {
+      fp4_open(a, x, s.start_unit, kBN);
+      x.c = s.start_chunk;
+    }
+  }
+  // chunks of this worker in the current unit, from the current chunk on
+  __device__ __forceinline__ int here() const { return (int)(left < x.n - x.c ? left : x.n - x.c); }
+  __device__ __forceinline__ void next_unit(const Fp4DecodeArgs& a, int done) {
+    left -= done;
+    if (left > 0) fp4_open(a, x, x.unit + 1, kBN);
+  }
+};
+
+// ------------------------------------------------------------------ producers
+// Warp pw owns rows [16 pw, +16) of every chunk, lane i (and i + 16) row i.  The entry
+// is read two chunks ahead, its block-table word one chunk ahead.  A run of
+// consecutive slots (the pages of a whole context) is one bulk copy, other
+// rows go four at a time through gather4; masked rows are not read (a group
+// with some fetches row 0 for them) and their bits stay clear.
+__device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, int64_t per, int pw, int lane) {
+  const int row = 16 * pw + (lane & 15);
+  Walk ahead(a, s, per);
+  int32_t req_ahead = 0;
+  const int32_t* idx_row = nullptr;
+  auto open = [&]() {
+    if (ahead.left <= 0) return;
+    req_ahead = a.block_table != nullptr ? a.req_id[ahead.x.t] : 0;
+    if (a.lens == nullptr) idx_row = a.idx + ahead.x.t * a.idx_st + ahead.x.grp * a.idx_sg;
+  };
+  open();
+  struct Entry {
+    int32_t v, req;
+  };
+  auto fetch = [&]() -> Entry {
+    Entry e{-1, 0};
+    if (ahead.left <= 0) return e;
+    const int pos = ahead.x.c * kBN + row;
+    e.req = req_ahead;
+    if (pos < ahead.x.entries) e.v = a.lens == nullptr ? idx_row[pos] : pos;
+    ++ahead.x.c;
+    --ahead.left;
+    if (ahead.x.c == ahead.x.n && ahead.left > 0) {
+      fp4_open(a, ahead.x, ahead.x.unit + 1, kBN);
+      open();
+    }
+    return e;
+  };
+  const int64_t chunks = ahead.left;
+  Entry e0 = fetch(), e1 = fetch();
+  int32_t pg0 = fp4_table(a, e0.req, e0.v);
+  bool ok = true;
+  int64_t armed = 0;
+  for (int64_t g = 0; g < chunks; ++g) {
+    const int32_t slot = fp4_slot(a, e0.v, pg0);
+    const Entry e2 = fetch();
+    pg0 = fp4_table(a, e1.req, e1.v);
+    e0 = e1;
+    e1 = e2;
+    const int st = (int)(g % kStages);
+    if (g >= kStages) ok = warp_wait(smem_u32(&s.raw_empty[st]), (uint32_t)(g / kStages + 1) & 1, 20);
+    if (!ok) break;
+    const uint32_t live = __ballot_sync(0xFFFFFFFFu, slot >= 0) & 0xFFFFu;
+    const int n = __popc(live);
+    const int32_t s0 = __shfl_sync(0xFFFFFFFFu, slot, 0);
+    const bool run = __all_sync(0xFFFFFFFFu, slot < 0 || slot == s0 + (lane & 15)) && (live & (live + 1)) == 0;
+    const uint32_t bar = smem_u32(&s.raw_full[st]);
+    const uint32_t dst = smem_u32(&s.raw[st][16 * pw * kFp4RowBytes]);
+    // groups of four rows with a live one
+    const uint32_t grp = (live & 0xFu ? 1u : 0u) | (live & 0xF0u ? 2u : 0u) | (live & 0xF00u ? 4u : 0u) |
+                         (live & 0xF000u ? 8u : 0u);
+    if (lane == 0) {
+      reinterpret_cast<uint16_t*>(s.live[st])[pw] = (uint16_t)live;
+      mbar_arrive_expect_tx(bar, run ? (uint32_t)(n * kFp4RowBytes) : (uint32_t)(__popc(grp) * 4 * kFp4RowBytes));
+    }
+    __syncwarp();
+    if (run) {
+      if (lane == 0 && n > 0) bulk_g2s(dst, a.kv + (int64_t)s0 * kFp4RowBytes, (uint32_t)(n * kFp4RowBytes), bar);
+    } else {
+      const int32_t r = slot >= 0 ? slot : 0;
+      const int src = (4 * lane) & 15;
+      const int32_t r0 = __shfl_sync(0xFFFFFFFFu, r, src);
+      const int32_t r1 = __shfl_sync(0xFFFFFFFFu, r, src + 1);
+      const int32_t r2 = __shfl_sync(0xFFFFFFFFu, r, src + 2);
+      const int32_t r3 = __shfl_sync(0xFFFFFFFFu, r, src + 3);
+      if (lane < 4 && ((grp >> lane) & 1u)) tma_gather4(dst + lane * 4 * kFp4RowBytes, tm, 0, r0, r1, r2, r3, bar);
+    }
+    ++armed;
+  }
+  // the stages armed last have landed before the warp returns, even after a
+  // failed wait
+  for (int64_t x = armed > kStages ? armed - kStages : 0; x < armed; ++x)
+    (void)warp_wait(smem_u32(&s.raw_full[x % kStages]), (uint32_t)(x / kStages) & 1, 26);
+}
+
+// ------------------------------------------------------------------ S and softmax
+// Fragment coordinates: lane = 4 gq + q4.  Thread q4 of a quad owns latent
+// dims [128 q4, +128) of a row and rope dims [16 q4, +16); it walks its four
+// 32-dim pieces in the order i ^ (q4 >> 1) and its two rope halves in the order
+// h ^ (q4 & 1), so that 8 lanes' 16-byte loads cover all banks.  q's fragments
+// follow the same order.
+struct QFrag {
+  uint32_t a[36][4];
+  float scale[2];  // heads gq, gq + 8: score = scale * accumulator (log2 units)
+};
+__device__ __forceinline__ void load_q(const Fp4DecodeArgs& a, QFrag& f, const Fp4Cursor& x, int gq, int q4) {
+  const int h0 = x.grp * a.hpg + x.hb * kBH;
+  const int nh = min(kBH, a.hpg - x.hb * kBH);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = gq + 8 * r;
+    const bool hv = row < nh;
+    const uint16_t* src = a.q + x.t * a.q_st + (int64_t)(h0 + (hv ? row : 0)) * a.q_sh;
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4* p = reinterpret_cast<const uint4*>(src + 128 * q4 + 32 * (i ^ (q4 >> 1)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // 8 dims: k-steps 8i + 2j and 8i + 2j + 1
+        const uint4 v = hv ? p[j] : make_uint4(0, 0, 0, 0);
+        f.a[8 * i + 2 * j][r] = v.x;
+        f.a[8 * i + 2 * j][2 + r] = v.y;
+        f.a[8 * i + 2 * j + 1][r] = v.z;
+        f.a[8 * i + 2 * j + 1][2 + r] = v.w;
+        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
+                                   __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+      }
+    }
+    uint32_t mxr = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 v = hv ? *reinterpret_cast<const uint4*>(src + kNope + 16 * q4 + 8 * (h ^ (q4 & 1)))
+                         : make_uint4(0, 0, 0, 0);
+      f.a[32 + 2 * h][r] = v.x;
+      f.a[32 + 2 * h][2 + r] = v.y;
+      f.a[32 + 2 * h + 1][r] = v.z;
+      f.a[32 + 2 * h + 1][2 + r] = v.w;
+      mxr = __vmaxu2(mxr, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
+                                   __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+    }
+    // largest magnitudes (as bits) of the head's latent part and of its rope
+    uint32_t m = max(mx & 0xFFFFu, mx >> 16), mr = max(mxr & 0xFFFFu, mxr >> 16);
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      mr = max(mr, __shfl_xor_sync(0xFFFFFFFFu, mr, o));
+    }
+    // 2^k brings the latent part's largest value to [2^8, 2^9), but the rope's
+    // at most to 2^101, where its products are still finite; 1 for rows of
+    // zeros, inf or NaN.  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are
+    // normal.
+    int k = min(8 - ((int)(m >> 7) - 127), 100 - ((int)(mr >> 7) - 127));
+    k = (m == 0 || m >= 0x7F80u) ? 0 : min(126, k);
+    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+    f.scale[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      f.a[i][r] = pack_f16x2(bf16_lo(f.a[i][r]) * up, bf16_hi(f.a[i][r]) * up);
+      f.a[i][2 + r] = pack_f16x2(bf16_lo(f.a[i][2 + r]) * up, bf16_hi(f.a[i][2 + r]) * up);
+    }
+#pragma unroll
+    for (int i = 32; i < 36; ++i) {
+      f.a[i][r] = pack_bf16x2(bf16_lo(f.a[i][r]) * up, bf16_hi(f.a[i][r]) * up);
+      f.a[i][2 + r] = pack_bf16x2(bf16_lo(f.a[i][2 + r]) * up, bf16_hi(f.a[i][2 + r]) * up);
+    }
+  }
+}
+
+// Accumulators of 8 entries: the row at `row` (this lane's column gq).
+__device__ __forceinline__ void score_tile(const QFrag& f, const uint8_t* row, int q4, float (&acc)[4]) {
+  float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+  float c2[4] = {0.f, 0.f, 0.f, 0.f}, c3[4] = {0.f, 0.f, 0.f, 0.f};
+  uint2 sc = *reinterpret_cast<const uint2*>(row + kFp4ScaleOff + 8 * q4);
+  const uint32_t sel = (q4 >> 1) ? 0x1032u : 0x3210u;
+  sc.x = __byte_perm(sc.x, 0, sel);
+  sc.y = __byte_perm(sc.y, 0, sel);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 w = *reinterpret_cast<const uint4*>(row + 64 * q4 + 16 * (i ^ (q4 >> 1)));
+    const uint32_t sw = i < 2 ? sc.x : sc.y;
+    const uint32_t s2 = e4m3x2_to_f16((i & 1) ? sw >> 16 : sw);
+    const uint32_t s_lo = __byte_perm(s2, 0, 0x1010), s_hi = __byte_perm(s2, 0, 0x3232);
+    uint32_t h[4];
+    e2m1x8_to_f16(w.x, h);
+    mma_f16(c0, f.a[8 * i], mul_f16x2(h[0], s_lo), mul_f16x2(h[1], s_lo));
+    mma_f16(c1, f.a[8 * i + 1], mul_f16x2(h[2], s_lo), mul_f16x2(h[3], s_lo));
+    e2m1x8_to_f16(w.y, h);
+    mma_f16(c2, f.a[8 * i + 2], mul_f16x2(h[0], s_lo), mul_f16x2(h[1], s_lo));
+    mma_f16(c3, f.a[8 * i + 3], mul_f16x2(h[2], s_lo), mul_f16x2(h[3], s_lo));
+    e2m1x8_to_f16(w.z, h);
+    mma_f16(c0, f.a[8 * i + 4], mul_f16x2(h[0], s_hi), mul_f16x2(h[1], s_hi));
+    mma_f16(c1, f.a[8 * i + 5], mul_f16x2(h[2], s_hi), mul_f16x2(h[3], s_hi));
+    e2m1x8_to_f16(w.w, h);
+    mma_f16(c2, f.a[8 * i + 6], mul_f16x2(h[0], s_hi), mul_f16x2(h[1], s_hi));
+    mma_f16(c3, f.a[8 * i + 7], mul_f16x2(h[2], s_hi), mul_f16x2(h[3], s_hi));
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint4 w = *reinterpret_cast<const uint4*>(row + kFp4RopeOff + 32 * q4 + 16 * (h ^ (q4 & 1)));
+    const uint32_t(&a0)[4] = f.a[32 + 2 * h];
+    const uint32_t(&a1)[4] = f.a[32 + 2 * h + 1];
+    mma_bf16_16816(h == 0 ? c0 : c2, a0[0], a0[1], a0[2], a0[3], w.x, w.y);
+    mma_bf16_16816(h == 0 ? c1 : c3, a1[0], a1[1], a1[2], a1[3], w.z, w.w);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = (c0[i] + c1[i]) + (c2[i] + c3[i]);
+}
+
+__device__ void scores(const Fp4DecodeArgs& a, Smem& s, int64_t per, int sw, int lane) {
+  const int gq = lane >> 2, q4 = lane & 3;
+  Walk w(a, s, per);
+  int64_t g = 0;
+  int piece = 0;
+  bool ok = true;
+  const int rowb = (gq & 1) ? row_odd(gq >> 1) : row_even(gq >> 1);
+  const int re = row_even(q4), ro = row_odd(q4);
+  while (w.left > 0) {
+    const int nch = w.here();
+    QFrag f;
+    load_q(a, f, w.x, gq, q4);
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int c = 0; c < nch; ++c, ++g) {
+      const int st = (int)(g % kStages), pb = (int)(g & 1);
+      if (ok) ok = acquire(smem_u32(&s.raw_full[st]), (uint32_t)(g / kStages) & 1, 21);
+      const uint32_t live = s.live[st][sw >> 1] >> (16 * (sw & 1));
+      const uint8_t* base = s.raw[st] + (16 * sw + rowb) * kFp4RowBytes;
+      float x[2][4];
+      score_tile(f, base, q4, x[0]);
+      score_tile(f, base + 8 * kFp4RowBytes, q4, x[1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s.raw_empty[st]));
+      // masked entries to -inf; maxima of heads gq and gq + 8
+      float mt[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const bool le = (live >> (8 * nt + re)) & 1u, lo = (live >> (8 * nt + ro)) & 1u;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          x[nt][2 * r] = le ? x[nt][2 * r] * f.scale[r] : -INFINITY;
+          x[nt][2 * r + 1] = lo ? x[nt][2 * r + 1] * f.scale[r] : -INFINITY;
+          mt[r] = fmaxf(mt[r], fmaxf(x[nt][2 * r], x[nt][2 * r + 1]));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xFFFFFFFFu, mt[r], 1));
+        mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xFFFFFFFFu, mt[r], 2));
+        if (q4 == 0) s.smax[pb][sw][gq + 8 * r] = mt[r];
+      }
+      named_sync(1, 32 * kSWarps);
+      float al[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int h = gq + 8 * r;
+        const float tm = fmaxf(fmaxf(s.smax[pb][0][h], s.smax[pb][1][h]), fmaxf(s.smax[pb][2][h], s.smax[pb][3][h]));
+        al[r] = 1.f;
+        if (tm > m[r] + kRescale || (m[r] == -INFINITY && tm > -INFINITY)) {
+          al[r] = m[r] == -INFINITY ? 0.f : ex2_approx(m[r] - tm);
+          m[r] = tm;
+        }
+        l[r] *= al[r];
+        const float sub = m[r] == -INFINITY ? 0.f : m[r] - kBias;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          x[nt][2 * r] = ex2_approx(x[nt][2 * r] - sub);
+          x[nt][2 * r + 1] = ex2_approx(x[nt][2 * r + 1] - sub);
+          l[r] += x[nt][2 * r] + x[nt][2 * r + 1];
+        }
+      }
+      if (ok && g >= 2) ok = warp_wait(smem_u32(&s.p_empty[pb]), (uint32_t)(g / 2 + 1) & 1, 22);
+      *reinterpret_cast<uint4*>(s.p[pb][sw][lane]) =
+          make_uint4(pack_f16x2(x[0][0], x[0][1]), pack_f16x2(x[0][2], x[0][3]), pack_f16x2(x[1][0], x[1][1]),
+                     pack_f16x2(x[1][2], x[1][3]));
+      if (sw == 0 && q4 == 0) {
+        s.alpha[pb][gq] = al[0];
+        s.alpha[pb][gq + 8] = al[1];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s.p_full[pb]));
+    }
+    // ---- the piece's sums
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
+      if (q4 == 0) s.lpart[sw][gq + 8 * r] = l[r];
+    }
+    named_sync(1, 32 * kSWarps);
+    const int fb = piece & 1;
+    if (ok && piece >= 2) ok = warp_wait(smem_u32(&s.fin_empty[fb]), (uint32_t)(piece / 2 + 1) & 1, 23);
+    if (sw == 0 && q4 == 0) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int h = gq + 8 * r;
+        s.fin[fb][h][0] = m[r];
+        s.fin[fb][h][1] = (s.lpart[0][h] + s.lpart[1][h]) + (s.lpart[2][h] + s.lpart[3][h]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&s.fin_full[fb]));
+    // (lpart is written again only after the next chunk's barrier)
+    ++piece;
+    w.next_unit(a, nch);
+  }
+}
+
+// ------------------------------------------------------------------ O
+__device__ void outputs(const Fp4DecodeArgs& a, Smem& s, int64_t per, int ow, int lane) {
+  const int gq = lane >> 2, q4 = lane & 3;
+  Walk w(a, s, per);
+  int64_t g = 0;
+  int piece = 0;
+  bool ok = true;
+  // rows of k indices 2 q4, 2 q4 + 1, + 8, + 9 of a 16-entry step
+  const int ra = row_even(q4), rb = row_odd(q4);
+  const int code_at = 32 * ow + 4 * gq, scale_at = kFp4ScaleOff + 4 * ow + (gq >> 1);
+  while (w.left > 0) {
+    const int nch = w.here();
+    float acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    for (int c = 0; c < nch; ++c, ++g) {
+      const int st = (int)(g % kStages), pb = (int)(g & 1);
+      if (ok) ok = acquire(smem_u32(&s.p_full[pb]), (uint32_t)(g / 2) & 1, 24);
+      if (ok) ok = acquire(smem_u32(&s.raw_full[st]), (uint32_t)(g / kStages) & 1, 27);
+      const float al0 = s.alpha[pb][gq], al1 = s.alpha[pb][gq + 8];
+      if (__any_sync(0xFFFFFFFFu, al0 != 1.f || al1 != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          acc[i][0] *= al0;
+          acc[i][1] *= al0;
+          acc[i][2] *= al1;
+          acc[i][3] *= al1;
+        }
+      }
+      const uint64_t live = *reinterpret_cast<const uint64_t*>(s.live[st]);
+      const uint8_t* raw = s.raw[st];
+#pragma unroll
+      for (int kk = 0; kk < kBN / 16; ++kk) {
+        const uint4 pv = *reinterpret_cast<const uint4*>(s.p[pb][kk][lane]);
+        const uint32_t pa[4] = {pv.x, pv.y, pv.z, pv.w};
+        const uint8_t* r0 = raw + (16 * kk + ra) * kFp4RowBytes;
+        const uint8_t* r1 = raw + (16 * kk + rb) * kFp4RowBytes;
+        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(r0 + code_at);
+        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(r1 + code_at);
+        const uint32_t w2 = *reinterpret_cast<const uint32_t*>(r0 + 8 * kFp4RowBytes + code_at);
+        const uint32_t w3 = *reinterpret_cast<const uint32_t*>(r1 + 8 * kFp4RowBytes + code_at);
+        uint32_t b0 = r0[scale_at], b1 = r1[scale_at];
+        uint32_t b2 = r0[8 * kFp4RowBytes + scale_at], b3 = r1[8 * kFp4RowBytes + scale_at];
+        if (live != ~0ull) {  // P is 0 there, but a NaN scale would still spread
+          const uint32_t lv = (uint32_t)(live >> (16 * kk));
+          b0 = (lv >> ra) & 1u ? b0 : 0u;
+          b1 = (lv >> rb) & 1u ? b1 : 0u;
+          b2 = (lv >> (ra + 8)) & 1u ? b2 : 0u;
+          b3 = (lv >> (rb + 8)) & 1u ? b3 : 0u;
+        }
+        const uint32_t s01 = e4m3x2_to_f16(b0 | (b1 << 8)), s23 = e4m3x2_to_f16(b2 | (b3 << 8));
+        // nibble pairs (row of the even k index low, of the odd one high):
+        // even dims, then odd dims of this thread's eight
+        uint32_t e01[4], e23[4];
+        e2m1x8_to_f16((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), e01);
+        e2m1x8_to_f16((w2 & 0x0F0F0F0Fu) | ((w3 << 4) & 0xF0F0F0F0u), e23);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) mma_f16(acc[2 * b], pa, mul_f16x2(e01[b], s01), mul_f16x2(e23[b], s23));
+        e2m1x8_to_f16(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), e01);
+        e2m1x8_to_f16(((w2 >> 4) & 0x0F0F0F0Fu) | (w3 & 0xF0F0F0F0u), e23);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) mma_f16(acc[2 * b + 1], pa, mul_f16x2(e01[b], s01), mul_f16x2(e23[b], s23));
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&s.raw_empty[st]));
+        mbar_arrive(smem_u32(&s.p_empty[pb]));
+      }
+    }
+    // ---- the piece: a whole unit goes to the output, a cut one to its slot
+    const int fb = piece & 1;
+    if (ok) ok = acquire(smem_u32(&s.fin_full[fb]), (uint32_t)(piece / 2) & 1, 25);
+    const bool whole = w.x.c == 0 && nch == w.x.n;
+    const int h0 = w.x.grp * a.hpg + w.x.hb * kBH;
+    const int nh = min(kBH, a.hpg - w.x.hb * kBH);
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (w.x.c == 0 ? 1 : 0);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = gq + 8 * r;
+      if (row >= nh) continue;
+      const float m = s.fin[fb][row][0], l = s.fin[fb][row][1];
+      const int d = 64 * ow + 16 * q4;
+      if (whole) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        uint16_t* o = a.out + w.x.t * a.out_st + (int64_t)(h0 + row) * a.out_sh + d;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(acc[2 * i][2 * r + j] * inv, acc[2 * i + 1][2 * r + j] * inv);
+          reinterpret_cast<uint4*>(o)[j] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        if (a.lse != nullptr && ow == 0 && q4 == 0)
+          a.lse[w.x.t * a.lse_st + h0 + row] = l == 0.f ? -INFINITY : (m - kBias) * kLn2 + logf(l);
+      } else {
+        float4* o = reinterpret_cast<float4*>(a.ws_o + (slot * kBH + row) * kNope + d);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            o[2 * j + i] = make_float4(acc[4 * i][2 * r + j], acc[4 * i + 1][2 * r + j], acc[4 * i + 2][2 * r + j],
+                                       acc[4 * i + 3][2 * r + j]);
+        if (ow == 0 && q4 == 0) a.ws_ml[slot * kBH + row] = make_float2(m, l);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&s.fin_empty[fb]));
+    ++piece;
+    w.next_unit(a, nch);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    decode_fp4_kernel(const Fp4DecodeArgs a, const __grid_constant__ CUtensorMap tm) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw + (((raw_base + 127u) & ~127u) - raw_base));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&s.raw_full[i]), kPWarps);
+      mbar_init(smem_u32(&s.raw_empty[i]), kSWarps + kOWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&s.p_full[i]), kSWarps);
+      mbar_init(smem_u32(&s.p_empty[i]), kOWarps);
+      mbar_init(smem_u32(&s.fin_full[i]), kSWarps);
+      mbar_init(smem_u32(&s.fin_empty[i]), kOWarps);
+    }
+    mbar_init_fence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  pdl_wait();  // the previous kernel of the stream has completed: global memory from here on
+  const int64_t per = divide_work(a, s);
+  if (threadIdx.x == 0) {
+    const int64_t at = (int64_t)blockIdx.x * per;
+    int64_t* info = a.ws_info + 4 * blockIdx.x;
+    if (at < s.tok_total) {
+      const int64_t t = s.start_unit / (a.G * a.hb_per_group);
+      info[0] = s.start_unit;
+      info[1] = s.start_chunk;
+      info[2] = fp4_chunks(fp4_entries(a, t), kBN);
+    } else {
+      info[1] = 0;
+    }
+    info[3] = per;
+  }
+  if (warp < kSWarps) {
+    regs_inc<232>();
+    scores(a, s, per, warp, lane);
+  } else if (warp < kSWarps + kOWarps) {
+    regs_dec<104>();
+    outputs(a, s, per, warp - kSWarps, lane);
+  } else {
+    regs_dec<64>();
+    produce(a, s, &tm, per, warp - kSWarps - kOWarps, lane);
+  }
+}
+
+// ------------------------------------------------------------------ merge
+// Block (w, y) joins the pieces of the unit that the border in front of worker
+// w cuts first, for one head: out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i.
+__global__ void __launch_bounds__(128) merge_fp4_kernel(const Fp4DecodeArgs a, float bias) {
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  pdl_wait();
+  const int w = blockIdx.x + 1;
+  const int64_t* info = a.ws_info + 4 * (int64_t)w;
+  const int64_t c = info[1], per = info[3];
+  if (c == 0 || c > per) return;  // no cut here, or cut by an earlier border too
+  const int64_t unit = info[0], n = info[2];
+  const int pieces = 1 + (int)((n - c + per - 1) / per);
+  const int per_tok = a.G * a.hb_per_group;
+  const int64_t t = unit / per_tok;
+  const int rest = (int)(unit - t * per_tok), grp = rest / a.hb_per_group, hb = rest - grp * a.hb_per_group;
+  const int row = blockIdx.y;
+  if (row >= min(a.rows, a.hpg - hb * a.rows)) return;
+  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)(w - 1) + 1 : 2 * (int64_t)(w - 1 + i); };
+  float m = -INFINITY;
+  for (int i = 0; i < pieces; ++i) m = fmaxf(m, a.ws_ml[slot(i) * a.rows + row].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) {
+    const float2 ml = a.ws_ml[slot(i) * a.rows + row];
+    const float4 o = reinterpret_cast<const float4*>(a.ws_o + (slot(i) * a.rows + row) * kNope)[threadIdx.x];
+    const float f = exp2f(ml.x - ref);
+    l += f * ml.y;
+    acc.x += f * o.x;
+    acc.y += f * o.y;
+    acc.z += f * o.z;
+    acc.w += f * o.w;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int64_t h = (int64_t)grp * a.hpg + hb * a.rows + row;
+  reinterpret_cast<uint2*>(a.out + t * a.out_st + h * a.out_sh)[threadIdx.x] =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (a.lse != nullptr && threadIdx.x == 0)
+    a.lse[t * a.lse_st + h] = l == 0.f ? -INFINITY : (m - bias) * kLn2 + logf(l);
+}
+
+}  // namespace
+
+int launch_merge_fp4(const Fp4DecodeArgs& a, float bias, cudaStream_t st) {
+  if (a.workers < 2) return FP8MLA_OK;
+  return check_cuda(launch_pdl(merge_fp4_kernel, dim3((unsigned)(a.workers - 1), (unsigned)a.rows), dim3(128), 0, st,
+                               a, bias),
+                    "merge_fp4_kernel launch");
+}
+
+int launch_decode_fp4(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st) {
+  CUtensorMap tm{};
+  if (a.num_slots > 0)
+    if (int rc = encode_fp4_row_map(&tm, a.kv, a.num_slots)) return rc;
+  const size_t smem = sizeof(Smem) + 128;
+  cudaError_t e = cudaFuncSetAttribute(decode_fp4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return check_cuda(e, "decode_fp4 smem attribute");
+  if (int rc = check_cuda(launch_pdl(decode_fp4_kernel, dim3((unsigned)a.workers), dim3(kThreads), smem, st, a, tm),
+                          "decode_fp4_kernel launch"))
+    return rc;
+  return cuts ? launch_merge_fp4(a, kBias, st) : FP8MLA_OK;
+}
+
+int decode_fp4_chunk() { return kBN; }
+
+int read_device_status_fp4(unsigned int* status, bool reset, cudaStream_t st) {
+  unsigned int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, tc::g_device_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && reset && v != 0) {
+    const unsigned int zero = 0;
+    e = cudaMemcpyToSymbolAsync(tc::g_device_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  *status = v;
+  return check_cuda(e, "device status read");
+}
+
+}  // namespace fp8mla

@@ -1,0 +1,57 @@
+// fp4.cuh -- the 4-bit MLA row (fp4_ds_mla) and its conversions.
+//
+// Row format (416 bytes per KV slot):
+//   [  0:256)  512 x e2m1          NoPE latent, element 2i in the low nibble of byte i
+//   [256:288)   32 x float8_e4m3fn one scale per 16 latent values
+//   [288:416)   64 x bfloat16      RoPE, raw
+// A latent value is code * scale.  e2m1 has 2 significant bits and e4m3 has 4,
+// so the product has at most 6 and lies in {0} u [2^-10, 2688] (a multiple of
+// 2^-10): exact in fp16 and in bf16, subnormal scales included.  The kernels
+// therefore feed the tensor cores fp16 latents without any rounding.
+#pragma once
+#include "common.cuh"
+
+namespace fp8mla {
+namespace fp4 {
+
+constexpr int kFp4Group = 16;                   // latent values per scale
+constexpr int kFp4CodeBytes = kNope / 2;        // 256
+constexpr int kFp4ScaleOff = kFp4CodeBytes;        // 256
+constexpr int kFp4RopeOff = kFp4ScaleOff + kNope / kFp4Group;  // 288
+constexpr int kFp4RowBytes = kFp4RopeOff + 2 * kRope;       // 416
+static_assert(kFp4RowBytes == FP8MLA_FP4_ROW_BYTES && kFp4ScaleOff == FP8MLA_FP4_SCALE_OFF &&
+                  kFp4RopeOff == FP8MLA_FP4_ROPE_OFF && kFp4RowBytes % 16 == 0,
+              "row geometry");
+
+// 8 e2m1 codes -> 4 f16x2, element 2b in the low half of h[b]
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}\n"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+// 2 e4m3 bytes (low 16 bits of w) -> f16x2
+__device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, l;\n}\n" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 2 exact fp16 products -> bf16x2 (exact: at most 6 significant bits)
+__device__ __forceinline__ uint32_t f16x2_to_bf16x2(uint32_t h) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack_bf16x2(f.x, f.y);
+}
+
+}  // namespace fp4
+}  // namespace fp8mla

@@ -23,11 +23,13 @@ EncodeTiledFn encode_fn() {
 }
 }  // namespace
 
-int encode_row_map(CUtensorMap* tm, const uint8_t* kv, int64_t num_slots, uint32_t box_u64) {
+namespace {
+// [num_slots] rows of row_u64 uint64, a one-row box of box_u64 words
+int encode_rows(CUtensorMap* tm, const uint8_t* kv, int64_t num_slots, uint32_t row_u64, uint32_t box_u64) {
   EncodeTiledFn enc = encode_fn();
   if (enc == nullptr) return set_error(FP8MLA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  const cuuint64_t dims[2] = {kRowBytes / 8, (cuuint64_t)num_slots};
-  const cuuint64_t strides[1] = {kRowBytes};
+  const cuuint64_t dims[2] = {row_u64, (cuuint64_t)num_slots};
+  const cuuint64_t strides[1] = {8 * (cuuint64_t)row_u64};
   const cuuint32_t box[2] = {box_u64, 1};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<uint8_t*>(kv), dims, strides,
@@ -35,6 +37,15 @@ int encode_row_map(CUtensorMap* tm, const uint8_t* kv, int64_t num_slots, uint32
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(FP8MLA_ERR_CUDA, "tensor map encode failed (%d)", (int)r);
   return FP8MLA_OK;
+}
+}  // namespace
+
+int encode_row_map(CUtensorMap* tm, const uint8_t* kv, int64_t num_slots, uint32_t box_u64) {
+  return encode_rows(tm, kv, num_slots, kRowBytes / 8, box_u64);
+}
+
+int encode_fp4_row_map(CUtensorMap* tm, const uint8_t* kv, int64_t num_slots) {
+  return encode_rows(tm, kv, num_slots, FP8MLA_FP4_ROW_BYTES / 8, FP8MLA_FP4_ROW_BYTES / 8);
 }
 
 int encode_indexer_page_map(CUtensorMap* tm, const uint8_t* k_cache, int64_t num_blocks,

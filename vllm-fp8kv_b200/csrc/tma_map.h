@@ -17,6 +17,10 @@ namespace fp8mla {
 // error code with the message recorded.
 int encode_row_map(CUtensorMap* tm, const uint8_t* kv, int64_t num_slots, uint32_t box_u64);
 
+// The same over fp4_ds_mla rows: [num_slots] rows of 52 uint64 (416 bytes), a
+// box is a whole row.
+int encode_fp4_row_map(CUtensorMap* tm, const uint8_t* kv, int64_t num_slots);
+
 // Encodes `tm` over the DSA indexer's paged key cache: blocks of block_size
 // tokens, each block_size x head_dim e4m3 bytes followed by block_size fp32
 // scales.  One box is one block's values (block_size rows of head_dim = 128

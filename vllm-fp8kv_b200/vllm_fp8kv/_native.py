@@ -64,6 +64,28 @@ SIGNATURES = {
         _P, _P, _I64, _I64,                    # context_lens, block_table, bt_stride, max_blocks
         _P, _I64, _I64, _P]),                  # logits, logits_stride, max_model_len, stream
     "fp8mla_indexer_topk": (_I32, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P]),
+    "fp8mla_fp4_write": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P]),
+    "fp8mla_fp4_dequant_rows": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P]),
+    "fp8mla_fp4_gather": (_I32, [_P, _I64, _P, _I64, _I64, _I64,  # kv, num_slots, block table, block_size
+                                 _P, _I64, _P, _I64, _P, _I64, _P]),
+    "fp8mla_fp4_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "fp8mla_fp4_kernel_name": (ctypes.c_char_p, [_I64, _I64]),
+    "fp8mla_fp4_sparse_decode": (_I32, [
+        _P, _I64, _I64, _I64, _I64,            # q, T, H, q strides
+        _P, _I64,                              # kv, num_slots
+        _P, _I64, _I64, _I64, _I64,            # indices, G, topk, idx strides
+        _F32, _P, _I64, _I64, _P, _I64,        # sm_scale, out, out strides, lse, lse stride
+        _P, _I64, _P]),                        # workspace, bytes, stream
+    "fp8mla_fp4_sparse_decode_paged": (_I32, [
+        _P, _I64, _I64, _I64, _I64, _P, _I64,  # q, T, H, q strides, kv, num_slots
+        _P, _P, _I64, _I64, _I64,              # req_id, block_table, bt stride, max_blocks, block_size
+        _P, _I64, _I64, _I64, _I64,            # token_idx, G, topk, token_idx strides
+        _F32, _P, _I64, _I64, _P, _I64, _P, _I64, _P]),
+    "fp8mla_fp4_decode": (_I32, [
+        _P, _I64, _I64, _I64, _I64, _P, _I64,  # q, T, H, q strides, kv, num_slots
+        _P, _P, _I64, _I64, _I64,              # req_id, block_table, bt stride, max_blocks, block_size
+        _P,                                    # context_lens
+        _F32, _P, _I64, _I64, _P, _I64, _P, _I64, _P]),
 }
 
 _lib = None

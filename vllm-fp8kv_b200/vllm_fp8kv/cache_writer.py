@@ -16,6 +16,7 @@ from __future__ import annotations
 import torch
 
 from vllm_fp8kv import _native as N
+from vllm_fp8kv.fp4_ds_mla import concat_and_cache_fp4_ds_mla
 
 ROW_BYTES = 656
 
@@ -43,7 +44,10 @@ def concat_and_cache_ds_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: to
 def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
                          slot_mapping: torch.Tensor, kv_cache_dtype: str,
                          scale: torch.Tensor | float | None = None) -> None:
-    """vLLM-signature wrapper; only the fp8_ds_mla format is implemented here."""
+    """vLLM-signature wrapper: the fp8_ds_mla format, and this library's fp4_ds_mla."""
+    if kv_cache_dtype == "fp4_ds_mla":
+        concat_and_cache_fp4_ds_mla(kv_c, k_pe, kv_cache, slot_mapping)
+        return
     if kv_cache_dtype != "fp8_ds_mla":
-        raise NotImplementedError(f"only fp8_ds_mla is implemented, got {kv_cache_dtype!r}")
+        raise NotImplementedError(f"only fp8_ds_mla and fp4_ds_mla are implemented, got {kv_cache_dtype!r}")
     concat_and_cache_ds_mla(kv_c, k_pe, kv_cache, slot_mapping)
