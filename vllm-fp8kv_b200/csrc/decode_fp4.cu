@@ -13,14 +13,16 @@
 //   * the rope (bf16 as stored) and q's rope (times the same power of two)
 //     go through bf16 MMAs into the same accumulators.
 //
-// Warp roles (512 threads, one of each kind per SM sub-partition but for PV):
-//   warps 0-3   S and softmax: warp w owns entries [16w, +16) of the chunk and
-//               holds all of q (16 heads x 576) as 144 registers of fragments;
-//               the four agree on the chunk's maxima through shared memory
-//   warps 4-11  O: warp w owns 64 of the 512 output dims
+// Warp roles (512 threads):
+//   warps 0-11  three groups of four.  A group takes every third chunk of a
+//               unit's piece on its own, with its own maximum, sum and O, so the
+//               three stand at different phases and fill each other's waits.
+//               Warp w of a group computes S of entries [16w, +16), then, behind
+//               the group's barrier, O of dims [128w, +128).  q (16 heads x 576,
+//               as A fragments) is read from shared memory, once per 16 entries.
+//               At the end of a piece the groups' results are joined.
 //   warps 12-15 producers: entries -> slots -> TMA copies of 16 rows each
-// The registers move between the warpgroups accordingly (setmaxnreg: 232, 104,
-// 104, 64; the launch holds 128 each).
+// The registers move from the producers to the others (setmaxnreg).
 #include "decode_fp4.h"
 #include "fp4.cuh"
 #include "tc_cluster.cuh"
@@ -34,10 +36,14 @@ using namespace fp8mla::tc;
 
 constexpr int kBH = 16;           // heads per unit
 constexpr int kBN = 64;           // entries per chunk
-constexpr int kStages = 7;
+constexpr int kStages = 6;
 constexpr int kStageBytes = kBN * kFp4RowBytes;  // 26624
-constexpr int kSWarps = 4, kOWarps = 8, kPWarps = 4;
-constexpr int kThreads = 32 * (kSWarps + kOWarps + kPWarps);
+constexpr int kGroups = 3, kGWarps = 4, kPWarps = 4;
+constexpr int kCWarps = kGroups * kGWarps;
+constexpr int kThreads = 32 * (kCWarps + kPWarps);
+constexpr int kCRegs = 152, kPRegs = 56;  // launched with 128 each
+static_assert(kCWarps * kCRegs + kPWarps * kPRegs <= (kCWarps + kPWarps) * 128, "register split");
+constexpr int kQSteps = kDqk / 16;        // 36: 32 of the latents, 4 of the rope
 constexpr int kRowsPerPWarp = kBN / kPWarps;  // 16
 constexpr float kRescale = 8.0f;  // the reference maximum lags by at most 2^8 ...
 constexpr float kBias = 6.0f;     // ... and P is stored times 2^6: below 2^14 in
@@ -45,19 +51,20 @@ constexpr float kBias = 6.0f;     // ... and P is stored times 2^6: below 2^14 i
 
 struct Smem {
   uint8_t raw[kStages][kStageBytes];   // 128-B aligned TMA destinations
-  uint32_t p[2][kSWarps][32][4];       // P as A fragments of the O product
-  float smax[2][kSWarps][kBH];
-  float alpha[2][kBH];
-  float fin[2][kBH][2];                // a piece's reference maximum and sum
-  float lpart[kSWarps][kBH];
-  uint32_t live[kStages][2];           // 16 bits per producer warp
+  uint32_t q[kQSteps][32][4];             // q as A fragments
+  float join[kGWarps][16][32][4];         // a group's O on its way to the next group
+  uint32_t p[kGroups][2][kBN / 16][32][4];  // P as A fragments of the O product
+  float smax[kGroups][2][kGWarps][kBH];
+  float lpart[kGroups][kGWarps][kBH];     // a piece's sums
+  float gm[kGroups][kBH], gl[kGroups][kBH];
+  float qscale[kBH];                      // score = qscale * accumulator (log2 units)
+  uint32_t live[kStages][2];              // 16 bits per producer warp
   uint64_t raw_full[kStages], raw_empty[kStages];
-  uint64_t p_full[2], p_empty[2], fin_full[2], fin_empty[2];
   int64_t tok_total, start_unit;
   int start_chunk;
   int64_t scan[kThreads / 32];
 };
-static_assert(offsetof(Smem, p) % 16 == 0 && offsetof(Smem, raw_full) % 8 == 0, "alignment");
+static_assert(offsetof(Smem, q) % 16 == 0 && offsetof(Smem, live) % 8 == 0 && offsetof(Smem, raw_full) % 8 == 0, "alignment");
 static_assert(sizeof(Smem) + 128 <= 227 * 1024, "shared memory budget");
 
 template <int kRegs>
@@ -73,6 +80,24 @@ __device__ __forceinline__ bool acquire(uint32_t bar, uint32_t parity, uint32_t 
   const bool ok = warp_wait(bar, parity, where);
   if (ok) (void)mbar_try_wait(bar, parity);
   return ok;
+}
+// Barriers: all compute warps (id 1), one group (id 2 + group), and the same
+// with an "any of us" vote.
+__device__ __forceinline__ void compute_sync() {
+  asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kCWarps) : "memory");
+}
+__device__ __forceinline__ void group_sync(int grp) {
+  asm volatile("bar.sync %0, %1;\n" ::"r"(2 + grp), "n"(32 * kGWarps) : "memory");
+}
+__device__ __forceinline__ bool group_any(int grp, bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, %2, %3, p;\n"
+      " selp.b32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)mine), "r"(2 + grp), "n"(32 * kGWarps)
+      : "memory");
+  return r != 0;
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -152,6 +177,19 @@ __device__ int64_t divide_work(const Fp4DecodeArgs& a, Smem& s) {
   return per;
 }
 
+// Place in the ring of stages: the stage, and the parity of its current round.
+struct Ring {
+  int st = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void ahead(int n) {  // 0 <= n <= kStages
+    st += n;
+    if (st >= kStages) {
+      st -= kStages;
+      ph ^= 1;
+    }
+  }
+};
+
 // A worker's chunks in order.
 struct Walk {
   Fp4Cursor x;
@@ -211,14 +249,15 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
   int32_t pg0 = fp4_table(a, e0.req, e0.v);
   bool ok = true;
   int64_t armed = 0;
-  for (int64_t g = 0; g < chunks; ++g) {
+  Ring ring;
+  for (int64_t g = 0; g < chunks; ++g, ring.ahead(1)) {
     const int32_t slot = fp4_slot(a, e0.v, pg0);
     const Entry e2 = fetch();
     pg0 = fp4_table(a, e1.req, e1.v);
     e0 = e1;
     e1 = e2;
-    const int st = (int)(g % kStages);
-    if (g >= kStages) ok = warp_wait(smem_u32(&s.raw_empty[st]), (uint32_t)(g / kStages + 1) & 1, 20);
+    const int st = ring.st;
+    if (g >= kStages) ok = warp_wait(smem_u32(&s.raw_empty[st]), ring.ph ^ 1, 20);
     if (!ok) break;
     const uint32_t live = __ballot_sync(0xFFFFFFFFu, slot >= 0) & 0xFFFFu;
     const int n = __popc(live);
@@ -253,325 +292,361 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
     (void)warp_wait(smem_u32(&s.raw_full[x % kStages]), (uint32_t)(x / kStages) & 1, 26);
 }
 
-// ------------------------------------------------------------------ S and softmax
+// ------------------------------------------------------------------ compute
 // Fragment coordinates: lane = 4 gq + q4.  Thread q4 of a quad owns latent
 // dims [128 q4, +128) of a row and rope dims [16 q4, +16); it walks its four
 // 32-dim pieces in the order i ^ (q4 >> 1) and its two rope halves in the order
 // h ^ (q4 & 1), so that 8 lanes' 16-byte loads cover all banks.  q's fragments
-// follow the same order.
-struct QFrag {
-  uint32_t a[36][4];
-  float scale[2];  // heads gq, gq + 8: score = scale * accumulator (log2 units)
-};
-__device__ __forceinline__ void load_q(const Fp4DecodeArgs& a, QFrag& f, const Fp4Cursor& x, int gq, int q4) {
-  const int h0 = x.grp * a.hpg + x.hb * kBH;
-  const int nh = min(kBH, a.hpg - x.hb * kBH);
+// follow the same order: k-step 8 i + 2 j (+ 1) of piece i holds dims 8 j, .. + 3
+// (+ 4, .. + 7) of it, k-step 32 + 2 h (+ 1) the same of rope half h.
+
+// q of the unit -> fragments in shared memory.  A half-warp owns a head, lane
+// j of it dims [32 j, +32) and rope dims [4 j, +4).
+__device__ void load_q(const Fp4DecodeArgs& a, Smem& s, const Fp4Cursor& x, int cw, int lane) {
+  if (cw >= kBH / 2) return;
+  const int row = 2 * cw + (lane >> 4), j16 = lane & 15;
+  const bool hv = row < min(kBH, a.hpg - x.hb * kBH);
+  const uint16_t* src = a.q + x.t * a.q_st + (int64_t)(x.grp * a.hpg + x.hb * kBH + (hv ? row : 0)) * a.q_sh;
+  const uint4 z4 = make_uint4(0, 0, 0, 0);
+  uint4 v[4];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = gq + 8 * r;
-    const bool hv = row < nh;
-    const uint16_t* src = a.q + x.t * a.q_st + (int64_t)(h0 + (hv ? row : 0)) * a.q_sh;
-    uint32_t mx = 0;
+  for (int j = 0; j < 4; ++j) v[j] = hv ? reinterpret_cast<const uint4*>(src + 32 * j16)[j] : z4;
+  const uint2 rp = hv ? *reinterpret_cast<const uint2*>(src + kNope + 4 * j16) : make_uint2(0, 0);
+  uint32_t mx = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4* p = reinterpret_cast<const uint4*>(src + 128 * q4 + 32 * (i ^ (q4 >> 1)));
+  for (int j = 0; j < 4; ++j)
+    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(v[j].x & 0x7FFF7FFFu, v[j].y & 0x7FFF7FFFu),
+                               __vmaxu2(v[j].z & 0x7FFF7FFFu, v[j].w & 0x7FFF7FFFu)));
+  const uint32_t mxr = __vmaxu2(rp.x & 0x7FFF7FFFu, rp.y & 0x7FFF7FFFu);
+  // largest magnitudes (as bits) of the head's latent part and of its rope
+  uint32_t m = max(mx & 0xFFFFu, mx >> 16), mr = max(mxr & 0xFFFFu, mxr >> 16);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // 8 dims: k-steps 8i + 2j and 8i + 2j + 1
-        const uint4 v = hv ? p[j] : make_uint4(0, 0, 0, 0);
-        f.a[8 * i + 2 * j][r] = v.x;
-        f.a[8 * i + 2 * j][2 + r] = v.y;
-        f.a[8 * i + 2 * j + 1][r] = v.z;
-        f.a[8 * i + 2 * j + 1][2 + r] = v.w;
-        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
-                                   __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
-      }
+  for (int o = 1; o < 16; o <<= 1) {
+    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    mr = max(mr, __shfl_xor_sync(0xFFFFFFFFu, mr, o));
+  }
+  // 2^k brings the latent part's largest value to [2^8, 2^9), but the rope's
+  // at most to 2^101, where its products are still finite; 1 for rows of
+  // zeros, inf or NaN.  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are
+  // normal.
+  int k = min(8 - ((int)(m >> 7) - 127), 100 - ((int)(mr >> 7) - 127));
+  k = (m == 0 || m >= 0x7F80u) ? 0 : min(126, k);
+  const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+  if (j16 == 0) s.qscale[row] = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+  const int r = row >> 3, gq = row & 7;
+  {
+    const int q4 = j16 >> 2, i = (j16 & 3) ^ (q4 >> 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t* f0 = s.q[8 * i + 2 * j][4 * gq + q4];
+      uint32_t* f1 = s.q[8 * i + 2 * j + 1][4 * gq + q4];
+      f0[r] = pack_f16x2(bf16_lo(v[j].x) * up, bf16_hi(v[j].x) * up);
+      f0[2 + r] = pack_f16x2(bf16_lo(v[j].y) * up, bf16_hi(v[j].y) * up);
+      f1[r] = pack_f16x2(bf16_lo(v[j].z) * up, bf16_hi(v[j].z) * up);
+      f1[2 + r] = pack_f16x2(bf16_lo(v[j].w) * up, bf16_hi(v[j].w) * up);
     }
-    uint32_t mxr = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 v = hv ? *reinterpret_cast<const uint4*>(src + kNope + 16 * q4 + 8 * (h ^ (q4 & 1)))
-                         : make_uint4(0, 0, 0, 0);
-      f.a[32 + 2 * h][r] = v.x;
-      f.a[32 + 2 * h][2 + r] = v.y;
-      f.a[32 + 2 * h + 1][r] = v.z;
-      f.a[32 + 2 * h + 1][2 + r] = v.w;
-      mxr = __vmaxu2(mxr, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
-                                   __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
-    }
-    // largest magnitudes (as bits) of the head's latent part and of its rope
-    uint32_t m = max(mx & 0xFFFFu, mx >> 16), mr = max(mxr & 0xFFFFu, mxr >> 16);
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-      mr = max(mr, __shfl_xor_sync(0xFFFFFFFFu, mr, o));
-    }
-    // 2^k brings the latent part's largest value to [2^8, 2^9), but the rope's
-    // at most to 2^101, where its products are still finite; 1 for rows of
-    // zeros, inf or NaN.  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are
-    // normal.
-    int k = min(8 - ((int)(m >> 7) - 127), 100 - ((int)(mr >> 7) - 127));
-    k = (m == 0 || m >= 0x7F80u) ? 0 : min(126, k);
-    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-    f.scale[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      f.a[i][r] = pack_f16x2(bf16_lo(f.a[i][r]) * up, bf16_hi(f.a[i][r]) * up);
-      f.a[i][2 + r] = pack_f16x2(bf16_lo(f.a[i][2 + r]) * up, bf16_hi(f.a[i][2 + r]) * up);
-    }
-#pragma unroll
-    for (int i = 32; i < 36; ++i) {
-      f.a[i][r] = pack_bf16x2(bf16_lo(f.a[i][r]) * up, bf16_hi(f.a[i][r]) * up);
-      f.a[i][2 + r] = pack_bf16x2(bf16_lo(f.a[i][2 + r]) * up, bf16_hi(f.a[i][2 + r]) * up);
-    }
+  }
+  {
+    // rope dims 4 j16 .. + 3: quad thread j16 / 4, 8-dim half (j16 / 2) % 2, k-step j16 % 2 of it
+    const int q4 = j16 >> 2, h = ((j16 >> 1) & 1) ^ (q4 & 1);
+    uint32_t* f = s.q[32 + 2 * h + (j16 & 1)][4 * gq + q4];
+    f[r] = pack_bf16x2(bf16_lo(rp.x) * up, bf16_hi(rp.x) * up);
+    f[2 + r] = pack_bf16x2(bf16_lo(rp.y) * up, bf16_hi(rp.y) * up);
   }
 }
 
-// Accumulators of 8 entries: the row at `row` (this lane's column gq).
-__device__ __forceinline__ void score_tile(const QFrag& f, const uint8_t* row, int q4, float (&acc)[4]) {
-  float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
-  float c2[4] = {0.f, 0.f, 0.f, 0.f}, c3[4] = {0.f, 0.f, 0.f, 0.f};
-  uint2 sc = *reinterpret_cast<const uint2*>(row + kFp4ScaleOff + 8 * q4);
-  const uint32_t sel = (q4 >> 1) ? 0x1032u : 0x3210u;
-  sc.x = __byte_perm(sc.x, 0, sel);
-  sc.y = __byte_perm(sc.y, 0, sel);
+// Accumulators of 16 entries (two tiles of 8, their rows 8 apart): row is this
+// lane's column gq of the first.
+__device__ __forceinline__ void score_tiles(const uint32_t (*q)[32][4], const uint8_t* row, int lane,
+                                            float (&x)[2][4]) {
+  const int q4 = lane & 3;
+  float c0[2][4], c1[2][4];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c0[t][i] = c1[t][i] = 0.f;
+  uint32_t sc[2][2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint2 v = *reinterpret_cast<const uint2*>(row + t * 8 * kFp4RowBytes + kFp4ScaleOff + 8 * q4);
+    const uint32_t sel = (q4 >> 1) ? 0x1032u : 0x3210u;
+    sc[t][0] = __byte_perm(v.x, 0, sel);
+    sc[t][1] = __byte_perm(v.y, 0, sel);
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 w = *reinterpret_cast<const uint4*>(row + 64 * q4 + 16 * (i ^ (q4 >> 1)));
-    const uint32_t sw = i < 2 ? sc.x : sc.y;
-    const uint32_t s2 = e4m3x2_to_f16((i & 1) ? sw >> 16 : sw);
-    const uint32_t s_lo = __byte_perm(s2, 0, 0x1010), s_hi = __byte_perm(s2, 0, 0x3232);
-    uint32_t h[4];
-    e2m1x8_to_f16(w.x, h);
-    mma_f16(c0, f.a[8 * i], mul_f16x2(h[0], s_lo), mul_f16x2(h[1], s_lo));
-    mma_f16(c1, f.a[8 * i + 1], mul_f16x2(h[2], s_lo), mul_f16x2(h[3], s_lo));
-    e2m1x8_to_f16(w.y, h);
-    mma_f16(c2, f.a[8 * i + 2], mul_f16x2(h[0], s_lo), mul_f16x2(h[1], s_lo));
-    mma_f16(c3, f.a[8 * i + 3], mul_f16x2(h[2], s_lo), mul_f16x2(h[3], s_lo));
-    e2m1x8_to_f16(w.z, h);
-    mma_f16(c0, f.a[8 * i + 4], mul_f16x2(h[0], s_hi), mul_f16x2(h[1], s_hi));
-    mma_f16(c1, f.a[8 * i + 5], mul_f16x2(h[2], s_hi), mul_f16x2(h[3], s_hi));
-    e2m1x8_to_f16(w.w, h);
-    mma_f16(c2, f.a[8 * i + 6], mul_f16x2(h[0], s_hi), mul_f16x2(h[1], s_hi));
-    mma_f16(c3, f.a[8 * i + 7], mul_f16x2(h[2], s_hi), mul_f16x2(h[3], s_hi));
+    uint4 w[2];
+    uint32_t s_lo[2], s_hi[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      w[t] = *reinterpret_cast<const uint4*>(row + t * 8 * kFp4RowBytes + 64 * q4 + 16 * (i ^ (q4 >> 1)));
+      const uint32_t s2 = e4m3x2_to_f16((i & 1) ? sc[t][i >> 1] >> 16 : sc[t][i >> 1]);
+      s_lo[t] = __byte_perm(s2, 0, 0x1010);
+      s_hi[t] = __byte_perm(s2, 0, 0x3232);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 a0 = *reinterpret_cast<const uint4*>(q[8 * i + 2 * j][lane]);
+      const uint4 a1 = *reinterpret_cast<const uint4*>(q[8 * i + 2 * j + 1][lane]);
+      const uint32_t f0[4] = {a0.x, a0.y, a0.z, a0.w}, f1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        uint32_t h[4];
+        e2m1x8_to_f16(j == 0 ? w[t].x : j == 1 ? w[t].y : j == 2 ? w[t].z : w[t].w, h);
+        const uint32_t sj = j < 2 ? s_lo[t] : s_hi[t];
+        mma_f16(c0[t], f0, mul_f16x2(h[0], sj), mul_f16x2(h[1], sj));
+        mma_f16(c1[t], f1, mul_f16x2(h[2], sj), mul_f16x2(h[3], sj));
+      }
+    }
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint4 w = *reinterpret_cast<const uint4*>(row + kFp4RopeOff + 32 * q4 + 16 * (h ^ (q4 & 1)));
-    const uint32_t(&a0)[4] = f.a[32 + 2 * h];
-    const uint32_t(&a1)[4] = f.a[32 + 2 * h + 1];
-    mma_bf16_16816(h == 0 ? c0 : c2, a0[0], a0[1], a0[2], a0[3], w.x, w.y);
-    mma_bf16_16816(h == 0 ? c1 : c3, a1[0], a1[1], a1[2], a1[3], w.z, w.w);
+    const uint4 a0 = *reinterpret_cast<const uint4*>(q[32 + 2 * h][lane]);
+    const uint4 a1 = *reinterpret_cast<const uint4*>(q[33 + 2 * h][lane]);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row + t * 8 * kFp4RowBytes + kFp4RopeOff + 32 * q4 +
+                                                      16 * (h ^ (q4 & 1)));
+      mma_bf16_16816(c0[t], a0.x, a0.y, a0.z, a0.w, w.x, w.y);
+      mma_bf16_16816(c1[t], a1.x, a1.y, a1.z, a1.w, w.z, w.w);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] = (c0[i] + c1[i]) + (c2[i] + c3[i]);
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[t][i] = c0[t][i] + c1[t][i];
 }
 
-__device__ void scores(const Fp4DecodeArgs& a, Smem& s, int64_t per, int sw, int lane) {
+// O += P V of one chunk over this warp's 128 dims.  A thread owns 16 of them (one scale
+// group): code_at, scale_at name it within a row.
+__device__ __forceinline__ void output_step(const uint8_t* raw, const uint32_t (*p)[32][4], uint64_t live, int lane,
+                                            int code_at, int scale_at, int ra, int rb, float (&acc)[16][4]) {
+#pragma unroll
+  for (int kk = 0; kk < kBN / 16; ++kk) {
+    const uint4 pv = *reinterpret_cast<const uint4*>(p[kk][lane]);
+    const uint32_t pa[4] = {pv.x, pv.y, pv.z, pv.w};
+    const uint8_t* r0 = raw + (16 * kk + ra) * kFp4RowBytes;
+    const uint8_t* r1 = raw + (16 * kk + rb) * kFp4RowBytes;
+    const uint2 w0 = *reinterpret_cast<const uint2*>(r0 + code_at);
+    const uint2 w1 = *reinterpret_cast<const uint2*>(r1 + code_at);
+    const uint2 w2 = *reinterpret_cast<const uint2*>(r0 + 8 * kFp4RowBytes + code_at);
+    const uint2 w3 = *reinterpret_cast<const uint2*>(r1 + 8 * kFp4RowBytes + code_at);
+    uint32_t b0 = r0[scale_at], b1 = r1[scale_at];
+    uint32_t b2 = r0[8 * kFp4RowBytes + scale_at], b3 = r1[8 * kFp4RowBytes + scale_at];
+    if (live != ~0ull) {  // P is 0 there, but a NaN scale would still spread
+      const uint32_t lv = (uint32_t)(live >> (16 * kk));
+      b0 = (lv >> ra) & 1u ? b0 : 0u;
+      b1 = (lv >> rb) & 1u ? b1 : 0u;
+      b2 = (lv >> (ra + 8)) & 1u ? b2 : 0u;
+      b3 = (lv >> (rb + 8)) & 1u ? b3 : 0u;
+    }
+    const uint32_t s01 = e4m3x2_to_f16(b0 | (b1 << 8)), s23 = e4m3x2_to_f16(b2 | (b3 << 8));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // 8 of the thread's dims
+      const uint32_t c0 = h ? w0.y : w0.x, c1 = h ? w1.y : w1.x, c2 = h ? w2.y : w2.x, c3 = h ? w3.y : w3.x;
+      // nibble pairs (row of the even k index low, of the odd one high): even
+      // dims, then odd dims
+      uint32_t e01[4], e23[4];
+      e2m1x8_to_f16((c0 & 0x0F0F0F0Fu) | ((c1 << 4) & 0xF0F0F0F0u), e01);
+      e2m1x8_to_f16((c2 & 0x0F0F0F0Fu) | ((c3 << 4) & 0xF0F0F0F0u), e23);
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        mma_f16(acc[8 * h + 2 * b], pa, mul_f16x2(e01[b], s01), mul_f16x2(e23[b], s23));
+      e2m1x8_to_f16(((c0 >> 4) & 0x0F0F0F0Fu) | (c1 & 0xF0F0F0F0u), e01);
+      e2m1x8_to_f16(((c2 >> 4) & 0x0F0F0F0Fu) | (c3 & 0xF0F0F0F0u), e23);
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        mma_f16(acc[8 * h + 2 * b + 1], pa, mul_f16x2(e01[b], s01), mul_f16x2(e23[b], s23));
+    }
+  }
+}
+
+__device__ void compute(const Fp4DecodeArgs& a, Smem& s, int64_t per, int cw, int lane) {
   const int gq = lane >> 2, q4 = lane & 3;
+  const int grp = cw / kGWarps, gw = cw % kGWarps;
   Walk w(a, s, per);
-  int64_t g = 0;
-  int piece = 0;
+  int pb = 0;
+  Ring piece_at;  // stage of the piece's first chunk
   bool ok = true;
-  const int rowb = (gq & 1) ? row_odd(gq >> 1) : row_even(gq >> 1);
-  const int re = row_even(q4), ro = row_odd(q4);
+  const int ra = row_even(q4), rb = row_odd(q4);  // rows of k indices 2 q4, 2 q4 + 1
+  const uint32_t tile_at = (16 * gw + ((gq & 1) ? row_odd(gq >> 1) : row_even(gq >> 1))) * kFp4RowBytes;
+  const int code_at = 64 * gw + 8 * gq, scale_at = kFp4ScaleOff + 8 * gw + gq;
   while (w.left > 0) {
     const int nch = w.here();
-    QFrag f;
-    load_q(a, f, w.x, gq, q4);
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int c = 0; c < nch; ++c, ++g) {
-      const int st = (int)(g % kStages), pb = (int)(g & 1);
-      if (ok) ok = acquire(smem_u32(&s.raw_full[st]), (uint32_t)(g / kStages) & 1, 21);
-      const uint32_t live = s.live[st][sw >> 1] >> (16 * (sw & 1));
-      const uint8_t* base = s.raw[st] + (16 * sw + rowb) * kFp4RowBytes;
-      float x[2][4];
-      score_tile(f, base, q4, x[0]);
-      score_tile(f, base + 8 * kFp4RowBytes, q4, x[1]);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.raw_empty[st]));
-      // masked entries to -inf; maxima of heads gq and gq + 8
-      float mt[2] = {-INFINITY, -INFINITY};
+    load_q(a, s, w.x, cw, lane);
+    compute_sync();
+    float acc[16][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const bool le = (live >> (8 * nt + re)) & 1u, lo = (live >> (8 * nt + ro)) & 1u;
+    for (int i = 0; i < 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const float qs[2] = {s.qscale[gq], s.qscale[gq + 8]};
+    Ring ring = piece_at;
+    ring.ahead(grp);
+    for (int c = grp; c < nch; c += kGroups) {
+      if (ok) ok = acquire(smem_u32(&s.raw_full[ring.st]), ring.ph, 21);
+      const uint64_t live = *reinterpret_cast<const uint64_t*>(s.live[ring.st]);
+      const uint8_t* raw = s.raw[ring.st];
+      float x[2][4];
+      score_tiles(s.q, raw + tile_at, lane, x);
+      // scores in log2 units, masked ones -inf, and this warp's maxima
+      const uint32_t lv = (uint32_t)(live >> (16 * gw));
+      bool grown = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          x[t][2 * r] = (lv >> (8 * t + ra)) & 1u ? x[t][2 * r] * qs[r] : -INFINITY;
+          x[t][2 * r + 1] = (lv >> (8 * t + rb)) & 1u ? x[t][2 * r + 1] * qs[r] : -INFINITY;
+          mt = fmaxf(mt, fmaxf(x[t][2 * r], x[t][2 * r + 1]));
+        }
+        mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 1));
+        mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 2));
+        if (q4 == 0) s.smax[grp][pb][gw][gq + 8 * r] = mt;
+        grown |= mt > m[r] + kRescale;
+      }
+      // P against the reference maximum so far
+      float p[2][4];
+      auto exps = [&]() {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          x[nt][2 * r] = le ? x[nt][2 * r] * f.scale[r] : -INFINITY;
-          x[nt][2 * r + 1] = lo ? x[nt][2 * r + 1] * f.scale[r] : -INFINITY;
-          mt[r] = fmaxf(mt[r], fmaxf(x[nt][2 * r], x[nt][2 * r + 1]));
+          const float sub = m[r] == -INFINITY ? 0.f : m[r] - kBias;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            p[t][2 * r] = ex2_approx(x[t][2 * r] - sub);
+            p[t][2 * r + 1] = ex2_approx(x[t][2 * r + 1] - sub);
+          }
         }
-      }
+        *reinterpret_cast<uint4*>(s.p[grp][pb][gw][lane]) =
+            make_uint4(pack_f16x2(p[0][0], p[0][1]), pack_f16x2(p[0][2], p[0][3]), pack_f16x2(p[1][0], p[1][1]),
+                       pack_f16x2(p[1][2], p[1][3]));
+      };
+      exps();
+      // The group's barrier: P is in place.  Where a maximum has outgrown the
+      // reference (the first chunk, seldom later) all take the chunk's maximum.
+      if (group_any(grp, grown)) {
+        float al[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xFFFFFFFFu, mt[r], 1));
-        mt[r] = fmaxf(mt[r], __shfl_xor_sync(0xFFFFFFFFu, mt[r], 2));
-        if (q4 == 0) s.smax[pb][sw][gq + 8 * r] = mt[r];
-      }
-      named_sync(1, 32 * kSWarps);
-      float al[2];
+        for (int r = 0; r < 2; ++r) {
+          float tm = m[r];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int h = gq + 8 * r;
-        const float tm = fmaxf(fmaxf(s.smax[pb][0][h], s.smax[pb][1][h]), fmaxf(s.smax[pb][2][h], s.smax[pb][3][h]));
-        al[r] = 1.f;
-        if (tm > m[r] + kRescale || (m[r] == -INFINITY && tm > -INFINITY)) {
+          for (int i = 0; i < kGWarps; ++i) tm = fmaxf(tm, s.smax[grp][pb][i][gq + 8 * r]);
           al[r] = m[r] == -INFINITY ? 0.f : ex2_approx(m[r] - tm);
           m[r] = tm;
+          l[r] *= al[r];
         }
-        l[r] *= al[r];
-        const float sub = m[r] == -INFINITY ? 0.f : m[r] - kBias;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          x[nt][2 * r] = ex2_approx(x[nt][2 * r] - sub);
-          x[nt][2 * r + 1] = ex2_approx(x[nt][2 * r + 1] - sub);
-          l[r] += x[nt][2 * r] + x[nt][2 * r + 1];
+        for (int i = 0; i < 16; ++i) {
+          acc[i][0] *= al[0];
+          acc[i][1] *= al[0];
+          acc[i][2] *= al[1];
+          acc[i][3] *= al[1];
         }
+        exps();
+        group_sync(grp);
       }
-      if (ok && g >= 2) ok = warp_wait(smem_u32(&s.p_empty[pb]), (uint32_t)(g / 2 + 1) & 1, 22);
-      *reinterpret_cast<uint4*>(s.p[pb][sw][lane]) =
-          make_uint4(pack_f16x2(x[0][0], x[0][1]), pack_f16x2(x[0][2], x[0][3]), pack_f16x2(x[1][0], x[1][1]),
-                     pack_f16x2(x[1][2], x[1][3]));
-      if (sw == 0 && q4 == 0) {
-        s.alpha[pb][gq] = al[0];
-        s.alpha[pb][gq + 8] = al[1];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        l[0] += p[t][0] + p[t][1];
+        l[1] += p[t][2] + p[t][3];
       }
+      output_step(raw, s.p[grp][pb], live, lane, code_at, scale_at, ra, rb, acc);
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.p_full[pb]));
+      if (lane == 0) mbar_arrive(smem_u32(&s.raw_empty[ring.st]));
+      ring.ahead(kGroups);
+      pb ^= 1;
     }
-    // ---- the piece's sums
+    piece_at.ahead(nch % kStages);
+    if ((nch / kStages) & 1) piece_at.ph ^= 1;
+
+    // ---- join the groups: maxima and sums, then O from the last group to the first
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
       l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
-      if (q4 == 0) s.lpart[sw][gq + 8 * r] = l[r];
+      if (q4 == 0) s.lpart[grp][gw][gq + 8 * r] = l[r];
+      if (gw == 0 && q4 == 0) s.gm[grp][gq + 8 * r] = m[r];
     }
-    named_sync(1, 32 * kSWarps);
-    const int fb = piece & 1;
-    if (ok && piece >= 2) ok = warp_wait(smem_u32(&s.fin_empty[fb]), (uint32_t)(piece / 2 + 1) & 1, 23);
-    if (sw == 0 && q4 == 0) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int h = gq + 8 * r;
-        s.fin[fb][h][0] = m[r];
-        s.fin[fb][h][1] = (s.lpart[0][h] + s.lpart[1][h]) + (s.lpart[2][h] + s.lpart[3][h]);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&s.fin_full[fb]));
-    // (lpart is written again only after the next chunk's barrier)
-    ++piece;
-    w.next_unit(a, nch);
-  }
-}
-
-// ------------------------------------------------------------------ O
-__device__ void outputs(const Fp4DecodeArgs& a, Smem& s, int64_t per, int ow, int lane) {
-  const int gq = lane >> 2, q4 = lane & 3;
-  Walk w(a, s, per);
-  int64_t g = 0;
-  int piece = 0;
-  bool ok = true;
-  // rows of k indices 2 q4, 2 q4 + 1, + 8, + 9 of a 16-entry step
-  const int ra = row_even(q4), rb = row_odd(q4);
-  const int code_at = 32 * ow + 4 * gq, scale_at = kFp4ScaleOff + 4 * ow + (gq >> 1);
-  while (w.left > 0) {
-    const int nch = w.here();
-    float acc[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    for (int c = 0; c < nch; ++c, ++g) {
-      const int st = (int)(g % kStages), pb = (int)(g & 1);
-      if (ok) ok = acquire(smem_u32(&s.p_full[pb]), (uint32_t)(g / 2) & 1, 24);
-      if (ok) ok = acquire(smem_u32(&s.raw_full[st]), (uint32_t)(g / kStages) & 1, 27);
-      const float al0 = s.alpha[pb][gq], al1 = s.alpha[pb][gq + 8];
-      if (__any_sync(0xFFFFFFFFu, al0 != 1.f || al1 != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          acc[i][0] *= al0;
-          acc[i][1] *= al0;
-          acc[i][2] *= al1;
-          acc[i][3] *= al1;
-        }
-      }
-      const uint64_t live = *reinterpret_cast<const uint64_t*>(s.live[st]);
-      const uint8_t* raw = s.raw[st];
-#pragma unroll
-      for (int kk = 0; kk < kBN / 16; ++kk) {
-        const uint4 pv = *reinterpret_cast<const uint4*>(s.p[pb][kk][lane]);
-        const uint32_t pa[4] = {pv.x, pv.y, pv.z, pv.w};
-        const uint8_t* r0 = raw + (16 * kk + ra) * kFp4RowBytes;
-        const uint8_t* r1 = raw + (16 * kk + rb) * kFp4RowBytes;
-        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(r0 + code_at);
-        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(r1 + code_at);
-        const uint32_t w2 = *reinterpret_cast<const uint32_t*>(r0 + 8 * kFp4RowBytes + code_at);
-        const uint32_t w3 = *reinterpret_cast<const uint32_t*>(r1 + 8 * kFp4RowBytes + code_at);
-        uint32_t b0 = r0[scale_at], b1 = r1[scale_at];
-        uint32_t b2 = r0[8 * kFp4RowBytes + scale_at], b3 = r1[8 * kFp4RowBytes + scale_at];
-        if (live != ~0ull) {  // P is 0 there, but a NaN scale would still spread
-          const uint32_t lv = (uint32_t)(live >> (16 * kk));
-          b0 = (lv >> ra) & 1u ? b0 : 0u;
-          b1 = (lv >> rb) & 1u ? b1 : 0u;
-          b2 = (lv >> (ra + 8)) & 1u ? b2 : 0u;
-          b3 = (lv >> (rb + 8)) & 1u ? b3 : 0u;
-        }
-        const uint32_t s01 = e4m3x2_to_f16(b0 | (b1 << 8)), s23 = e4m3x2_to_f16(b2 | (b3 << 8));
-        // nibble pairs (row of the even k index low, of the odd one high):
-        // even dims, then odd dims of this thread's eight
-        uint32_t e01[4], e23[4];
-        e2m1x8_to_f16((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), e01);
-        e2m1x8_to_f16((w2 & 0x0F0F0F0Fu) | ((w3 << 4) & 0xF0F0F0F0u), e23);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) mma_f16(acc[2 * b], pa, mul_f16x2(e01[b], s01), mul_f16x2(e23[b], s23));
-        e2m1x8_to_f16(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), e01);
-        e2m1x8_to_f16(((w2 >> 4) & 0x0F0F0F0Fu) | (w3 & 0xF0F0F0F0u), e23);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) mma_f16(acc[2 * b + 1], pa, mul_f16x2(e01[b], s01), mul_f16x2(e23[b], s23));
-      }
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&s.raw_empty[st]));
-        mbar_arrive(smem_u32(&s.p_empty[pb]));
-      }
-    }
-    // ---- the piece: a whole unit goes to the output, a cut one to its slot
-    const int fb = piece & 1;
-    if (ok) ok = acquire(smem_u32(&s.fin_full[fb]), (uint32_t)(piece / 2) & 1, 25);
-    const bool whole = w.x.c == 0 && nch == w.x.n;
-    const int h0 = w.x.grp * a.hpg + w.x.hb * kBH;
-    const int nh = min(kBH, a.hpg - w.x.hb * kBH);
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (w.x.c == 0 ? 1 : 0);
+    compute_sync();
+    float mm[2], lt[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = gq + 8 * r;
-      if (row >= nh) continue;
-      const float m = s.fin[fb][row][0], l = s.fin[fb][row][1];
-      const int d = 64 * ow + 16 * q4;
-      if (whole) {
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        uint16_t* o = a.out + w.x.t * a.out_st + (int64_t)(h0 + row) * a.out_sh + d;
+      const int h = gq + 8 * r;
+      mm[r] = fmaxf(fmaxf(s.gm[0][h], s.gm[1][h]), s.gm[2][h]);
+      const float ref = mm[r] == -INFINITY ? 0.f : mm[r];
+      lt[r] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t v[4];
+      for (int i = 0; i < kGroups; ++i) {
+        float li = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(acc[2 * i][2 * r + j] * inv, acc[2 * i + 1][2 * r + j] * inv);
-          reinterpret_cast<uint4*>(o)[j] = make_uint4(v[0], v[1], v[2], v[3]);
+        for (int k = 0; k < kGWarps; ++k) li += s.lpart[i][k][h];
+        lt[r] += li == 0.f ? 0.f : li * ex2_approx(s.gm[i][h] - ref);
+      }
+      const float f = m[r] == -INFINITY ? 0.f : ex2_approx(m[r] - ref);
+      if (m[r] != -INFINITY || l[r] != 0.f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          acc[i][2 * r] *= f;
+          acc[i][2 * r + 1] *= f;
         }
-        if (a.lse != nullptr && ow == 0 && q4 == 0)
-          a.lse[w.x.t * a.lse_st + h0 + row] = l == 0.f ? -INFINITY : (m - kBias) * kLn2 + logf(l);
-      } else {
-        float4* o = reinterpret_cast<float4*>(a.ws_o + (slot * kBH + row) * kNope + d);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            o[2 * j + i] = make_float4(acc[4 * i][2 * r + j], acc[4 * i + 1][2 * r + j], acc[4 * i + 2][2 * r + j],
-                                       acc[4 * i + 3][2 * r + j]);
-        if (ow == 0 && q4 == 0) a.ws_ml[slot * kBH + row] = make_float2(m, l);
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&s.fin_empty[fb]));
-    ++piece;
+#pragma unroll
+    for (int g = kGroups - 1; g >= 0; --g) {
+      if (grp == g) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float4* at = reinterpret_cast<float4*>(s.join[gw][i][lane]);
+          if (g < kGroups - 1) {
+            const float4 o = *at;
+            acc[i][0] += o.x;
+            acc[i][1] += o.y;
+            acc[i][2] += o.z;
+            acc[i][3] += o.w;
+          }
+          if (g > 0) *at = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+        }
+      }
+      if (g > 0) compute_sync();
+    }
+    // ---- the piece: a whole unit goes to the output, a cut one to its slot
+    if (grp == 0) {
+      const bool whole = w.x.c == 0 && nch == w.x.n;
+      const int h0 = w.x.grp * a.hpg + w.x.hb * kBH;
+      const int nh = min(kBH, a.hpg - w.x.hb * kBH);
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (w.x.c == 0 ? 1 : 0);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = gq + 8 * r;
+        if (row >= nh) continue;
+        // column 2 q4 + j of the 16 tiles: the 16 dims of thread gq = 2 q4 + j
+        const int d = 128 * gw + 32 * q4;
+        if (whole) {
+          const float inv = lt[r] > 0.f ? 1.f / lt[r] : (lt[r] == 0.f ? 0.f : lt[r]);
+          uint4* o = reinterpret_cast<uint4*>(a.out + w.x.t * a.out_st + (int64_t)(h0 + row) * a.out_sh + d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i] = pack_bf16x2(acc[8 * (j & 1) + 2 * i][2 * r + (j >> 1)] * inv,
+                                 acc[8 * (j & 1) + 2 * i + 1][2 * r + (j >> 1)] * inv);
+            o[j] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+          if (a.lse != nullptr && gw == 0 && q4 == 0)
+            a.lse[w.x.t * a.lse_st + h0 + row] = lt[r] == 0.f ? -INFINITY : (mm[r] - kBias) * kLn2 + logf(lt[r]);
+        } else {
+          float4* o = reinterpret_cast<float4*>(a.ws_o + (slot * kBH + row) * kNope + d);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[4 * j + i] = make_float4(acc[4 * i][2 * r + j], acc[4 * i + 1][2 * r + j], acc[4 * i + 2][2 * r + j],
+                                         acc[4 * i + 3][2 * r + j]);
+          if (gw == 0 && q4 == 0) a.ws_ml[slot * kBH + row] = make_float2(mm[r], lt[r]);
+        }
+      }
+    }
     w.next_unit(a, nch);
   }
 }
@@ -585,13 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&s.raw_full[i]), kPWarps);
-      mbar_init(smem_u32(&s.raw_empty[i]), kSWarps + kOWarps);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&s.p_full[i]), kSWarps);
-      mbar_init(smem_u32(&s.p_empty[i]), kOWarps);
-      mbar_init(smem_u32(&s.fin_full[i]), kSWarps);
-      mbar_init(smem_u32(&s.fin_empty[i]), kOWarps);
+      mbar_init(smem_u32(&s.raw_empty[i]), kGWarps);
     }
     mbar_init_fence();
   }
@@ -612,15 +681,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     info[3] = per;
   }
-  if (warp < kSWarps) {
-    regs_inc<232>();
-    scores(a, s, per, warp, lane);
-  } else if (warp < kSWarps + kOWarps) {
-    regs_dec<104>();
-    outputs(a, s, per, warp - kSWarps, lane);
+  if (warp < kCWarps) {
+    regs_inc<kCRegs>();
+    compute(a, s, per, warp, lane);
   } else {
-    regs_dec<64>();
-    produce(a, s, &tm, per, warp - kSWarps - kOWarps, lane);
+    regs_dec<kPRegs>();
+    produce(a, s, &tm, per, warp - kCWarps, lane);
   }
 }
 
