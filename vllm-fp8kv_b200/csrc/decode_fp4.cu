@@ -211,80 +211,101 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------ producers
-// Warp pw owns rows [16 pw, +16) of every chunk, lane i (and i + 16) row i.  The entry
-// is read two chunks ahead, its block-table word one chunk ahead.  A run of
-// consecutive slots (the pages of a whole context) is one bulk copy, other
-// rows go four at a time through gather4; masked rows are not read (a group
-// with some fetches row 0 for them) and their bits stay clear.
+// Warp pw owns rows [16 pw, +16) of every chunk.  Lanes 0-15 hold the rows of the
+// even chunks of the worker's run, lanes 16-31 those of the odd ones: each
+// half walks the run in steps of two, reading entries three steps (six chunks)
+// ahead of their copy and block-table words two steps ahead, so that neither
+// latency is waited for.  A run of consecutive slots (the pages of a whole
+// context) is one bulk copy, other rows go four at a time through gather4;
+// masked rows are not read (a group with some fetches row 0 for them) and
+// their bits stay clear.
 __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, int64_t per, int pw, int lane) {
   const int row = 16 * pw + (lane & 15);
   Walk ahead(a, s, per);
-  int32_t req_ahead = 0;
+  const int64_t chunks = ahead.left;
+  int32_t req = 0;
   const int32_t* idx_row = nullptr;
   auto open = [&]() {
     if (ahead.left <= 0) return;
-    req_ahead = a.block_table != nullptr ? a.req_id[ahead.x.t] : 0;
+    if (a.block_table != nullptr) req = a.req_id[ahead.x.t];
     if (a.lens == nullptr) idx_row = a.idx + ahead.x.t * a.idx_st + ahead.x.grp * a.idx_sg;
   };
-  open();
-  struct Entry {
-    int32_t v, req;
-  };
-  auto fetch = [&]() -> Entry {
-    Entry e{-1, 0};
-    if (ahead.left <= 0) return e;
-    const int pos = ahead.x.c * kBN + row;
-    e.req = req_ahead;
-    if (pos < ahead.x.entries) e.v = a.lens == nullptr ? idx_row[pos] : pos;
-    ++ahead.x.c;
-    --ahead.left;
-    if (ahead.x.c == ahead.x.n && ahead.left > 0) {
+  auto step = [&]() {
+    if (--ahead.left > 0 && ++ahead.x.c == ahead.x.n) {
       fp4_open(a, ahead.x, ahead.x.unit + 1, kBN);
       open();
     }
+  };
+  open();
+  if (lane >= 16) step();
+  int32_t v[3], rq[3], pg[2];  // steps g / 2 .. + 2: entry, request; .. + 1: block-table word
+  auto fetch = [&]() -> int32_t {
+    int32_t e = -1;
+    if (ahead.left > 0) {
+      const int pos = ahead.x.c * kBN + row;
+      if (pos < ahead.x.entries) e = a.lens == nullptr ? idx_row[pos] : pos;
+    }
     return e;
   };
-  const int64_t chunks = ahead.left;
-  Entry e0 = fetch(), e1 = fetch();
-  int32_t pg0 = fp4_table(a, e0.req, e0.v);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    v[i] = fetch();
+    rq[i] = req;
+    step();
+    step();
+  }
+  pg[0] = fp4_table(a, rq[0], v[0]);
+  pg[1] = fp4_table(a, rq[1], v[1]);
   bool ok = true;
   int64_t armed = 0;
   Ring ring;
-  for (int64_t g = 0; g < chunks; ++g, ring.ahead(1)) {
-    const int32_t slot = fp4_slot(a, e0.v, pg0);
-    const Entry e2 = fetch();
-    pg0 = fp4_table(a, e1.req, e1.v);
-    e0 = e1;
-    e1 = e2;
-    const int st = ring.st;
-    if (g >= kStages) ok = warp_wait(smem_u32(&s.raw_empty[st]), ring.ph ^ 1, 20);
-    if (!ok) break;
-    const uint32_t live = __ballot_sync(0xFFFFFFFFu, slot >= 0) & 0xFFFFu;
-    const int n = __popc(live);
-    const int32_t s0 = __shfl_sync(0xFFFFFFFFu, slot, 0);
-    const bool run = __all_sync(0xFFFFFFFFu, slot < 0 || slot == s0 + (lane & 15)) && (live & (live + 1)) == 0;
-    const uint32_t bar = smem_u32(&s.raw_full[st]);
-    const uint32_t dst = smem_u32(&s.raw[st][16 * pw * kFp4RowBytes]);
-    // groups of four rows with a live one
-    const uint32_t grp = (live & 0xFu ? 1u : 0u) | (live & 0xF0u ? 2u : 0u) | (live & 0xF00u ? 4u : 0u) |
-                         (live & 0xF000u ? 8u : 0u);
-    if (lane == 0) {
-      reinterpret_cast<uint16_t*>(s.live[st])[pw] = (uint16_t)live;
-      mbar_arrive_expect_tx(bar, run ? (uint32_t)(n * kFp4RowBytes) : (uint32_t)(__popc(grp) * 4 * kFp4RowBytes));
+  for (int64_t g = 0; g < chunks && ok; g += 2) {
+    const int32_t slot = fp4_slot(a, v[0], pg[0]);
+    v[0] = v[1];
+    v[1] = v[2];
+    rq[1] = rq[2];
+    v[2] = fetch();
+    rq[2] = req;
+    pg[0] = pg[1];
+    pg[1] = fp4_table(a, rq[1], v[1]);
+    step();
+    step();
+    const uint32_t live2 = __ballot_sync(0xFFFFFFFFu, slot >= 0);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (g + half >= chunks) break;
+      const int st = ring.st;
+      if (g + half >= kStages) ok = warp_wait(smem_u32(&s.raw_empty[st]), ring.ph ^ 1, 20);
+      if (!ok) break;
+      const uint32_t live = (live2 >> (16 * half)) & 0xFFFFu;
+      const int n = __popc(live);
+      const int32_t s0 = __shfl_sync(0xFFFFFFFFu, slot, 16 * half);
+      const bool run = (live & (live + 1)) == 0 &&
+                       __all_sync(0xFFFFFFFFu, (lane >> 4) != half || slot < 0 || slot == s0 + (lane & 15));
+      const uint32_t bar = smem_u32(&s.raw_full[st]);
+      const uint32_t dst = smem_u32(&s.raw[st][16 * pw * kFp4RowBytes]);
+      // groups of four rows with a live one
+      const uint32_t grp = (live & 0xFu ? 1u : 0u) | (live & 0xF0u ? 2u : 0u) | (live & 0xF00u ? 4u : 0u) |
+                           (live & 0xF000u ? 8u : 0u);
+      if (lane == 0) {
+        reinterpret_cast<uint16_t*>(s.live[st])[pw] = (uint16_t)live;
+        mbar_arrive_expect_tx(bar, run ? (uint32_t)(n * kFp4RowBytes) : (uint32_t)(__popc(grp) * 4 * kFp4RowBytes));
+      }
+      __syncwarp();
+      if (run) {
+        if (lane == 0 && n > 0) bulk_g2s(dst, a.kv + (int64_t)s0 * kFp4RowBytes, (uint32_t)(n * kFp4RowBytes), bar);
+      } else {
+        const int32_t r = slot >= 0 ? slot : 0;
+        const int src = 16 * half + ((4 * lane) & 15);
+        const int32_t r0 = __shfl_sync(0xFFFFFFFFu, r, src);
+        const int32_t r1 = __shfl_sync(0xFFFFFFFFu, r, src + 1);
+        const int32_t r2 = __shfl_sync(0xFFFFFFFFu, r, src + 2);
+        const int32_t r3 = __shfl_sync(0xFFFFFFFFu, r, src + 3);
+        if (lane < 4 && ((grp >> lane) & 1u)) tma_gather4(dst + lane * 4 * kFp4RowBytes, tm, 0, r0, r1, r2, r3, bar);
+      }
+      ++armed;
+      ring.ahead(1);
     }
-    __syncwarp();
-    if (run) {
-      if (lane == 0 && n > 0) bulk_g2s(dst, a.kv + (int64_t)s0 * kFp4RowBytes, (uint32_t)(n * kFp4RowBytes), bar);
-    } else {
-      const int32_t r = slot >= 0 ? slot : 0;
-      const int src = (4 * lane) & 15;
-      const int32_t r0 = __shfl_sync(0xFFFFFFFFu, r, src);
-      const int32_t r1 = __shfl_sync(0xFFFFFFFFu, r, src + 1);
-      const int32_t r2 = __shfl_sync(0xFFFFFFFFu, r, src + 2);
-      const int32_t r3 = __shfl_sync(0xFFFFFFFFu, r, src + 3);
-      if (lane < 4 && ((grp >> lane) & 1u)) tma_gather4(dst + lane * 4 * kFp4RowBytes, tm, 0, r0, r1, r2, r3, bar);
-    }
-    ++armed;
   }
   // the stages armed last have landed before the warp returns, even after a
   // failed wait
