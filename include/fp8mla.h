@@ -386,10 +386,12 @@ FP8MLA_API int fp8mla_fp4_gather(const uint8_t* kv, int64_t num_slots, const int
                                  const int32_t* cu_seq_lens, int64_t B, const int32_t* seq_starts,
                                  int64_t n, uint16_t* out, int64_t out_stride, void* stream);
 
-/* Bytes of device workspace the three attention calls below need for a shape
- * (16-byte aligned; the contents need no initialisation and carry nothing
- * from call to call; calls that may run at once need one each). */
-FP8MLA_API int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G);
+/* Bytes of device workspace an attention call below needs (16-byte aligned;
+ * the contents need no initialisation and carry nothing from call to call;
+ * calls that may run at once need one each).  topk: the index rows' width (0
+ * bytes where whole rows go to single SMs), or -1 for whole contexts, which is
+ * also the most any topk needs. */
+FP8MLA_API int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t topk);
 
 /* Name of the attention kernel for H heads in G kv groups (introspection). */
 FP8MLA_API const char* fp8mla_fp4_kernel_name(int64_t H, int64_t G);

@@ -119,6 +119,9 @@ def test_c_table_refusals():
 def test_workspace_and_names():
     assert F.fp4_workspace_bytes(0, 16) == 0
     assert F.fp4_workspace_bytes(1, 16) > 0 and F.fp4_workspace_bytes(1, 16) % 16 == 0
+    assert F.fp4_workspace_bytes(3, 16, 1, 64) == 0            # whole rows: nothing to join
+    for T, topk in ((1, 2048), (5, 100), (300, 777)):
+        assert F.fp4_workspace_bytes(T, 16, 1, topk) <= F.fp4_workspace_bytes(T, 16)
     assert F.fp4_kernel_name(16).startswith("decode_fp4")
 
 

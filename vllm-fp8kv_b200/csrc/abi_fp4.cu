@@ -9,17 +9,46 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+constexpr int64_t kMaxTopk = 1LL << 30, kMaxT = 1LL << 24, kMaxH = 1 << 16;
+
+// How a call's units are dealt out (decode_fp4.h).
 struct Plan {
-  int rows, workers;
+  int rows, workers, hb_per_group;
+  int64_t per;  // 0: from the lengths, on the device
+  bool cuts;    // some unit may be cut
 };
-Plan plan_of(int64_t hpg) {
-  (void)hpg;
-  return Plan{16, device_sm_count()};
+// topk < 0: whole contexts, of at most max_len positions
+Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
+  Plan p;
+  const int64_t hpg = H / G;
+  p.rows = 16;
+  p.workers = device_sm_count();
+  p.hb_per_group = (int)((hpg + p.rows - 1) / p.rows);
+  const int64_t chunk = decode_fp4_chunk(), units = T * G * p.hb_per_group;
+  const int64_t len = topk < 0 ? max_len : topk;
+  const int64_t n = len > chunk ? (len + chunk - 1) / chunk : 1;  // chunks of a unit (at most)
+  const int64_t total = units * n;
+  if (total < p.workers) p.workers = (int)total;
+  if (topk < 0) {
+    p.per = 0;
+    p.cuts = n > 1;
+    return p;
+  }
+  p.per = (total + p.workers - 1) / p.workers;
+  p.cuts = p.per % n != 0;
+  // whole units where that costs a sixth more at most: no partials, no merge
+  const int64_t whole = (p.per + n - 1) / n * n;
+  if (whole * 6 <= p.per * 7) {
+    p.per = whole;
+    p.cuts = false;
+  }
+  p.workers = (int)((total + p.per - 1) / p.per);
+  return p;
 }
 int64_t info_bytes(const Plan& p) { return (int64_t)p.workers * 4 * 8; }
 int64_t part_bytes(const Plan& p) { return (int64_t)2 * p.workers * p.rows * FP8MLA_NOPE * 4; }
 int64_t workspace_of(const Plan& p) {
-  return part_bytes(p) + (int64_t)2 * p.workers * p.rows * 8 + info_bytes(p);
+  return p.cuts ? part_bytes(p) + (int64_t)2 * p.workers * p.rows * 8 + info_bytes(p) : 0;
 }
 
 int check_table(const int32_t* req_id, const int32_t* block_table, int64_t bt_stride, int64_t max_blocks,
@@ -46,7 +75,7 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
   if (H % G != 0)
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "h_q=%lld not divisible by kv_groups=%lld", (long long)H,
                      (long long)G);
-  if (topk > (1LL << 30) || T > (1LL << 24) || H > (1 << 16))
+  if (topk > kMaxTopk || T > kMaxT || H > kMaxH)
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "topk, T or H too large");
   if (T == 0) return FP8MLA_OK;
   if (q == nullptr || out == nullptr || (num_slots > 0 && kv == nullptr) || (lens == nullptr && topk > 0 && idx == nullptr))
@@ -59,8 +88,8 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
   if (int rc = require_sm100()) return rc;
 
   const int64_t hpg = H / G;
-  const Plan p = plan_of(hpg);
-  if (workspace == nullptr || workspace_bytes < workspace_of(p) || !aligned16(workspace))
+  const Plan p = plan_of(T, H, G, lens != nullptr ? -1 : topk, max_blocks * block_size);
+  if (p.cuts && (workspace == nullptr || workspace_bytes < workspace_of(p) || !aligned16(workspace)))
     return set_error(FP8MLA_ERR_WORKSPACE, "needs %lld bytes of 16-B aligned workspace, got %lld",
                      (long long)workspace_of(p), (long long)workspace_bytes);
   Fp4DecodeArgs a{};
@@ -79,7 +108,9 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
   a.topk = (int)topk;
   a.hpg = (int)hpg;
   a.rows = p.rows;
-  a.hb_per_group = (int)((hpg + p.rows - 1) / p.rows);
+  a.hb_per_group = p.hb_per_group;
+  a.workers = p.workers;
+  a.per = p.per;
   a.scale_log2 = sm_scale * kLog2e;
   a.out = out;
   a.out_st = out_st;
@@ -97,32 +128,14 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
   for (int k = 0; k < 31; ++k)
     if (block_table != nullptr && (int64_t)1 << k == block_size) a.block_shift = k;
   a.max_len = max_blocks * block_size;
-  char* ws = static_cast<char*>(workspace);
-  a.ws_o = reinterpret_cast<float*>(ws);
-  a.ws_info = reinterpret_cast<int64_t*>(ws + part_bytes(p));
-  a.ws_ml = reinterpret_cast<float2*>(ws + part_bytes(p) + info_bytes(p));
-
-  const int64_t chunk = decode_fp4_chunk();
-  const int64_t units = T * G * a.hb_per_group;
-  bool cuts = true;
-  if (lens == nullptr) {
-    const int64_t n = topk > chunk ? (topk + chunk - 1) / chunk : 1;
-    const int64_t total = units * n;
-    a.workers = (int)(total < p.workers ? total : p.workers);
-    a.per = (total + a.workers - 1) / a.workers;
-    // whole units where that costs a sixth more at most: no partials, no merge
-    const int64_t whole = (a.per + n - 1) / n * n;
-    if (whole * 6 <= a.per * 7) {
-      a.per = whole;
-      cuts = false;
-    }
-    a.workers = (int)((total + a.per - 1) / a.per);
-  } else {
-    const int64_t most = units * (a.max_len > chunk ? (a.max_len + chunk - 1) / chunk : 1);
-    a.workers = (int)(most < p.workers ? most : p.workers);
-    cuts = a.max_len > chunk;
+  if (p.cuts) {
+    char* ws = static_cast<char*>(workspace);
+    a.ws_o = reinterpret_cast<float*>(ws);
+    a.ws_info = reinterpret_cast<int64_t*>(ws + part_bytes(p));
+    a.ws_ml = reinterpret_cast<float2*>(ws + part_bytes(p) + info_bytes(p));
   }
-  return launch_decode_fp4(a, cuts, static_cast<cudaStream_t>(stream));
+
+  return launch_decode_fp4(a, p.cuts, static_cast<cudaStream_t>(stream));
 }
 
 }  // namespace
@@ -175,9 +188,9 @@ int fp8mla_fp4_gather(const uint8_t* kv, int64_t num_slots, const int32_t* block
                            seq_starts, n, out, out_stride, static_cast<cudaStream_t>(stream));
 }
 
-int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G) {
-  if (T <= 0 || H <= 0 || G <= 0 || H % G != 0) return 0;
-  return workspace_of(plan_of(H / G));
+int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t topk) {
+  if (T <= 0 || T > kMaxT || H <= 0 || H > kMaxH || G <= 0 || H % G != 0 || topk < -1 || topk > kMaxTopk) return 0;
+  return workspace_of(plan_of(T, H, G, topk, INT32_MAX));
 }
 
 const char* fp8mla_fp4_kernel_name(int64_t H, int64_t G) {

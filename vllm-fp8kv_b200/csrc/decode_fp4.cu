@@ -689,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) pdl_launch_dependents();
   pdl_wait();  // the previous kernel of the stream has completed: global memory from here on
   const int64_t per = divide_work(a, s);
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && a.ws_info != nullptr) {
     const int64_t at = (int64_t)blockIdx.x * per;
     int64_t* info = a.ws_info + 4 * blockIdx.x;
     if (at < s.tok_total) {
@@ -767,8 +767,8 @@ int launch_decode_fp4(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st) {
   if (a.num_slots > 0)
     if (int rc = encode_fp4_row_map(&tm, a.kv, a.num_slots)) return rc;
   const size_t smem = sizeof(Smem) + 128;
-  cudaError_t e = cudaFuncSetAttribute(decode_fp4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return check_cuda(e, "decode_fp4 smem attribute");
+  static SmemLimit limit;
+  if (int rc = limit.raise(decode_fp4_kernel, smem)) return rc;
   if (int rc = check_cuda(launch_pdl(decode_fp4_kernel, dim3((unsigned)a.workers), dim3(kThreads), smem, st, a, tm),
                           "decode_fp4_kernel launch"))
     return rc;

@@ -12,6 +12,9 @@
 // The merge kernel joins a cut unit's pieces in order, so results do not
 // depend on timing.
 #pragma once
+#include <atomic>
+
+#include "common.cuh"
 #include "decode.h"
 
 namespace fp8mla {
@@ -95,6 +98,20 @@ __device__ __forceinline__ int32_t fp4_slot(const Fp4DecodeArgs& a, int32_t v, i
   return s >= 0 && s < a.num_slots ? (int32_t)s : -1;
 }
 #endif
+
+// Raises a kernel's dynamic shared memory limit, once per device.
+struct SmemLimit {
+  std::atomic<uint64_t> done{0};  // bit per device
+  template <typename Kern>
+  int raise(Kern kern, size_t bytes) {
+    int dev = 0;
+    if (int rc = check_cuda(cudaGetDevice(&dev), "current device")) return rc;
+    if (dev < 64 && ((done.load(std::memory_order_acquire) >> dev) & 1u)) return FP8MLA_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    return check_cuda(e, "shared memory attribute");
+  }
+};
 
 // One worker per SM, 16 heads per unit (decode_fp4.cu).  `cuts`: some unit may
 // be cut, so the merge follows.

@@ -6,6 +6,7 @@ library is missing or the device is not sm_100, the call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -68,7 +69,7 @@ SIGNATURES = {
     "fp8mla_fp4_dequant_rows": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P]),
     "fp8mla_fp4_gather": (_I32, [_P, _I64, _P, _I64, _I64, _I64,  # kv, num_slots, block table, block_size
                                  _P, _I64, _P, _I64, _P, _I64, _P]),
-    "fp8mla_fp4_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "fp8mla_fp4_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
     "fp8mla_fp4_kernel_name": (ctypes.c_char_p, [_I64, _I64]),
     "fp8mla_fp4_sparse_decode": (_I32, [
         _P, _I64, _I64, _I64, _I64,            # q, T, H, q strides
@@ -135,6 +136,25 @@ def stream_ptr(device) -> int:
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(device):
+    """``torch.cuda.device(device)``, or nothing where it is current already
+    (entering the context costs more than the look)."""
+    import torch
+
+    return _HERE_ALREADY if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device) -> int:
+    """``stream_ptr`` of a tensor's device without building a Stream object."""
+    import torch
+
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(device.index) if get is not None else stream_ptr(device)
 
 
 def require_cuda(*tensors):

@@ -41,12 +41,16 @@ SCALE_OFF = 256
 ROPE_OFF = 288
 
 
-def _pool(kv_cache: torch.Tensor) -> torch.Tensor:
-    """The [num_slots, 416] uint8 view of a pool."""
+def _pool(kv_cache: torch.Tensor) -> int:
+    """Checks a pool; its number of slots."""
     assert kv_cache.dtype == torch.uint8, f"an fp4_ds_mla pool is uint8, got {kv_cache.dtype}"
     assert kv_cache.is_contiguous(), "kv_cache must be contiguous"
     assert kv_cache.dim() >= 2 and kv_cache.shape[-1] == ROW_BYTES, "fp4_ds_mla rows are 416 bytes"
-    return kv_cache.view(-1, ROW_BYTES)
+    return kv_cache.numel() // ROW_BYTES
+
+
+def _int64(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
 def concat_and_cache_fp4_ds_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
@@ -57,16 +61,16 @@ def concat_and_cache_fp4_ds_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache
     assert kv_c.dim() == 2 and kv_c.shape[1] == NOPE and kv_c.stride(1) == 1
     assert k_pe.dim() == 2 and k_pe.shape[1] == ROPE and k_pe.stride(1) == 1
     assert slot_mapping.dim() == 1 and kv_c.shape[0] == k_pe.shape[0] == slot_mapping.shape[0]
-    flat = _pool(kv_cache)
+    num_slots = _pool(kv_cache)
     dev = N.require_cuda(kv_c, k_pe, kv_cache, slot_mapping)
     # one token's stride is never used, but a view's may be anything
     st_c = kv_c.stride(0) if kv_c.shape[0] > 1 else NOPE
     st_pe = k_pe.stride(0) if k_pe.shape[0] > 1 else ROPE
     assert st_c >= NOPE and st_pe >= ROPE, "token rows must not overlap"
-    slots = slot_mapping.to(torch.int64).contiguous()
-    with torch.cuda.device(dev):
+    slots = _int64(slot_mapping)
+    with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_write(kv_c.data_ptr(), st_c, k_pe.data_ptr(), st_pe, slots.data_ptr(),
-                                      slots.numel(), flat.data_ptr(), flat.shape[0], N.stream_ptr(dev))
+                                      slots.shape[0], kv_cache.data_ptr(), num_slots, N.raw_stream(dev))
     N.check(rc, "concat_and_cache_fp4_ds_mla")
 
 
@@ -86,14 +90,14 @@ def dequant_fp4_ds_mla_rows(kv_cache: torch.Tensor, slots: torch.Tensor,
                             out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 [n, 576] rows (latent, rope) of slots [n]; slots outside the pool
     give zero rows.  `out`: a bf16 [n, 576] tensor to fill (16-byte aligned rows)."""
-    kv = _pool(kv_cache)
+    num_slots = _pool(kv_cache)
     assert slots.dim() == 1 and slots.dtype in (torch.int32, torch.int64), "slots must be int32 or int64 [n]"
     dev = N.require_cuda(kv_cache, slots, out)
-    sl = slots.to(torch.int64).contiguous()
+    sl = _int64(slots)
     out = _check_out(out, sl.numel(), dev)
-    with torch.cuda.device(dev):
-        rc = N.lib().fp8mla_fp4_dequant_rows(kv.data_ptr(), kv.shape[0], sl.data_ptr(), sl.numel(), out.data_ptr(),
-                                             _row_stride(out), N.stream_ptr(dev))
+    with N.on_device(dev):
+        rc = N.lib().fp8mla_fp4_dequant_rows(kv_cache.data_ptr(), num_slots, sl.data_ptr(), sl.numel(), out.data_ptr(),
+                                             _row_stride(out), N.raw_stream(dev))
     N.check(rc, "dequant_fp4_ds_mla_rows")
     return out
 
@@ -108,7 +112,7 @@ def gather_fp4_ds_mla(kv_cache: torch.Tensor, block_table: torch.Tensor, cu_seq_
     holds its pages.  Positions behind the table, or on pages outside the pool,
     give zero rows.  num_tokens is cu_seq_lens[-1]; where it (or `out`) has more
     rows, those behind the last sequence are left as they were."""
-    kv = _pool(kv_cache)
+    num_slots = _pool(kv_cache)
     assert block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table [B, max_blocks] int32"
     assert block_table.shape[1] == 0 or block_table.stride(1) == 1, "block_table rows must be unit-strided"
     B = block_table.shape[0]
@@ -121,18 +125,19 @@ def gather_fp4_ds_mla(kv_cache: torch.Tensor, block_table: torch.Tensor, cu_seq_
     out = _check_out(out, num_tokens, dev)
     bt_stride = block_table.stride(0) if B > 1 else block_table.shape[1]
     assert bt_stride >= block_table.shape[1], "block_table rows must not overlap"
-    with torch.cuda.device(dev):
+    with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_gather(
-            kv.data_ptr(), kv.shape[0], block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
+            kv_cache.data_ptr(), num_slots, block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
             cu_seq_lens.data_ptr(), B, seq_starts.data_ptr() if seq_starts is not None else None, num_tokens,
-            out.data_ptr(), _row_stride(out), N.stream_ptr(dev))
+            out.data_ptr(), _row_stride(out), N.raw_stream(dev))
     N.check(rc, "gather_fp4_ds_mla")
     return out
 
 
-def fp4_workspace_bytes(T: int, H: int, G: int = 1) -> int:
-    """Device workspace one attention call needs."""
-    return int(N.lib().fp8mla_fp4_workspace_bytes(T, H, G))
+def fp4_workspace_bytes(T: int, H: int, G: int = 1, topk: int = -1) -> int:
+    """Device workspace one attention call needs (0 where no unit is cut); topk -1:
+    the most any call of T tokens needs, whole contexts included."""
+    return int(N.lib().fp8mla_fp4_workspace_bytes(T, H, G, topk))
 
 
 def fp4_kernel_name(H: int, G: int = 1) -> str:
@@ -140,28 +145,32 @@ def fp4_kernel_name(H: int, G: int = 1) -> str:
     return N.lib().fp8mla_fp4_kernel_name(H, G).decode()
 
 
-def _prepare(q, kv_cache, groups, workspace, *others):
-    """Checks shared by the attention calls; q in 16-byte rows, out, workspace, device."""
-    kv = _pool(kv_cache)
+def _prepare(q, kv_cache, groups, topk, return_lse, workspace, *others):
+    """Checks shared by the attention calls; q in 16-byte rows, the pool's slots,
+    out, lse, workspace and the pointers' device."""
+    num_slots = _pool(kv_cache)
     assert q.dtype == torch.bfloat16, f"rope is stored bf16; q must be bf16, got {q.dtype}"
     assert q.dim() == 3 and q.shape[2] == NOPE + ROPE, f"q must be [T, H, {NOPE + ROPE}], got {tuple(q.shape)}"
     assert q.stride(-1) == 1, "need unit last-dim strides"
-    assert q.shape[1] % groups == 0, f"h_q={q.shape[1]} not divisible by kv_groups={groups}"
+    T, H, _ = q.shape
+    assert H % groups == 0, f"h_q={H} not divisible by kv_groups={groups}"
     dev = N.require_cuda(q, kv_cache, workspace, *others)
     # the kernels read q in 16-byte vectors; re-lay a misaligned view once
     if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-    T, H = q.shape[0], q.shape[1]
-    out = torch.empty((T, H, NOPE), dtype=q.dtype, device=dev)
-    lse = torch.empty((T, H), dtype=torch.float32, device=dev)
-    need = fp4_workspace_bytes(T, H, groups)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    else:
+    out = q.new_empty((T, H, NOPE))
+    lse = q.new_empty((T, H), dtype=torch.float32) if return_lse else None
+    need = N.lib().fp8mla_fp4_workspace_bytes(T, H, groups, topk)
+    if workspace is not None:
         assert workspace.is_contiguous(), "workspace must be contiguous"
-    return q, kv, out, lse, workspace, dev
+        if workspace.numel() * workspace.element_size() < need:
+            workspace = None
+    if workspace is None and need:
+        workspace = q.new_empty((need,), dtype=torch.uint8)
+    ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
+    return q, num_slots, out, lse, (lse.data_ptr(), H) if return_lse else (None, 0), ws, workspace, dev
 
 
 def _check_table(req_id, block_table, T, block_size):
@@ -200,13 +209,12 @@ def fp4_ds_mla_sparse_decode(
     indices = _with_groups(indices)
     G, topk = indices.shape[1], indices.shape[2]
     assert indices.shape[0] == q.shape[0], "one index row per query token"
-    q, kv, out, lse, ws, dev = _prepare(q, kv_cache, G, workspace, indices)
-    with torch.cuda.device(dev):
+    q, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace, indices)
+    with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_sparse_decode(
-            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv.data_ptr(), kv.shape[0],
+            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv_cache.data_ptr(), num_slots,
             indices.data_ptr(), G, topk, indices.stride(0), indices.stride(1), float(sm_scale),
-            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0),
-            ws.data_ptr(), ws.numel() * ws.element_size(), N.stream_ptr(dev))
+            out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
     N.check(rc, "fp4_ds_mla_sparse_decode")
     return (out, lse) if return_lse else out
 
@@ -230,14 +238,14 @@ def fp4_ds_mla_sparse_decode_paged(
     G, topk = token_indices.shape[1], token_indices.shape[2]
     assert token_indices.shape[0] == q.shape[0], "one index row per query token"
     bt_stride = _check_table(req_id, block_table, q.shape[0], block_size)
-    q, kv, out, lse, ws, dev = _prepare(q, kv_cache, G, workspace, token_indices, req_id, block_table)
-    with torch.cuda.device(dev):
+    q, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace, token_indices, req_id,
+                                                             block_table)
+    with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_sparse_decode_paged(
-            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv.data_ptr(), kv.shape[0],
+            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv_cache.data_ptr(), num_slots,
             req_id.data_ptr(), block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
             token_indices.data_ptr(), G, topk, token_indices.stride(0), token_indices.stride(1), float(sm_scale),
-            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0),
-            ws.data_ptr(), ws.numel() * ws.element_size(), N.stream_ptr(dev))
+            out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
     N.check(rc, "fp4_ds_mla_sparse_decode_paged")
     return (out, lse) if return_lse else out
 
@@ -264,13 +272,13 @@ def fp4_ds_mla_decode(
     assert context_lens.dtype == torch.int32 and context_lens.dim() == 1 and context_lens.is_contiguous()
     assert context_lens.shape[0] == q.shape[0], "one context length per query token"
     bt_stride = _check_table(req_id, block_table, q.shape[0], block_size)
-    q, kv, out, lse, ws, dev = _prepare(q, kv_cache, 1, workspace, context_lens, req_id, block_table)
-    with torch.cuda.device(dev):
+    q, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, 1, -1, return_lse, workspace, context_lens, req_id,
+                                                             block_table)
+    with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_decode(
-            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv.data_ptr(), kv.shape[0],
+            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv_cache.data_ptr(), num_slots,
             req_id.data_ptr(), block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
             context_lens.data_ptr(), float(sm_scale),
-            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0),
-            ws.data_ptr(), ws.numel() * ws.element_size(), N.stream_ptr(dev))
+            out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
     N.check(rc, "fp4_ds_mla_decode")
     return (out, lse) if return_lse else out
