@@ -13,7 +13,7 @@ constexpr int64_t kMaxTopk = 1LL << 30, kMaxT = 1LL << 24, kMaxH = 1 << 16;
 
 // How a call's units are dealt out (decode_fp4.h).
 struct Plan {
-  int rows, workers, hb_per_group;
+  int rows, workers, hb_per_group, chunk, min_per;
   int64_t per;  // 0: from the lengths, on the device
   bool cuts;    // some unit may be cut
 };
@@ -24,7 +24,9 @@ Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
   p.rows = 16;
   p.workers = device_sm_count();
   p.hb_per_group = (int)((hpg + p.rows - 1) / p.rows);
-  const int64_t chunk = decode_fp4_chunk(), units = T * G * p.hb_per_group;
+  p.chunk = kFp4Chunk;
+  p.min_per = kFp4MinPer;
+  const int64_t chunk = p.chunk, units = T * G * p.hb_per_group;
   const int64_t len = topk < 0 ? max_len : topk;
   const int64_t n = len > chunk ? (len + chunk - 1) / chunk : 1;  // chunks of a unit (at most)
   const int64_t total = units * n;
@@ -35,13 +37,13 @@ Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
     return p;
   }
   p.per = (total + p.workers - 1) / p.workers;
-  p.cuts = p.per % n != 0;
-  // whole units where that costs a sixth more at most: no partials, no merge
+  if (p.per < p.min_per) p.per = p.min_per;
+  // whole units where that adds a sixth, or 256 entries, at most: there are no
+  // partials then and the merge's launch (4 us, the time of about four chunks)
+  // is saved
   const int64_t whole = (p.per + n - 1) / n * n;
-  if (whole * 6 <= p.per * 7) {
-    p.per = whole;
-    p.cuts = false;
-  }
+  p.cuts = whole * 6 > p.per * 7 && (whole - p.per) * chunk > 256;
+  if (!p.cuts) p.per = whole;
   p.workers = (int)((total + p.per - 1) / p.per);
   return p;
 }
@@ -111,6 +113,7 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
   a.hb_per_group = p.hb_per_group;
   a.workers = p.workers;
   a.per = p.per;
+  a.min_per = p.min_per;
   a.scale_log2 = sm_scale * kLog2e;
   a.out = out;
   a.out_st = out_st;

@@ -25,6 +25,7 @@
 // The registers move from the producers to the others (setmaxnreg).
 #include "decode_fp4.h"
 #include "fp4.cuh"
+#include "fp4_walk.cuh"
 #include "tc_cluster.cuh"
 #include "tc_ptx.cuh"
 #include "tma_map.h"
@@ -35,10 +36,10 @@ using namespace fp8mla::fp4;
 using namespace fp8mla::tc;
 
 constexpr int kBH = 16;           // heads per unit
-constexpr int kBN = 64;           // entries per chunk
+constexpr int kBN = kFp4Chunk;    // entries per chunk
 constexpr int kStages = 6;
 constexpr int kStageBytes = kBN * kFp4RowBytes;  // 26624
-constexpr int kGroups = 3, kGWarps = 4, kPWarps = 4;
+constexpr int kGroups = kFp4MinPer, kGWarps = 4, kPWarps = 4;
 constexpr int kCWarps = kGroups * kGWarps;
 constexpr int kThreads = 32 * (kCWarps + kPWarps);
 constexpr int kCRegs = 152, kPRegs = 56;  // launched with 128 each
@@ -60,9 +61,7 @@ struct Smem {
   float qscale[kBH];                      // score = qscale * accumulator (log2 units)
   uint32_t live[kStages][2];              // 16 bits per producer warp
   uint64_t raw_full[kStages], raw_empty[kStages];
-  int64_t tok_total, start_unit;
-  int start_chunk;
-  int64_t scan[kThreads / 32];
+  Share share;
 };
 static_assert(offsetof(Smem, q) % 16 == 0 && offsetof(Smem, live) % 8 == 0 && offsetof(Smem, raw_full) % 8 == 0, "alignment");
 static_assert(sizeof(Smem) + 128 <= 227 * 1024, "shared memory budget");
@@ -106,13 +105,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-
 // The chunk row that column n of an 8-column tile stands for, n even: n / 2,
 // n odd: 4 + (n / 2 + 1) % 4.  It is both the S product's B column and the O
 // product's k index, so P needs no shuffle between them; the rows of a column
@@ -121,61 +113,6 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t
 // modulo 4 (neither do the O loads of four rows).
 __device__ __forceinline__ int row_even(int pair) { return pair; }
 __device__ __forceinline__ int row_odd(int pair) { return 4 + ((pair + 1) & 3); }
-
-// Where this worker starts, and how many chunks each worker takes: from the
-// sizes, or (lengths on the device) from two passes over the lengths.
-// Returns `per`; the start goes to shared memory.
-__device__ int64_t divide_work(const Fp4DecodeArgs& a, Smem& s) {
-  const int per_tok = a.G * a.hb_per_group;
-  int64_t per = a.per;
-  if (a.lens == nullptr) {
-    if (threadIdx.x == 0) {
-      const int64_t n = fp4_chunks(a.topk, kBN), at = (int64_t)blockIdx.x * per;
-      s.tok_total = (int64_t)a.T * per_tok * n;
-      s.start_unit = at / n;
-      s.start_chunk = (int)(at - s.start_unit * n);
-    }
-    __syncthreads();
-    return per;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t sum = 0;
-  for (int t = threadIdx.x; t < a.T; t += kThreads) sum += fp4_chunks(fp4_entries(a, t), kBN);
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (lane == 0) s.scan[warp] = sum;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) total += s.scan[w];
-  total *= per_tok;
-  per = (total + a.workers - 1) / a.workers;
-  const int64_t at = (int64_t)blockIdx.x * per;
-  int64_t before = 0;  // chunks of the tokens in front of this pass
-  for (int t0 = 0; t0 < a.T; t0 += kThreads) {
-    const int t = t0 + threadIdx.x;
-    const int n = t < a.T ? fp4_chunks(fp4_entries(a, t), kBN) : 0;
-    const int64_t mine = (int64_t)n * per_tok;
-    int64_t inc = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    __syncthreads();
-    if (lane == 31) s.scan[warp] = inc;
-    __syncthreads();
-    int64_t base = before;
-    for (int w = 0; w < warp; ++w) base += s.scan[w];
-    const int64_t hi = base + inc, lo = hi - mine;
-    if (t < a.T && at >= lo && at < hi) {
-      const int64_t u = (at - lo) / n;
-      s.start_unit = (int64_t)t * per_tok + u;
-      s.start_chunk = (int)(at - lo - u * n);
-    }
-    for (int w = 0; w < kThreads / 32; ++w) before += s.scan[w];
-  }
-  if (threadIdx.x == 0) s.tok_total = total;
-  __syncthreads();
-  return per;
-}
 
 // Place in the ring of stages: the stage, and the parity of its current round.
 struct Ring {
@@ -190,86 +127,20 @@ struct Ring {
   }
 };
 
-// A worker's chunks in order.
-struct Walk {
-  Fp4Cursor x;
-  int64_t left;  // chunks of this worker from the current one on
-  __device__ __forceinline__ Walk(const Fp4DecodeArgs& a, const Smem& s, int64_t per) {
-    const int64_t at = (int64_t)blockIdx.x * per;
-    left = s.tok_total - at < per ? s.tok_total - at : per;
-    if (left > 0) {
-      fp4_open(a, x, s.start_unit, kBN);
-      x.c = s.start_chunk;
-    }
-  }
-  // chunks of this worker in the current unit, from the current chunk on
-  __device__ __forceinline__ int here() const { return (int)(left < x.n - x.c ? left : x.n - x.c); }
-  __device__ __forceinline__ void next_unit(const Fp4DecodeArgs& a, int done) {
-    left -= done;
-    if (left > 0) fp4_open(a, x, x.unit + 1, kBN);
-  }
-};
-
 // ------------------------------------------------------------------ producers
-// Warp pw owns rows [16 pw, +16) of every chunk.  Lanes 0-15 hold the rows of the
-// even chunks of the worker's run, lanes 16-31 those of the odd ones: each
-// half walks the run in steps of two, reading entries three steps (six chunks)
-// ahead of their copy and block-table words two steps ahead, so that neither
-// latency is waited for.  A run of consecutive slots (the pages of a whole
-// context) is one bulk copy, other rows go four at a time through gather4;
-// masked rows are not read (a group with some fetches row 0 for them) and
-// their bits stay clear.
-__device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, int64_t per, int pw, int lane) {
-  const int row = 16 * pw + (lane & 15);
-  Walk ahead(a, s, per);
-  const int64_t chunks = ahead.left;
-  int32_t req = 0;
-  const int32_t* idx_row = nullptr;
-  auto open = [&]() {
-    if (ahead.left <= 0) return;
-    if (a.block_table != nullptr) req = a.req_id[ahead.x.t];
-    if (a.lens == nullptr) idx_row = a.idx + ahead.x.t * a.idx_st + ahead.x.grp * a.idx_sg;
-  };
-  auto step = [&]() {
-    if (--ahead.left > 0 && ++ahead.x.c == ahead.x.n) {
-      fp4_open(a, ahead.x, ahead.x.unit + 1, kBN);
-      open();
-    }
-  };
-  open();
-  if (lane >= 16) step();
-  int32_t v[3], rq[3], pg[2];  // steps g / 2 .. + 2: entry, request; .. + 1: block-table word
-  auto fetch = [&]() -> int32_t {
-    int32_t e = -1;
-    if (ahead.left > 0) {
-      const int pos = ahead.x.c * kBN + row;
-      if (pos < ahead.x.entries) e = a.lens == nullptr ? idx_row[pos] : pos;
-    }
-    return e;
-  };
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    v[i] = fetch();
-    rq[i] = req;
-    step();
-    step();
-  }
-  pg[0] = fp4_table(a, rq[0], v[0]);
-  pg[1] = fp4_table(a, rq[1], v[1]);
+// Warp pw owns rows [16 pw, +16) of every chunk: lanes 0-15 those of the even
+// chunks of the worker's run, lanes 16-31 of the odd ones.  A run of consecutive
+// slots (the pages of a whole context) is one bulk copy, other rows go four at
+// a time through gather4; masked rows are not read (a group with some fetches
+// row 0 for them) and their bits stay clear.
+__device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, int pw, int lane) {
+  Slots<kBN, 2> slots(a, s.share, blockIdx.x, 16 * pw + (lane & 15), lane >> 4);
+  const int64_t chunks = Walk<kBN>(a, s.share, blockIdx.x).left;
   bool ok = true;
   int64_t armed = 0;
   Ring ring;
   for (int64_t g = 0; g < chunks && ok; g += 2) {
-    const int32_t slot = fp4_slot(a, v[0], pg[0]);
-    v[0] = v[1];
-    v[1] = v[2];
-    rq[1] = rq[2];
-    v[2] = fetch();
-    rq[2] = req;
-    pg[0] = pg[1];
-    pg[1] = fp4_table(a, rq[1], v[1]);
-    step();
-    step();
+    const int32_t slot = slots.next(a);
     const uint32_t live2 = __ballot_sync(0xFFFFFFFFu, slot >= 0);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -323,7 +194,7 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
 
 // q of the unit -> fragments in shared memory.  A half-warp owns a head, lane
 // j of it dims [32 j, +32) and rope dims [4 j, +4).
-__device__ void load_q(const Fp4DecodeArgs& a, Smem& s, const Fp4Cursor& x, int cw, int lane) {
+__device__ void load_q(const Fp4DecodeArgs& a, Smem& s, const Walk<kBN>& x, int cw, int lane) {
   if (cw >= kBH / 2) return;
   const int row = 2 * cw + (lane >> 4), j16 = lane & 15;
   const bool hv = row < min(kBH, a.hpg - x.hb * kBH);
@@ -482,10 +353,10 @@ __device__ __forceinline__ void output_step(const uint8_t* raw, const uint32_t (
   }
 }
 
-__device__ void compute(const Fp4DecodeArgs& a, Smem& s, int64_t per, int cw, int lane) {
+__device__ void compute(const Fp4DecodeArgs& a, Smem& s, int cw, int lane) {
   const int gq = lane >> 2, q4 = lane & 3;
   const int grp = cw / kGWarps, gw = cw % kGWarps;
-  Walk w(a, s, per);
+  Walk<kBN> w(a, s.share, blockIdx.x);
   int pb = 0;
   Ring piece_at;  // stage of the piece's first chunk
   bool ok = true;
@@ -494,7 +365,7 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int64_t per, int cw, in
   const int code_at = 64 * gw + 8 * gq, scale_at = kFp4ScaleOff + 8 * gw + gq;
   while (w.left > 0) {
     const int nch = w.here();
-    load_q(a, s, w.x, cw, lane);
+    load_q(a, s, w, cw, lane);
     compute_sync();
     float acc[16][4];
 #pragma unroll
@@ -632,10 +503,10 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int64_t per, int cw, in
     }
     // ---- the piece: a whole unit goes to the output, a cut one to its slot
     if (grp == 0) {
-      const bool whole = w.x.c == 0 && nch == w.x.n;
-      const int h0 = w.x.grp * a.hpg + w.x.hb * kBH;
-      const int nh = min(kBH, a.hpg - w.x.hb * kBH);
-      const int64_t slot = 2 * (int64_t)blockIdx.x + (w.x.c == 0 ? 1 : 0);
+      const bool whole = w.c == 0 && nch == w.n;
+      const int h0 = w.grp * a.hpg + w.hb * kBH;
+      const int nh = min(kBH, a.hpg - w.hb * kBH);
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (w.c == 0 ? 1 : 0);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int row = gq + 8 * r;
@@ -644,7 +515,7 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int64_t per, int cw, in
         const int d = 128 * gw + 32 * q4;
         if (whole) {
           const float inv = lt[r] > 0.f ? 1.f / lt[r] : (lt[r] == 0.f ? 0.f : lt[r]);
-          uint4* o = reinterpret_cast<uint4*>(a.out + w.x.t * a.out_st + (int64_t)(h0 + row) * a.out_sh + d);
+          uint4* o = reinterpret_cast<uint4*>(a.out + w.t * a.out_st + (int64_t)(h0 + row) * a.out_sh + d);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t v[4];
@@ -655,7 +526,7 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int64_t per, int cw, in
             o[j] = make_uint4(v[0], v[1], v[2], v[3]);
           }
           if (a.lse != nullptr && gw == 0 && q4 == 0)
-            a.lse[w.x.t * a.lse_st + h0 + row] = lt[r] == 0.f ? -INFINITY : (mm[r] - kBias) * kLn2 + logf(lt[r]);
+            a.lse[w.t * a.lse_st + h0 + row] = lt[r] == 0.f ? -INFINITY : (mm[r] - kBias) * kLn2 + logf(lt[r]);
         } else {
           float4* o = reinterpret_cast<float4*>(a.ws_o + (slot * kBH + row) * kNope + d);
 #pragma unroll
@@ -688,26 +559,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (threadIdx.x == 0) pdl_launch_dependents();
   pdl_wait();  // the previous kernel of the stream has completed: global memory from here on
-  const int64_t per = divide_work(a, s);
-  if (threadIdx.x == 0 && a.ws_info != nullptr) {
-    const int64_t at = (int64_t)blockIdx.x * per;
-    int64_t* info = a.ws_info + 4 * blockIdx.x;
-    if (at < s.tok_total) {
-      const int64_t t = s.start_unit / (a.G * a.hb_per_group);
-      info[0] = s.start_unit;
-      info[1] = s.start_chunk;
-      info[2] = fp4_chunks(fp4_entries(a, t), kBN);
-    } else {
-      info[1] = 0;
-    }
-    info[3] = per;
-  }
+  divide<kBN, kThreads>(a, s.share, blockIdx.x);
+  if (threadIdx.x == 0) note_start<kBN>(a, s.share, blockIdx.x);
   if (warp < kCWarps) {
     regs_inc<kCRegs>();
-    compute(a, s, per, warp, lane);
+    compute(a, s, warp, lane);
   } else {
     regs_dec<kPRegs>();
-    produce(a, s, &tm, per, warp - kCWarps, lane);
+    produce(a, s, &tm, warp - kCWarps, lane);
   }
 }
 
@@ -774,8 +633,6 @@ int launch_decode_fp4(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st) {
     return rc;
   return cuts ? launch_merge_fp4(a, kBias, st) : FP8MLA_OK;
 }
-
-int decode_fp4_chunk() { return kBN; }
 
 int read_device_status_fp4(unsigned int* status, bool reset, cudaStream_t st) {
   unsigned int v = 0;

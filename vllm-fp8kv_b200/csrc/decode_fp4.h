@@ -43,61 +43,12 @@ struct Fp4DecodeArgs {
   int block_shift;       // log2(block_size) when it is a power of two, else -1
   int64_t max_len;       // max_blocks * block_size (lens set)
   int64_t per;           // chunks per worker; 0 = from the lengths, on the device
+  int min_per;           // ... but at least this many
   int workers;
   float* ws_o;           // [2 * workers][rows][512] unnormalised partials
   float2* ws_ml;         // [2 * workers][rows] (reference max in log2 units, sum)
   int64_t* ws_info;      // [workers][4]: unit, first chunk in it, its chunks, per
 };
-
-#ifdef __CUDACC__
-// Chunks of one unit of token t.
-__device__ __forceinline__ int fp4_entries(const Fp4DecodeArgs& a, int64_t t) {
-  if (a.lens == nullptr) return a.topk;
-  const int64_t n = a.lens[t];
-  return (int)(n < 0 ? 0 : n > a.max_len ? a.max_len : n);
-}
-__device__ __forceinline__ int fp4_chunks(int entries, int chunk) {
-  return entries > chunk ? (entries + chunk - 1) / chunk : 1;
-}
-
-// A worker's place in the chunk list.
-struct Fp4Cursor {
-  int64_t unit;   // t * (G * hb_per_group) + group * hb_per_group + head block
-  int64_t t;
-  int grp, hb;
-  int c, n;       // chunk within the unit, chunks of the unit
-  int entries;
-};
-__device__ __forceinline__ void fp4_open(const Fp4DecodeArgs& a, Fp4Cursor& x, int64_t unit, int chunk) {
-  const int per_tok = a.G * a.hb_per_group;
-  x.unit = unit;
-  x.t = unit / per_tok;
-  const int r = (int)(unit - x.t * per_tok);
-  x.grp = r / a.hb_per_group;
-  x.hb = r - x.grp * a.hb_per_group;
-  x.c = 0;
-  x.entries = fp4_entries(a, x.t);
-  x.n = fp4_chunks(x.entries, chunk);
-}
-
-// Slot of an entry, in two steps for a pipelined gather: the block-table read
-// first, the arithmetic one step later.  -1: masked, behind the table, or
-// outside the pool.
-__device__ __forceinline__ int32_t fp4_table(const Fp4DecodeArgs& a, int32_t req, int32_t v) {
-  if (a.block_table == nullptr || v < 0) return 0;
-  const int32_t blk = a.block_shift >= 0 ? (v >> a.block_shift) : v / a.block_size;
-  return blk < a.max_blocks ? a.block_table[(int64_t)req * a.bt_stride + blk] : -1;
-}
-__device__ __forceinline__ int32_t fp4_slot(const Fp4DecodeArgs& a, int32_t v, int32_t page) {
-  int64_t s = v;
-  if (a.block_table != nullptr) {
-    if (v < 0 || page < 0) return -1;
-    const int32_t blk = a.block_shift >= 0 ? (v >> a.block_shift) : v / a.block_size;
-    s = (int64_t)page * a.block_size + (v - blk * a.block_size);
-  }
-  return s >= 0 && s < a.num_slots ? (int32_t)s : -1;
-}
-#endif
 
 // Raises a kernel's dynamic shared memory limit, once per device.
 struct SmemLimit {
@@ -117,7 +68,8 @@ struct SmemLimit {
 // be cut, so the merge follows.
 int launch_decode_fp4(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st);
 int launch_merge_fp4(const Fp4DecodeArgs& a, float bias, cudaStream_t st);
-int decode_fp4_chunk();
+constexpr int kFp4Chunk = 64;   // entries per chunk
+constexpr int kFp4MinPer = 3;   // a worker's three groups of warps take a chunk each
 int read_device_status_fp4(unsigned int* status, bool reset, cudaStream_t st);
 
 int launch_fp4_write(const uint16_t* kv_c, int64_t kv_c_stride, const uint16_t* k_pe, int64_t k_pe_stride,
