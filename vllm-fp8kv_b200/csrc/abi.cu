@@ -133,12 +133,13 @@ int fp8mla_device_status(unsigned int* status, int reset, void* stream) {
   *status = 0;
   if (int rc = require_sm100()) return rc;
   // each kernel file keeps its own status word
-  unsigned int v2 = 0, v3 = 0, v4 = 0, v5 = 0;
+  unsigned int v2 = 0, v3 = 0, v4 = 0, v5 = 0, v6 = 0;
   int rc = read_device_status_ws(&v2, reset != 0, static_cast<cudaStream_t>(stream));
   if (rc == FP8MLA_OK) rc = read_device_status_tc3(&v3, reset != 0, static_cast<cudaStream_t>(stream));
   if (rc == FP8MLA_OK) rc = read_device_status_idx(&v4, reset != 0, static_cast<cudaStream_t>(stream));
   if (rc == FP8MLA_OK) rc = read_device_status_fp4(&v5, reset != 0, static_cast<cudaStream_t>(stream));
-  *status = v2 | v3 | v4 | v5;
+  if (rc == FP8MLA_OK) rc = read_device_status_fp4_tc(&v6, reset != 0, static_cast<cudaStream_t>(stream));
+  *status = v2 | v3 | v4 | v5 | v6;
   return rc;
 }
 

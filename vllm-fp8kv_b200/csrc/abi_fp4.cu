@@ -11,21 +11,26 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 constexpr int64_t kMaxTopk = 1LL << 30, kMaxT = 1LL << 24, kMaxH = 1 << 16;
 
+// Heads per kv group from which the paired kernel is used.
+constexpr int64_t kTcHeads = 49;
+
 // How a call's units are dealt out (decode_fp4.h).
 struct Plan {
   int rows, workers, hb_per_group, chunk, min_per;
   int64_t per;  // 0: from the lengths, on the device
   bool cuts;    // some unit may be cut
+  bool tc;      // the paired tensor-core kernel
 };
 // topk < 0: whole contexts, of at most max_len positions
 Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
   Plan p;
   const int64_t hpg = H / G;
-  p.rows = 16;
-  p.workers = device_sm_count();
+  p.tc = hpg >= kTcHeads;
+  p.rows = p.tc ? kFp4TcRows : 16;
+  p.workers = p.tc ? device_sm_count() / 2 : device_sm_count();
   p.hb_per_group = (int)((hpg + p.rows - 1) / p.rows);
-  p.chunk = kFp4Chunk;
-  p.min_per = kFp4MinPer;
+  p.chunk = p.tc ? kFp4TcChunk : kFp4Chunk;
+  p.min_per = p.tc ? 1 : kFp4MinPer;
   const int64_t chunk = p.chunk, units = T * G * p.hb_per_group;
   const int64_t len = topk < 0 ? max_len : topk;
   const int64_t n = len > chunk ? (len + chunk - 1) / chunk : 1;  // chunks of a unit (at most)
@@ -138,7 +143,8 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
     a.ws_ml = reinterpret_cast<float2*>(ws + part_bytes(p) + info_bytes(p));
   }
 
-  return launch_decode_fp4(a, p.cuts, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return p.tc ? launch_decode_fp4_tc(a, p.cuts, st) : launch_decode_fp4(a, p.cuts, st);
 }
 
 }  // namespace
@@ -198,7 +204,7 @@ int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t topk
 
 const char* fp8mla_fp4_kernel_name(int64_t H, int64_t G) {
   if (H <= 0 || G <= 0 || H % G != 0) return "";
-  return "decode_fp4_kernel";
+  return H / G >= kTcHeads ? "decode_fp4_tc_kernel" : "decode_fp4_kernel";
 }
 
 int fp8mla_fp4_sparse_decode(const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t, int64_t q_stride_h,

@@ -45,7 +45,6 @@ constexpr int kThreads = 32 * (kCWarps + kPWarps);
 constexpr int kCRegs = 152, kPRegs = 56;  // launched with 128 each
 static_assert(kCWarps * kCRegs + kPWarps * kPRegs <= (kCWarps + kPWarps) * 128, "register split");
 constexpr int kQSteps = kDqk / 16;        // 36: 32 of the latents, 4 of the rope
-constexpr int kRowsPerPWarp = kBN / kPWarps;  // 16
 constexpr float kRescale = 8.0f;  // the reference maximum lags by at most 2^8 ...
 constexpr float kBias = 6.0f;     // ... and P is stored times 2^6: below 2^14 in
                                   // fp16, above its smallest value from 2^-30 on

@@ -1,0 +1,748 @@
+// decode_fp4_tc.cu -- attention over fp4_ds_mla rows for many heads: up to 128
+// query heads per unit on a pair of SMs (a 2-CTA cluster) that share
+// cta_group::2 tcgen05 MMAs.
+//
+//   S = scale q . [latent | rope],  P = softmax(S),  O = P . latent
+//
+// The pair splits the heads: CTA c owns heads [64c, +64) and its tensor memory
+// holds their S and O.  A tile is 128 entries and an MMA spans both SMs:
+//   S    M=128 heads, N=128 entries, K=576 (36 k-steps); CTA c supplies the rows
+//        of its "own" entries [64c, +64)
+//   O    M=128 heads, N=256 dims (two MMAs for the 512), K=128 entries; CTA c
+//        supplies dims [128c, +128) of each MMA (latent tiles c and c + 2, its
+//        "half") of all 128 entries
+// An M=128 pair MMA costs about 45 cycles up to N=128 and 64 at N=256 (measured),
+// so the issuing thread's stream, not the arithmetic, is what bounds such a
+// kernel: 128-entry tiles need 52 MMAs per 128 entries, 64-entry tiles 88.  What
+// makes room for them in shared memory (K own rows 72 KB, V halves 64 KB, both
+// in fp16 and single) is the 4-bit rows, whose ring takes 39 KB, and letting each
+// buffer drain in parts: K in two groups of blocks, refilled for the next tile
+// while the other group and the O product of the tile before are still running; V while the
+// next tile's S runs.
+//
+// The latents are exact in fp16 (fp4.cuh), so the 32 latent k-steps of S and the
+// O product are fp16 MMAs: q is scaled per head by a power of two to a largest
+// value in [2^8, 2^9) and converted, and P keeps 11 bits where bf16 keeps 8.  The
+// rope's four k-steps are bf16 MMAs (q's rope times the same power of two) into
+// the same accumulator.
+//
+// Units are dealt to the pairs in equal runs of tiles (decode_fp4.h).  Every role
+// walks the run on its own; only q, the softmax state and O change at unit
+// borders, and the next unit's q is in place before the last unit's O is stored.
+//
+// Accumulator layout of an M=128 pair MMA (measured): per CTA, lanes [0,64) hold
+// its 64 rows x columns [0, N/2), lanes [64,128) the same rows x [N/2, N).  So
+// softmax thread L owns head L & 63 and entries [64 (L >> 6), +64) of a tile.
+//
+// Tensor memory (512 columns, both CTAs):
+//   [  0,256)  O, dims [0,256) MMA in [0,128), dims [256,512) MMA in [128,256)
+//   [256,320)  S
+//   [320,512)  q dims [0,384), the A operand of 24 k-steps (lanes L and L^64
+//              hold the same head)
+// Shared memory (about 218 KB):
+//   q    dims [384,512) fp16, rope bf16: 3 x 64-dim swizzled blocks of 64 rows  24 KB
+//   k    own 64 entries x 576 dims, 9 blocks of 64 rows                         72 KB
+//   v    128 entries x this CTA's half, 4 blocks of 128 rows                    64 KB
+//   p    P of 64 heads x 128 entries, 2 blocks                                  16 KB
+//   raw  a ring of 3 units of 8 own rows per K warp, as copied by TMA            39 KB
+//
+// Warp roles (512 threads per CTA; warp w runs on SM sub-partition w % 4):
+//   warps 0-3         softmax, q, and the stores of O
+//   warp 4            tensor memory allocation; lane 0 of the even CTA issues
+//                     every MMA of the pair
+//   warps 5, 6, 7, 9  K: own rows [16i, +16) of every tile, raw ring -> K blocks
+//   warps 10, 11, 13, 14
+//                     V: entries [32i, +32) of every tile, the half's codes and
+//                     scales by register loads one tile ahead -> V blocks; and
+//                     the tile's live bits
+//   warps 8, 15       producers: entries -> slots -> TMA copies, 32 own rows each
+//   warp 12           idle
+// Barriers that gate the issuing thread live in the even CTA and count arrivals
+// of both CTAs; the completion of pair MMAs reaches both CTAs through a multicast
+// commit.  Every wait is bounded; after a failed wait a role stops, and the
+// producers wait (with the full limit) for the copies they issued, so none
+// outlives the CTA.  No load uses cluster multicast.
+#include "decode_fp4.h"
+#include "fp4.cuh"
+#include "fp4_walk.cuh"
+#include "tc_cluster.cuh"
+#include "tc_ptx.cuh"
+#include "tma_map.h"
+
+namespace fp8mla {
+namespace {
+using namespace fp8mla::fp4;
+using namespace fp8mla::tc;
+
+constexpr int kN = kFp4TcChunk;            // 128 entries per tile
+constexpr int kOwn = kN / 2;
+constexpr int kQTmemSteps = 24;            // q dims [0,384) from tensor memory
+constexpr int kQBlockBytes = 64 * 128;
+constexpr int kKBlockBytes = kOwn * 128;   // 8 KB: 64 own rows of a 64-dim block
+constexpr int kVBlockBytes = kN * 128;     // 16 KB
+constexpr int kPBlockBytes = 64 * 128;     // 64 heads x 64 entries
+constexpr int kUnitRows = 8;               // rows of a raw unit: half of a K warp's rows of a tile
+constexpr int kUnitBytes = kUnitRows * kFp4RowBytes;  // 3328 = 26 * 128
+constexpr int kUnits = 3;                  // per K warp: a ring of its own, so that every
+                                           // waiter sees every phase of its barriers
+constexpr int kMaskSlots = 4;
+constexpr int kSoftmaxWarps = 4, kKWarps = 4, kVWarps = 4;
+constexpr int kMmaWarp = 4;
+constexpr int kThreads = 16 * 32;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320;
+constexpr float kRescale = 8.0f;  // the reference maximum lags by at most 2^8 ...
+constexpr float kBias = 6.0f;     // ... and P is stored times 2^6: below 2^14 in
+                                  // fp16, above its smallest value from 2^-30 on
+
+constexpr uint32_t idesc(int n, bool bf16, bool b_mn_major) {
+  return bf16 ? idesc_bf16(128, n, b_mn_major)
+              : idesc_bf16(128, n, b_mn_major) & ~((1u << 7) | (1u << 10));
+}
+constexpr uint32_t kIdescLatent = idesc(kN, false, false);
+constexpr uint32_t kIdescRope = idesc(kN, true, false);
+constexpr uint32_t kIdescPV = idesc(256, false, true);
+
+struct Smem {
+  uint8_t q[3 * kQBlockBytes];  // 1024-aligned (offset 0)
+  uint8_t k[9 * kKBlockBytes];
+  uint8_t v[4 * kVBlockBytes];
+  uint8_t p[2 * kPBlockBytes];
+  uint8_t raw[kKWarps][kUnits][kUnitBytes];
+  float half_max[2][128];       // a tile's maxima per thread, by tile parity
+  float lsum[128];
+  uint32_t qmax[2][128];        // largest magnitudes of q's halves: latents, rope
+  uint32_t vmask[kMaskSlots][4];  // a tile's live bits
+  uint64_t raw_full[kKWarps][kUnits], raw_empty[kKWarps][kUnits];
+  uint64_t kfull[2], kempty[2];  // K blocks [0,4) and [4,9); kfull: even CTA
+  uint64_t vfull, pfull, sempty, qready, oempty;  // even CTA, both CTAs arrive
+  uint64_t sfull, pvdone, ofull, drain;           // commits
+  uint64_t mfull[kMaskSlots];
+  uint64_t meet;                // the softmax warps of this CTA
+  Share share;
+  uint32_t tmem_base;
+};
+static_assert(offsetof(Smem, k) % 1024 == 0 && offsetof(Smem, v) % 1024 == 0 && offsetof(Smem, p) % 1024 == 0,
+              "swizzle atoms need 1024-B alignment");
+static_assert(offsetof(Smem, raw) % 128 == 0 && kUnitBytes % 128 == 0, "TMA destinations");
+static_assert(offsetof(Smem, raw_full) % 8 == 0, "");
+static_assert(sizeof(Smem) + 1024 <= 227 * 1024, "shared memory budget");
+
+__device__ __forceinline__ uint32_t swz(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
+
+struct Ctx {
+  const Fp4DecodeArgs* a;
+  Smem* s;
+  int worker;
+  uint32_t rank, tmem;
+  int64_t tiles;  // of this worker
+};
+__device__ __forceinline__ uint32_t bar(uint64_t& b) { return smem_u32(&b); }
+
+// ------------------------------------------------------------------ MMA issuer (even CTA)
+template <int kFrom, int kTo>
+__device__ __forceinline__ void issue_s(uint32_t tS, uint32_t tQ, uint64_t qdesc0, uint64_t kdesc0) {
+#pragma unroll
+  for (int kst = kFrom; kst < kTo; ++kst) {
+    const uint64_t bdesc = kdesc0 + (uint64_t)(((kst >> 2) * kKBlockBytes + (kst & 3) * 32) >> 4);
+    if (kst < kQTmemSteps) {
+      mma_pair_ts(tS, tQ + 8 * kst, bdesc, kIdescLatent, kst > 0 ? 1u : 0u);
+    } else {
+      const int qs = kst - kQTmemSteps;
+      const uint64_t adesc = qdesc0 + (uint64_t)(((qs >> 2) * kQBlockBytes + (qs & 3) * 32) >> 4);
+      mma_pair_ss(tS, adesc, bdesc, kst < 32 ? kIdescLatent : kIdescRope, 1u);
+    }
+  }
+}
+
+__device__ void mma_role(const Ctx& c) {
+  Smem& s = *c.s;
+  const uint32_t tQ = c.tmem + kColQ, tS = c.tmem + kColS;
+  const uint64_t qdesc0 = sdesc_sw128(smem_u32(s.q), 16, 1024);
+  const uint64_t kdesc0 = sdesc_sw128(smem_u32(s.k), 16, 1024);
+  const uint64_t pdesc0 = sdesc_sw128(smem_u32(s.p), 16, 1024);
+  const uint64_t vdesc0 = sdesc_sw128(smem_u32(s.v), kVBlockBytes, 1024);
+  Walk<kN> w(*c.a, s.share, c.worker);
+  bool ok = true;
+  uint32_t j = 0;                     // tile of the run
+  bool first = false, last = false;   // tile j - 1 opens / closes its piece
+  uint32_t piece = 0;                 // piece of tile j - 1
+  // O of tile j - 1
+  auto issue_o = [&]() {
+    if (!ok) return;
+    if (first && piece > 0) ok = thread_wait_cluster(bar(s.oempty), (piece - 1) & 1, 45);
+    if (ok) ok = thread_wait_cluster(bar(s.pfull), (j - 1) & 1, 36);
+    if (ok) ok = thread_wait_cluster(bar(s.vfull), (j - 1) & 1, 38);
+    if (!ok) return;
+    tc_fence_after();
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int kk = 0; kk < kN / 16; ++kk)
+        mma_pair_ss(c.tmem + kColO + 128 * hf,
+                    pdesc0 + (uint64_t)(((kk >> 2) * kPBlockBytes + (kk & 3) * 32) >> 4),
+                    vdesc0 + (uint64_t)((hf * 2 * kVBlockBytes + kk * 16 * 128) >> 4), kIdescPV,
+                    (kk > 0 || !first) ? 1u : 0u);
+    mma_commit_pair(bar(s.pvdone));  // P and V may be written again
+    if (last) mma_commit_pair(bar(s.ofull));
+  };
+  uint32_t p = 0;
+  while (w.left > 0 && ok) {
+    const int n = w.here();
+    ok = thread_wait_cluster(bar(s.qready), p & 1, 35);
+    for (int i = 0; i < n && ok; ++i) {
+      if (j > 0) ok = thread_wait_cluster(bar(s.sempty), (j - 1) & 1, 34);
+      if (ok) ok = thread_wait_cluster(bar(s.kfull[0]), j & 1, 37);
+      if (!ok) break;
+      tc_fence_after();
+      issue_s<0, 16>(tS, tQ, qdesc0, kdesc0);
+      mma_commit_pair(bar(s.kempty[0]));
+      ok = thread_wait_cluster(bar(s.kfull[1]), j & 1, 39);
+      if (!ok) break;
+      tc_fence_after();
+      issue_s<16, 36>(tS, tQ, qdesc0, kdesc0);
+      mma_commit_pair(bar(s.kempty[1]));
+      mma_commit_pair(bar(s.sfull));
+      if (j > 0) issue_o();
+      first = i == 0;
+      last = i == n - 1;
+      piece = p;
+      ++j;
+    }
+    ++p;
+    w.next_unit(*c.a, n);
+  }
+  if (j > 0) issue_o();
+  // drain: nothing this thread issued may still touch either CTA's memory
+  mma_commit_pair(bar(s.drain));
+  thread_wait_cluster(bar(s.drain), 0, 46);
+}
+
+// ------------------------------------------------------------------ producers
+// Place in a K warp's ring of units, and the times it was gone around.
+struct UnitRing {
+  int u = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void next() {
+    if (++u == kUnits) {
+      u = 0;
+      ++round;
+    }
+  }
+};
+
+// Producer pw copies own rows [32 pw, +32) of every tile (lane = row) for K warps
+// 2 pw and 2 pw + 1: unit h of warp i holds the rows of lanes [16 i + 8 h, +8).
+__device__ void produce(const Ctx& c, const CUtensorMap* tm, int pw, int lane) {
+  const Fp4DecodeArgs& a = *c.a;
+  Smem& s = *c.s;
+  Slots<kN, 1> slots(a, s.share, c.worker, kOwn * (int)c.rank + 32 * pw + lane, 0);
+  bool ok = true;
+  int64_t armed[2] = {0, 0};
+  UnitRing ring;
+  for (int64_t j = 0; j < c.tiles && ok; ++j) {
+    const int32_t slot = slots.next(a);
+    const uint32_t live4 = __ballot_sync(0xFFFFFFFFu, slot >= 0);
+    const int32_t row = slot >= 0 ? slot : 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int l0 = 16 * i + 8 * h, kw = 2 * pw + i;
+        if (ok && ring.round > 0) ok = warp_wait(bar(s.raw_empty[kw][ring.u]), (ring.round - 1) & 1, 40);
+        if (!ok) break;
+        const uint32_t live = (live4 >> l0) & 0xFFu;
+        const int n = __popc(live);
+        const int32_t s0 = __shfl_sync(0xFFFFFFFFu, slot, l0);
+        // consecutive slots: one bulk copy; else the groups of four rows with a live one
+        const bool run = (live & (live + 1)) == 0 &&
+                         __all_sync(0xFFFFFFFFu, (lane & 24) != l0 || slot < 0 || slot == s0 + (lane & 7));
+        const uint32_t grp = (live & 0xFu ? 1u : 0u) | (live & 0xF0u ? 2u : 0u);
+        const uint32_t full = bar(s.raw_full[kw][ring.u]);
+        const uint32_t dst = smem_u32(s.raw[kw][ring.u]);
+        if (lane == 0)
+          mbar_arrive_expect_tx(full, run ? (uint32_t)(n * kFp4RowBytes) : (uint32_t)(__popc(grp) * 4 * kFp4RowBytes));
+        __syncwarp();
+        if (run) {
+          if (lane == 0 && n > 0) bulk_g2s(dst, a.kv + (int64_t)s0 * kFp4RowBytes, (uint32_t)(n * kFp4RowBytes), full);
+        } else {
+          const int src = l0 + ((4 * lane) & 7);
+          const int32_t r0 = __shfl_sync(0xFFFFFFFFu, row, src);
+          const int32_t r1 = __shfl_sync(0xFFFFFFFFu, row, src + 1);
+          const int32_t r2 = __shfl_sync(0xFFFFFFFFu, row, src + 2);
+          const int32_t r3 = __shfl_sync(0xFFFFFFFFu, row, src + 3);
+          if (lane < 2 && ((grp >> lane) & 1u)) tma_gather4(dst + lane * 4 * kFp4RowBytes, tm, 0, r0, r1, r2, r3, full);
+        }
+        ++armed[i];
+      }
+      if (!ok) break;
+      ring.next();
+    }
+  }
+  // the units armed last have landed before the warp returns, even after a
+  // failed wait
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    for (int64_t x = armed[i] > kUnits ? armed[i] - kUnits : 0; x < armed[i]; ++x)
+      (void)warp_wait(bar(s.raw_full[2 * pw + i][x % kUnits]), (uint32_t)(x / kUnits) & 1, 41);
+}
+
+// ------------------------------------------------------------------ K and V
+// Lane -> (row of 8, 32-dim quarter of a 128-dim latent tile): eight lanes that
+// store or load together cover four rows and two quarters, which touch every
+// bank once in the swizzled blocks and in the 416-byte rows alike.
+__device__ __forceinline__ int lane_row(int lane) { return (lane & 3) + 4 * ((lane >> 3) & 1); }
+__device__ __forceinline__ int lane_quarter(int lane) { return ((lane >> 2) & 1) + 2 * ((lane >> 4) & 1); }
+
+// 32 codes and their two scales -> four 16-byte chunks of fp16 at `at` (the
+// shared address of the first, swizzled: the others differ from it in bits 4 and
+// 5).  Not inlined: one copy serves every use.
+__device__ __noinline__ void unpack32(uint4 w, uint32_t scales, uint32_t at) {
+  const uint32_t s2 = e4m3x2_to_f16(scales);
+  const uint32_t sl = __byte_perm(s2, 0, 0x1010), sh = __byte_perm(s2, 0, 0x3232);
+  const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h[4];
+    e2m1x8_to_f16(word[i], h);
+    const uint32_t sc = i < 2 ? sl : sh;
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at ^ (16u * i)), "r"(mul_f16x2(h[0], sc)),
+                 "r"(mul_f16x2(h[1], sc)), "r"(mul_f16x2(h[2], sc)), "r"(mul_f16x2(h[3], sc))
+                 : "memory");
+  }
+}
+
+// K warp kw: own rows [16 kw, +16) of every tile.  Rows that were not copied
+// (masked) leave what the ring held: their scores are replaced in the softmax.
+__device__ void k_role(const Ctx& c, int kw, int lane) {
+  Smem& s = *c.s;
+  const int r8 = lane_row(lane), q = lane_quarter(lane);
+  bool ok = true;
+  UnitRing ring;
+  for (int64_t j = 0; j < c.tiles && ok; ++j) {
+    // both units into registers, and back to the producer
+    uint4 w[2][4], rope[2][2];
+    uint32_t sc[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t full = bar(s.raw_full[kw][ring.u]);
+      if (ok) ok = warp_wait(full, ring.round & 1, 42);
+      if (!ok) break;
+      (void)mbar_try_wait(full, ring.round & 1);  // every lane acquires
+      const uint8_t* row = s.raw[kw][ring.u] + r8 * kFp4RowBytes;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        w[h][t] = *reinterpret_cast<const uint4*>(row + 64 * t + 16 * q);
+        sc[h][t] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * t + 2 * q);
+      }
+      rope[h][0] = *reinterpret_cast<const uint4*>(row + kFp4RopeOff + 32 * q);
+      rope[h][1] = *reinterpret_cast<const uint4*>(row + kFp4RopeOff + 32 * q + 16);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(s.raw_empty[kw][ring.u]));
+      ring.next();
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {  // blocks [0,4): latent tiles 0, 1; blocks [4,9): 2, 3 and the rope
+      if (ok && j > 0) ok = warp_wait_cluster(bar(s.kempty[g]), (uint32_t)(j - 1) & 1, 43);
+      if (!ok) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t r = 16 * kw + 8 * h + r8;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          unpack32(w[h][2 * g + t], sc[h][2 * g + t],
+                   smem_u32(s.k + (4 * g + 2 * t + (q >> 1)) * kKBlockBytes + swz(r, 4 * (q & 1))));
+        if (g == 1) {
+          *reinterpret_cast<uint4*>(s.k + 8 * kKBlockBytes + swz(r, 2 * q)) = rope[h][0];
+          *reinterpret_cast<uint4*>(s.k + 8 * kKBlockBytes + swz(r, 2 * q + 1)) = rope[h][1];
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(bar(s.kfull[g]), 0);
+    }
+  }
+}
+
+// V warp vw: entries [32 vw, +32) of every tile, the CTA's half.
+__device__ void v_role(const Ctx& c, int vw, int lane) {
+  const Fp4DecodeArgs& a = *c.a;
+  Smem& s = *c.s;
+  const int r8 = lane_row(lane), q = lane_quarter(lane), cr = (int)c.rank;
+  Slots<kN, 1> slots(a, s.share, c.worker, 32 * vw + lane, 0);
+  uint4 w[4][2];
+  uint32_t sc[4];  // the two scales of each tile half
+  uint32_t live = 0;
+  auto load = [&]() {
+    const int32_t slot = slots.next(a);
+    live = __ballot_sync(0xFFFFFFFFu, slot >= 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t sl = __shfl_sync(0xFFFFFFFFu, slot, 8 * i + r8);
+      if (sl >= 0) {
+        const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
+        w[i][0] = ldg_v4(row + 64 * cr + 16 * q);
+        w[i][1] = ldg_v4(row + 64 * (cr + 2) + 16 * q);
+        sc[i] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * cr + 2 * q) |
+                ((uint32_t)*reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * (cr + 2) + 2 * q) << 16);
+      } else {  // zeros: P is 0 there, and nothing else may be
+        w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
+        sc[i] = 0;
+      }
+    }
+  };
+  if (c.tiles > 0) load();
+  for (int64_t j = 0; j < c.tiles; ++j) {
+    // The slot's reader of tile j - 4 is done: this warp saw O of tile j - 2
+    // complete before it wrote V of tile j - 1.
+    if (lane == 0) {
+      s.vmask[j % kMaskSlots][vw] = live;
+      mbar_arrive(bar(s.mfull[j % kMaskSlots]));
+    }
+    if (j > 0 && !warp_wait_cluster(bar(s.pvdone), (uint32_t)(j - 1) & 1, 44)) break;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = 32 * vw + 8 * i + r8;
+      const uint32_t at = smem_u32(s.v + (q >> 1) * kVBlockBytes + swz(r, 4 * (q & 1)));
+      unpack32(w[i][0], sc[i] & 0xFFFFu, at);
+      unpack32(w[i][1], sc[i] >> 16, at + 2 * kVBlockBytes);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(bar(s.vfull), 0);
+    if (j + 1 < c.tiles) load();  // behind the fence, so that it waits for no load
+  }
+}
+
+// ------------------------------------------------------------------ softmax
+// The four softmax warps of a CTA meet, with a bounded wait (a warp that gave up
+// elsewhere never comes).
+struct Meet {
+  uint32_t n = 0;
+  __device__ __forceinline__ bool operator()(Smem& s, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(s.meet));
+    const bool ok = warp_wait(bar(s.meet), n & 1, 47);
+    if (ok) (void)mbar_try_wait(bar(s.meet), n & 1);
+    ++n;
+    return ok;
+  }
+};
+
+// q of the unit: dims [0,384) -> tensor memory (lanes L and L^64 both hold head
+// L & 63), the rest -> swizzled shared memory (thread hh writes chunks [4 hh, +4)
+// of each block); padding rows are zero.  `scale` turns the head's accumulators
+// into scores in log2 units.
+__device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, Meet& meet, float& scale) {
+  const Fp4DecodeArgs& a = *c.a;
+  Smem& s = *c.s;
+  const int m = L & 63, hh = L >> 6;
+  const int head = w.hb * a.rows + 64 * (int)c.rank + m;  // of its group
+  const bool hv = 64 * (int)c.rank + m < a.rows && head < a.hpg;
+  const uint4* src = reinterpret_cast<const uint4*>(a.q + w.t * a.q_st +
+                                                    (int64_t)(w.grp * a.hpg + (hv ? head : 0)) * a.q_sh);
+  const uint4 z4 = make_uint4(0, 0, 0, 0);
+  auto mag = [](const uint4& v) {
+    return __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+  };
+  // largest magnitudes (as bits): each thread half of the latents and of the rope
+  uint32_t mx = 0, mr = 0;
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i) mx = __vmaxu2(mx, mag(hv ? src[32 * hh + i] : z4));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mr = __vmaxu2(mr, mag(hv ? src[64 + 4 * hh + i] : z4));
+  s.qmax[0][L] = max(mx & 0xFFFFu, mx >> 16);
+  s.qmax[1][L] = max(mr & 0xFFFFu, mr >> 16);
+  if (!meet(s, L & 31)) return false;
+  const int bm = (int)max(s.qmax[0][L], s.qmax[0][L ^ 64]), br = (int)max(s.qmax[1][L], s.qmax[1][L ^ 64]);
+  // 2^k brings the latent part's largest value to [2^8, 2^9), but the rope's at
+  // most to 2^101, where its products are still finite; 1 for rows of zeros, inf
+  // or NaN.  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.
+  int k = min(8 - ((bm >> 7) - 127), 100 - ((br >> 7) - 127));
+  k = (bm == 0 || bm >= 0x7F80) ? 0 : min(126, k);
+  const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+  auto f16 = [&](uint32_t v) { return pack_f16x2(bf16_lo(v) * up, bf16_hi(v) * up); };
+  auto bf = [&](uint32_t v) { return pack_bf16x2(bf16_lo(v) * up, bf16_hi(v) * up); };
+#pragma unroll
+  for (int b = 0; b < 3; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = hv ? src[48 + 8 * b + 4 * hh + i] : z4;
+      *reinterpret_cast<uint4*>(s.q + b * kQBlockBytes + swz(m, 4 * hh + i)) =
+          b < 2 ? make_uint4(f16(v.x), f16(v.y), f16(v.z), f16(v.w)) : make_uint4(bf(v.x), bf(v.y), bf(v.z), bf(v.w));
+    }
+  const uint32_t trow = c.tmem + ((uint32_t)((L >> 5) * 32) << 16);
+#pragma unroll 1
+  for (int c0 = 0; c0 < 192; c0 += 32) {
+    uint32_t o[32];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 v = hv ? src[c0 / 4 + i] : z4;
+      o[4 * i] = f16(v.x);
+      o[4 * i + 1] = f16(v.y);
+      o[4 * i + 2] = f16(v.z);
+      o[4 * i + 3] = f16(v.w);
+    }
+    tmem_st32(trow + kColQ + c0, o);
+  }
+  tmem_wait_st();
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncwarp();
+  if ((L & 31) == 0) mbar_arrive_cluster(bar(s.qready), 0);
+  scale = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+  return true;
+}
+
+__device__ void softmax_role(const Ctx& c, int warp, int lane) {
+  const Fp4DecodeArgs& a = *c.a;
+  Smem& s = *c.s;
+  const int L = threadIdx.x, m = L & 63, hh = L >> 6;
+  const uint32_t trow = c.tmem + ((uint32_t)(warp * 32) << 16);
+  Walk<kN> w(a, s.share, c.worker);
+  bool ok = true;
+  uint32_t j = 0, piece = 0;
+  float scale = 0.f;
+  Meet meet;
+  if (w.left > 0) ok = load_q(c, w, L, meet, scale);
+  while (w.left > 0 && ok) {
+    const int n = w.here();
+    float m_ref = -INFINITY, l = 0.f;
+    for (int i = 0; i < n; ++i, ++j) {
+      const uint32_t par = j & 1;
+      ok = warp_wait_cluster(bar(s.sfull), par, 31);
+      const uint32_t mslot = j % kMaskSlots, mpar = (j / kMaskSlots) & 1;
+      if (ok) ok = warp_wait(bar(s.mfull[mslot]), mpar, 30);
+      if (!ok) break;
+      (void)mbar_try_wait(bar(s.mfull[mslot]), mpar);
+      tc_fence_after();
+      // two passes over the 64 scores, 32 at a time (half the code): the maximum ...
+      float pm = -INFINITY;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sv[32];
+        tmem_ld32(trow + kColS + 32 * h, sv);
+        const uint32_t live = s.vmask[mslot][2 * hh + h];
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) pm = fmaxf(pm, (live >> e) & 1u ? __uint_as_float(sv[e]) * scale : -INFINITY);
+      }
+      s.half_max[par][L] = pm;
+      ok = meet(s, lane);
+      if (!ok) break;
+      const float tmax = fmaxf(pm, s.half_max[par][L ^ 64]);
+      float alpha = 1.f;
+      if (tmax > m_ref + kRescale || (m_ref == -INFINITY && tmax > -INFINITY)) {
+        alpha = m_ref == -INFINITY ? 1.f : ex2_approx(m_ref - tmax);
+        m_ref = tmax;
+        l *= alpha;
+      }
+      const float sub = m_ref == -INFINITY ? 0.f : m_ref - kBias;
+      // O of the tile before has read P (and is complete, should it be rescaled)
+      if (j > 0) ok = warp_wait_cluster(bar(s.pvdone), (j - 1) & 1, 33);
+      if (!ok) break;
+      if (__any_sync(0xFFFFFFFFu, alpha != 1.f) && i > 0) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int c0 = 0; c0 < 256; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32(trow + kColO + c0, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(trow + kColO + c0, o);
+        }
+        tmem_wait_st();
+      }
+      // ... then P
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sv[32];
+        tmem_ld32(trow + kColS + 32 * h, sv);
+        const uint32_t live = s.vmask[mslot][2 * hh + h];
+        tmem_wait_ld();
+        if (h == 1) {  // S may be written again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(bar(s.sempty), 0);
+        }
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float p0 = ex2_approx(fmaf(__uint_as_float(sv[2 * e]), scale, -sub));
+          float p1 = ex2_approx(fmaf(__uint_as_float(sv[2 * e + 1]), scale, -sub));
+          p0 = (live >> (2 * e)) & 1u ? p0 : 0.f;
+          p1 = (live >> (2 * e + 1)) & 1u ? p1 : 0.f;
+          l += p0 + p1;
+          pk[e] = pack_f16x2(p0, p1);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(s.p + hh * kPBlockBytes + swz(m, 4 * h + e)) =
+              make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(bar(s.pfull), 0);
+    }
+    if (!ok) break;
+    // ---- the piece: its sums, the next unit's q, then its O
+    s.lsum[L] = l;
+    ok = meet(s, lane);
+    if (!ok) break;
+    const float lt = l + s.lsum[L ^ 64];
+    const bool whole = w.c == 0 && n == w.n;
+    const int64_t t = w.t;
+    const int head = w.hb * a.rows + 64 * (int)c.rank + m;
+    const bool hv = 64 * (int)c.rank + m < a.rows && head < a.hpg;
+    const int64_t hg = (int64_t)w.grp * a.hpg + head;
+    const int64_t prow = (2 * (int64_t)c.worker + (w.c == 0 ? 1 : 0)) * a.rows + 64 * (int)c.rank + m;
+    w.next_unit(a, n);
+    if (w.left > 0) ok = load_q(c, w, L, meet, scale);
+    if (ok) ok = warp_wait_cluster(bar(s.ofull), piece & 1, 32);
+    if (!ok) break;
+    tc_fence_after();
+    const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+    if (hv && hh == 0) {
+      if (whole) {
+        if (a.lse != nullptr)
+          a.lse[t * a.lse_st + hg] = lt == 0.f ? -INFINITY : (m_ref - kBias) * kLn2 + logf(lt);
+      } else {
+        a.ws_ml[prow] = make_float2(m_ref, lt);
+      }
+    }
+#pragma unroll 1
+    for (int c0 = 0; c0 < 256; c0 += 32) {
+      uint32_t o[32];
+      tmem_ld32(trow + kColO + c0, o);
+      tmem_wait_ld();
+      const int d = 256 * (c0 >> 7) + 128 * hh + (c0 & 127);
+      if (hv && whole) {
+        uint4* dst = reinterpret_cast<uint4*>(a.out + t * a.out_st + hg * a.out_sh + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t v[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            v[x] = pack_bf16x2(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
+          dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      } else if (hv) {
+        uint4* dst = reinterpret_cast<uint4*>(a.ws_o + prow * kNope + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(bar(s.oempty), 0);
+    ++piece;
+  }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    decode_fp4_tc_kernel(const Fp4DecodeArgs a, const __grid_constant__ CUtensorMap tm) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw + (((raw_base + 1023u) & ~1023u) - raw_base));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Ctx c;
+  c.a = &a;
+  c.s = &s;
+  c.worker = blockIdx.x >> 1;
+  c.rank = cluster_rank();  // == blockIdx.x & 1
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kKWarps * kUnits; ++i) {
+      mbar_init(bar(s.raw_full[0][i]), 1);
+      mbar_init(bar(s.raw_empty[0][i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(s.kfull[i]), 2 * kKWarps);
+      mbar_init(bar(s.kempty[i]), 1);
+    }
+    for (int i = 0; i < kMaskSlots; ++i) mbar_init(bar(s.mfull[i]), kVWarps);
+    mbar_init(bar(s.vfull), 2 * kVWarps);
+    mbar_init(bar(s.pfull), 2 * kSoftmaxWarps);
+    mbar_init(bar(s.sempty), 2 * kSoftmaxWarps);
+    mbar_init(bar(s.qready), 2 * kSoftmaxWarps);
+    mbar_init(bar(s.oempty), 2 * kSoftmaxWarps);
+    mbar_init(bar(s.sfull), 1);
+    mbar_init(bar(s.pvdone), 1);
+    mbar_init(bar(s.ofull), 1);
+    mbar_init(bar(s.drain), 1);
+    mbar_init(bar(s.meet), kSoftmaxWarps);
+    mbar_init_fence();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc_pair(smem_u32(&s.tmem_base), kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // barriers of both CTAs initialised, tensor memory allocated
+  tc_fence_after();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  pdl_wait();  // the previous kernel of the stream has completed: global memory from here on
+  c.tmem = s.tmem_base;
+  divide<kN, kThreads>(a, s.share, c.worker);
+  if (threadIdx.x == 0 && c.rank == 0) note_start<kN>(a, s.share, c.worker);
+  c.tiles = Walk<kN>(a, s.share, c.worker).left;
+
+  // one call per role: the loops of all roles together have to stay in the SM's
+  // instruction cache (with each role inlined twice, and the unpacking and the
+  // softmax unrolled in full, warps waited for instructions most of the time:
+  // 182 instead of TODO us at 64 x 128 heads x top-2048)
+  if (warp < kSoftmaxWarps) {
+    softmax_role(c, warp, lane);
+  } else if (warp == kMmaWarp) {
+    if (c.rank == 0 && lane == 0) mma_role(c);
+  } else if (warp < 8 || warp == 9) {
+    k_role(c, warp < 8 ? warp - 5 : 3, lane);
+  } else if (warp == 8 || warp == 15) {
+    produce(c, &tm, warp == 8 ? 0 : 1, lane);
+  } else if (warp != 12) {
+    v_role(c, warp < 12 ? warp - 10 : warp - 11, lane);
+  }
+
+  // both CTAs: no MMA of the pair may still run, no arrival may still target the
+  // other CTA, before tensor memory is freed and the CTAs exit
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc_pair(c.tmem, kTmemCols);
+  }
+}
+
+}  // namespace
+
+int launch_decode_fp4_tc(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st) {
+  CUtensorMap tm{};
+  if (a.num_slots > 0)
+    if (int rc = encode_fp4_row_map(&tm, a.kv, a.num_slots)) return rc;
+  const size_t smem = sizeof(Smem) + 1024;  // + alignment slack
+  static SmemLimit limit;
+  if (int rc = limit.raise(decode_fp4_tc_kernel, smem)) return rc;
+  if (int rc = check_cuda(launch_pdl(decode_fp4_tc_kernel, dim3((unsigned)(2 * a.workers)), dim3(kThreads), smem, st,
+                                     a, tm),
+                          "decode_fp4_tc_kernel launch"))
+    return rc;
+  return cuts ? launch_merge_fp4(a, kBias, st) : FP8MLA_OK;
+}
+
+int read_device_status_fp4_tc(unsigned int* status, bool reset, cudaStream_t st) {
+  unsigned int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, tc::g_device_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && reset && v != 0) {
+    const unsigned int zero = 0;
+    e = cudaMemcpyToSymbolAsync(tc::g_device_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  *status = v;
+  return check_cuda(e, "device status read");
+}
+
+}  // namespace fp8mla
