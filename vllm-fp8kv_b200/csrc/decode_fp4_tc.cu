@@ -76,7 +76,6 @@ using namespace fp8mla::tc;
 
 constexpr int kN = kFp4TcChunk;            // 128 entries per tile
 constexpr int kOwn = kN / 2;
-constexpr int kQTmemSteps = 24;            // q dims [0,384) from tensor memory
 constexpr int kQBlockBytes = 64 * 128;
 constexpr int kKBlockBytes = kOwn * 128;   // 8 KB: 64 own rows of a 64-dim block
 constexpr int kVBlockBytes = kN * 128;     // 16 KB
@@ -113,6 +112,7 @@ struct Smem {
   float lsum[128];
   uint32_t qmax[2][128];        // largest magnitudes of q's halves: latents, rope
   uint32_t vmask[kMaskSlots][4];  // a tile's live bits
+  int piece_tiles[2];           // tiles of a piece, by its parity (softmax -> MMA)
   uint64_t raw_full[kKWarps][kUnits], raw_empty[kKWarps][kUnits];
   uint64_t kfull[2], kempty[2];  // K blocks [0,4) and [4,9); kfull: even CTA
   uint64_t vfull, pfull, sempty, qready, oempty;  // even CTA, both CTAs arrive
@@ -140,18 +140,57 @@ struct Ctx {
 __device__ __forceinline__ uint32_t bar(uint64_t& b) { return smem_u32(&b); }
 
 // ------------------------------------------------------------------ MMA issuer (even CTA)
-template <int kFrom, int kTo>
-__device__ __forceinline__ void issue_s(uint32_t tS, uint32_t tQ, uint64_t qdesc0, uint64_t kdesc0) {
+// The whole warp walks the issuing code, and each MMA and commit elects the lane
+// that issues it (always the same one): control and addresses are then uniform
+// over the warp and the operands stay in uniform registers, where the MMAs need
+// them.  Measured on one pair alone, cycles per S / O MMA: 32.5 / 64.7 so, 54 / 65
+// under `if (lane == 0)`.  The election stands in front of every instruction,
+// which also keeps the warp converged: with one election for the whole role the
+// lane parts from the others at the first commit, while the code goes on in
+// registers that they share.
+__device__ __forceinline__ void pair_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n elect.sync _|e, 0xFFFFFFFF;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void pair_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n elect.sync _|e, 0xFFFFFFFF;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t& b) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xFFFFFFFF;\n"
+      " @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(
+          bar(b)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// The issue loops stay rolled, four MMAs a turn: straight-line code for all 52
+// MMAs of a tile is fetched anew for every tile.
+// K blocks [from, to) with q in tensor memory (blocks below 6) ...
+__device__ __forceinline__ void issue_s_tmem(uint32_t tS, uint32_t tQ, uint64_t kdesc, int from, int to) {
+#pragma unroll 1
+  for (int b = from; b < to; ++b) {
+    const uint64_t bd = kdesc + (uint64_t)((b * kKBlockBytes) >> 4);
+    const uint32_t aq = tQ + 32 * b;
 #pragma unroll
-  for (int kst = kFrom; kst < kTo; ++kst) {
-    const uint64_t bdesc = kdesc0 + (uint64_t)(((kst >> 2) * kKBlockBytes + (kst & 3) * 32) >> 4);
-    if (kst < kQTmemSteps) {
-      mma_pair_ts(tS, tQ + 8 * kst, bdesc, kIdescLatent, kst > 0 ? 1u : 0u);
-    } else {
-      const int qs = kst - kQTmemSteps;
-      const uint64_t adesc = qdesc0 + (uint64_t)(((qs >> 2) * kQBlockBytes + (qs & 3) * 32) >> 4);
-      mma_pair_ss(tS, adesc, bdesc, kst < 32 ? kIdescLatent : kIdescRope, 1u);
-    }
+    for (int i = 0; i < 4; ++i) pair_ts(tS, aq + 8 * i, bd + (uint64_t)(2 * i), kIdescLatent, (b | i) ? 1u : 0u);
+  }
+}
+// ... and with q in shared memory (6 and 7 latents, 8 the rope)
+__device__ __forceinline__ void issue_s_smem(uint32_t tS, uint64_t qdesc, uint64_t kdesc) {
+#pragma unroll 1
+  for (int b = 6; b < 9; ++b) {
+    const uint64_t bd = kdesc + (uint64_t)((b * kKBlockBytes) >> 4);
+    const uint64_t ad = qdesc + (uint64_t)(((b - 6) * kQBlockBytes) >> 4);
+    const uint32_t id = b < 8 ? kIdescLatent : kIdescRope;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pair_ss(tS, ad + (uint64_t)(2 * i), bd + (uint64_t)(2 * i), id, 1u);
   }
 }
 
@@ -162,47 +201,51 @@ __device__ void mma_role(const Ctx& c) {
   const uint64_t kdesc0 = sdesc_sw128(smem_u32(s.k), 16, 1024);
   const uint64_t pdesc0 = sdesc_sw128(smem_u32(s.p), 16, 1024);
   const uint64_t vdesc0 = sdesc_sw128(smem_u32(s.v), kVBlockBytes, 1024);
-  Walk<kN> w(*c.a, s.share, c.worker);
   bool ok = true;
+  const uint32_t tiles = (uint32_t)c.tiles;
   uint32_t j = 0;                     // tile of the run
   bool first = false, last = false;   // tile j - 1 opens / closes its piece
   uint32_t piece = 0;                 // piece of tile j - 1
   // O of tile j - 1
   auto issue_o = [&]() {
     if (!ok) return;
-    if (first && piece > 0) ok = thread_wait_cluster(bar(s.oempty), (piece - 1) & 1, 45);
-    if (ok) ok = thread_wait_cluster(bar(s.pfull), (j - 1) & 1, 36);
-    if (ok) ok = thread_wait_cluster(bar(s.vfull), (j - 1) & 1, 38);
+    if (first && piece > 0) ok = warp_wait_cluster(bar(s.oempty), (piece - 1) & 1, 45);
+    if (ok) ok = warp_wait_cluster(bar(s.pfull), (j - 1) & 1, 36);
+    if (ok) ok = warp_wait_cluster(bar(s.vfull), (j - 1) & 1, 38);
     if (!ok) return;
     tc_fence_after();
+#pragma unroll 1
+    for (int x = 0; x < 4; ++x) {  // half x / 2 of the dims, entries [64 (x % 2), +64)
+      const uint64_t ad = pdesc0 + (uint64_t)(((x & 1) * kPBlockBytes) >> 4);
+      const uint64_t bd = vdesc0 + (uint64_t)(((x >> 1) * 2 * kVBlockBytes + (x & 1) * 64 * 128) >> 4);
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-      for (int kk = 0; kk < kN / 16; ++kk)
-        mma_pair_ss(c.tmem + kColO + 128 * hf,
-                    pdesc0 + (uint64_t)(((kk >> 2) * kPBlockBytes + (kk & 3) * 32) >> 4),
-                    vdesc0 + (uint64_t)((hf * 2 * kVBlockBytes + kk * 16 * 128) >> 4), kIdescPV,
-                    (kk > 0 || !first) ? 1u : 0u);
-    mma_commit_pair(bar(s.pvdone));  // P and V may be written again
-    if (last) mma_commit_pair(bar(s.ofull));
+      for (int i = 0; i < 4; ++i)
+        pair_ss(c.tmem + kColO + 128 * (x >> 1), ad + (uint64_t)(2 * i), bd + (uint64_t)((i * 16 * 128) >> 4),
+                    kIdescPV, ((x & 1) || i > 0 || !first) ? 1u : 0u);
+    }
+    commit(s.pvdone);  // P and V may be written again
+    if (last) commit(s.ofull);
   };
   uint32_t p = 0;
-  while (w.left > 0 && ok) {
-    const int n = w.here();
-    ok = thread_wait_cluster(bar(s.qready), p & 1, 35);
+  while (j < tiles && ok) {
+    ok = warp_wait_cluster(bar(s.qready), p & 1, 35);
+    if (!ok) break;
+    (void)mbar_try_wait(bar(s.qready), p & 1);  // every lane acquires
+    const int n = s.piece_tiles[p & 1];
     for (int i = 0; i < n && ok; ++i) {
-      if (j > 0) ok = thread_wait_cluster(bar(s.sempty), (j - 1) & 1, 34);
-      if (ok) ok = thread_wait_cluster(bar(s.kfull[0]), j & 1, 37);
+      if (j > 0) ok = warp_wait_cluster(bar(s.sempty), (j - 1) & 1, 34);
+      if (ok) ok = warp_wait_cluster(bar(s.kfull[0]), j & 1, 37);
       if (!ok) break;
       tc_fence_after();
-      issue_s<0, 16>(tS, tQ, qdesc0, kdesc0);
-      mma_commit_pair(bar(s.kempty[0]));
-      ok = thread_wait_cluster(bar(s.kfull[1]), j & 1, 39);
+      issue_s_tmem(tS, tQ, kdesc0, 0, 4);
+      commit(s.kempty[0]);
+      ok = warp_wait_cluster(bar(s.kfull[1]), j & 1, 39);
       if (!ok) break;
       tc_fence_after();
-      issue_s<16, 36>(tS, tQ, qdesc0, kdesc0);
-      mma_commit_pair(bar(s.kempty[1]));
-      mma_commit_pair(bar(s.sfull));
+      issue_s_tmem(tS, tQ, kdesc0, 4, 6);
+      issue_s_smem(tS, qdesc0, kdesc0);
+      commit(s.kempty[1]);
+      commit(s.sfull);
       if (j > 0) issue_o();
       first = i == 0;
       last = i == n - 1;
@@ -210,12 +253,26 @@ __device__ void mma_role(const Ctx& c) {
       ++j;
     }
     ++p;
-    w.next_unit(*c.a, n);
   }
   if (j > 0) issue_o();
-  // drain: nothing this thread issued may still touch either CTA's memory
-  mma_commit_pair(bar(s.drain));
-  thread_wait_cluster(bar(s.drain), 0, 46);
+  commit(s.drain);  // see settle()
+}
+
+// The MMA warp of both CTAs: every arrival that is still on its way to one of
+// this CTA's barriers is seen in before the CTA may exit (one that finds its
+// target gone is an illegal access; the closing cluster barrier alone does not
+// hold it back).  The drain commit arrives once every MMA is done.  Of the last
+// tile, the multicast arrivals of the other commits and the odd CTA's release of
+// S need not have been waited for by anyone; their earlier phases have been, so
+// the parity names the right one.  (Every other arrival gates a wait, and oempty
+// is not signalled for the last unit.)
+__device__ void settle(const Ctx& c) {
+  Smem& s = *c.s;
+  if (!warp_wait_cluster(bar(s.drain), 0, 46) || c.tiles == 0) return;
+  const uint32_t par = (uint32_t)(c.tiles - 1) & 1;
+  (void)(warp_wait_cluster(bar(s.kempty[0]), par, 48) && warp_wait_cluster(bar(s.kempty[1]), par, 48) &&
+         warp_wait_cluster(bar(s.pvdone), par, 48) &&
+         (c.rank != 0 || warp_wait_cluster(bar(s.sempty), par, 48)));
 }
 
 // ------------------------------------------------------------------ producers
@@ -433,7 +490,7 @@ struct Meet {
 // L & 63), the rest -> swizzled shared memory (thread hh writes chunks [4 hh, +4)
 // of each block); padding rows are zero.  `scale` turns the head's accumulators
 // into scores in log2 units.
-__device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, Meet& meet, float& scale) {
+__device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, Meet& meet, float& scale) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
   const int m = L & 63, hh = L >> 6;
@@ -445,52 +502,83 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, Meet& meet, float
   auto mag = [](const uint4& v) {
     return __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
   };
-  // largest magnitudes (as bits): each thread half of the latents and of the rope
-  uint32_t mx = 0, mr = 0;
-#pragma unroll 8
-  for (int i = 0; i < 32; ++i) mx = __vmaxu2(mx, mag(hv ? src[32 * hh + i] : z4));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) mr = __vmaxu2(mr, mag(hv ? src[64 + 4 * hh + i] : z4));
-  s.qmax[0][L] = max(mx & 0xFFFFu, mx >> 16);
-  s.qmax[1][L] = max(mr & 0xFFFFu, mr >> 16);
-  if (!meet(s, L & 31)) return false;
-  const int bm = (int)max(s.qmax[0][L], s.qmax[0][L ^ 64]), br = (int)max(s.qmax[1][L], s.qmax[1][L ^ 64]);
-  // 2^k brings the latent part's largest value to [2^8, 2^9), but the rope's at
-  // most to 2^101, where its products are still finite; 1 for rows of zeros, inf
-  // or NaN.  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.
-  int k = min(8 - ((bm >> 7) - 127), 100 - ((br >> 7) - 127));
-  k = (bm == 0 || bm >= 0x7F80) ? 0 : min(126, k);
-  const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-  auto f16 = [&](uint32_t v) { return pack_f16x2(bf16_lo(v) * up, bf16_hi(v) * up); };
-  auto bf = [&](uint32_t v) { return pack_bf16x2(bf16_lo(v) * up, bf16_hi(v) * up); };
-#pragma unroll
-  for (int b = 0; b < 3; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 v = hv ? src[48 + 8 * b + 4 * hh + i] : z4;
-      *reinterpret_cast<uint4*>(s.q + b * kQBlockBytes + swz(m, 4 * hh + i)) =
-          b < 2 ? make_uint4(f16(v.x), f16(v.y), f16(v.z), f16(v.w)) : make_uint4(bf(v.x), bf(v.y), bf(v.z), bf(v.w));
-    }
   const uint32_t trow = c.tmem + ((uint32_t)((L >> 5) * 32) << 16);
-#pragma unroll 1
-  for (int c0 = 0; c0 < 192; c0 += 32) {
-    uint32_t o[32];
+  // q times 2^k; returns the largest magnitudes (as bits) of the latents and of
+  // the rope among what this thread converted
+  auto convert = [&](int k, uint32_t& mx, uint32_t& mr) {
+    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+    auto f16 = [&](const uint4& v) {
+      auto one = [&](uint32_t u) { return pack_f16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
+      return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+    };
+    auto bf = [&](const uint4& v) {
+      auto one = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
+      return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+    };
+    mx = mr = 0;
+    {
+      uint4 x[12];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint4 v = hv ? src[c0 / 4 + i] : z4;
-      o[4 * i] = f16(v.x);
-      o[4 * i + 1] = f16(v.y);
-      o[4 * i + 2] = f16(v.z);
-      o[4 * i + 3] = f16(v.w);
+      for (int b = 0; b < 3; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * b + i] = hv ? src[48 + 8 * b + 4 * hh + i] : z4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mx = __vmaxu2(mx, __vmaxu2(mag(x[i]), mag(x[4 + i])));
+        mr = __vmaxu2(mr, mag(x[8 + i]));
+        *reinterpret_cast<uint4*>(s.q + swz(m, 4 * hh + i)) = f16(x[i]);
+        *reinterpret_cast<uint4*>(s.q + kQBlockBytes + swz(m, 4 * hh + i)) = f16(x[4 + i]);
+        *reinterpret_cast<uint4*>(s.q + 2 * kQBlockBytes + swz(m, 4 * hh + i)) = bf(x[8 + i]);
+      }
     }
-    tmem_st32(trow + kColQ + c0, o);
-  }
-  tmem_wait_st();
+#pragma unroll 1
+    for (int c0 = 0; c0 < 192; c0 += 64) {
+      uint4 x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = hv ? src[c0 / 4 + i] : z4;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t o[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          mx = __vmaxu2(mx, mag(x[8 * g + i]));
+          const uint4 v = f16(x[8 * g + i]);
+          o[4 * i] = v.x;
+          o[4 * i + 1] = v.y;
+          o[4 * i + 2] = v.z;
+          o[4 * i + 3] = v.w;
+        }
+        tmem_st32(trow + kColQ + c0 + 32 * g, o);
+      }
+    }
+    tmem_wait_st();
+    mx = max(mx & 0xFFFFu, mx >> 16);
+    mr = max(mr & 0xFFFFu, mr >> 16);
+  };
+  // As it is where the head's largest latent magnitude lies in [2^-2, 2^15] (an
+  // fp16 subnormal's error is below 2^-23 of it then).  Else times 2^k, which
+  // brings that magnitude to [2^8, 2^9), but the rope's at most to 2^101, where
+  // its products are still finite (1 for rows of zeros, inf or NaN).  Exponents
+  // of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.
+  uint32_t mx, mr;
+  convert(0, mx, mr);
+  s.qmax[0][L] = mx;
+  s.qmax[1][L] = mr;
+  if (!meet(s, L & 31)) return false;
+  mx = max(mx, s.qmax[0][L ^ 64]);
+  mr = max(mr, s.qmax[1][L ^ 64]);
+  int k = 0;
+  if (mx != 0 && mx < 0x7F80u && (mx < 0x3E80u || mx > 0x4700u))
+    k = min(126, min(8 - ((int)(mx >> 7) - 127), 100 - ((int)(mr >> 7) - 127)));
+  if (__any_sync(0xFFFFFFFFu, k != 0)) convert(k, mx, mr);
+  // (the piece two before this one, whose place it takes, is past its last S)
+  if (L == 0) s.piece_tiles[piece & 1] = w.here();
   fence_proxy_async_smem();
   tc_fence_before();
   __syncwarp();
   if ((L & 31) == 0) mbar_arrive_cluster(bar(s.qready), 0);
   scale = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+  if (scale == 0.f) scale = 1.1754944e-38f;  // a masked score is an infinity times the scale
   return true;
 }
 
@@ -504,10 +592,11 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
   uint32_t j = 0, piece = 0;
   float scale = 0.f;
   Meet meet;
-  if (w.left > 0) ok = load_q(c, w, L, meet, scale);
+  if (w.left > 0) ok = load_q(c, w, L, 0, meet, scale);
   while (w.left > 0 && ok) {
     const int n = w.here();
     float m_ref = -INFINITY, l = 0.f;
+    const uint32_t masked = __float_as_uint(scale < 0.f ? INFINITY : -INFINITY);  // -inf after scaling
     for (int i = 0; i < n; ++i, ++j) {
       const uint32_t par = j & 1;
       ok = warp_wait_cluster(bar(s.sfull), par, 31);
@@ -524,8 +613,13 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
         tmem_ld32(trow + kColS + 32 * h, sv);
         const uint32_t live = s.vmask[mslot][2 * hh + h];
         tmem_wait_ld();
+        if (live != 0xFFFFFFFFu) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) pm = fmaxf(pm, (live >> e) & 1u ? __uint_as_float(sv[e]) * scale : -INFINITY);
+          for (int e = 0; e < 32; ++e)
+            if (!((live >> e) & 1u)) sv[e] = masked;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) pm = fmaxf(pm, __uint_as_float(sv[e]) * scale);
       }
       s.half_max[par][L] = pm;
       ok = meet(s, lane);
@@ -538,7 +632,32 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
         l *= alpha;
       }
       const float sub = m_ref == -INFINITY ? 0.f : m_ref - kBias;
-      // O of the tile before has read P (and is complete, should it be rescaled)
+      // ... then P, in registers until O of the tile before has read its P
+      uint32_t pk[32];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sv[32];
+        tmem_ld32(trow + kColS + 32 * h, sv);
+        const uint32_t live = s.vmask[mslot][2 * hh + h];
+        tmem_wait_ld();
+        if (h == 1) {  // S may be written again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(bar(s.sempty), 0);
+        }
+        if (live != 0xFFFFFFFFu) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((live >> e) & 1u)) sv[e] = masked;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p0 = ex2_approx(fmaf(__uint_as_float(sv[2 * e]), scale, -sub));
+          const float p1 = ex2_approx(fmaf(__uint_as_float(sv[2 * e + 1]), scale, -sub));
+          l += p0 + p1;
+          pk[16 * h + e] = pack_f16x2(p0, p1);
+        }
+      }
       if (j > 0) ok = warp_wait_cluster(bar(s.pvdone), (j - 1) & 1, 33);
       if (!ok) break;
       if (__any_sync(0xFFFFFFFFu, alpha != 1.f) && i > 0) {
@@ -554,33 +673,10 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
         }
         tmem_wait_st();
       }
-      // ... then P
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        uint32_t sv[32];
-        tmem_ld32(trow + kColS + 32 * h, sv);
-        const uint32_t live = s.vmask[mslot][2 * hh + h];
-        tmem_wait_ld();
-        if (h == 1) {  // S may be written again
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(bar(s.sempty), 0);
-        }
-        uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float p0 = ex2_approx(fmaf(__uint_as_float(sv[2 * e]), scale, -sub));
-          float p1 = ex2_approx(fmaf(__uint_as_float(sv[2 * e + 1]), scale, -sub));
-          p0 = (live >> (2 * e)) & 1u ? p0 : 0.f;
-          p1 = (live >> (2 * e + 1)) & 1u ? p1 : 0.f;
-          l += p0 + p1;
-          pk[e] = pack_f16x2(p0, p1);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<uint4*>(s.p + hh * kPBlockBytes + swz(m, 4 * h + e)) =
-              make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
-      }
+      for (int e = 0; e < 8; ++e)
+        *reinterpret_cast<uint4*>(s.p + hh * kPBlockBytes + swz(m, e)) =
+            make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
@@ -599,7 +695,7 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
     const int64_t hg = (int64_t)w.grp * a.hpg + head;
     const int64_t prow = (2 * (int64_t)c.worker + (w.c == 0 ? 1 : 0)) * a.rows + 64 * (int)c.rank + m;
     w.next_unit(a, n);
-    if (w.left > 0) ok = load_q(c, w, L, meet, scale);
+    if (w.left > 0) ok = load_q(c, w, L, piece + 1, meet, scale);
     if (ok) ok = warp_wait_cluster(bar(s.ofull), piece & 1, 32);
     if (!ok) break;
     tc_fence_after();
@@ -636,7 +732,8 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
     }
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive_cluster(bar(s.oempty), 0);
+    // the next unit's O may begin (nobody waits behind the last one: see settle)
+    if (lane == 0 && w.left > 0) mbar_arrive_cluster(bar(s.oempty), 0);
     ++piece;
   }
 }
@@ -687,7 +784,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   c.tmem = s.tmem_base;
   divide<kN, kThreads>(a, s.share, c.worker);
   if (threadIdx.x == 0 && c.rank == 0) note_start<kN>(a, s.share, c.worker);
-  c.tiles = Walk<kN>(a, s.share, c.worker).left;
+  c.tiles = max((int64_t)0, Walk<kN>(a, s.share, c.worker).left);
 
   // one call per role: the loops of all roles together have to stay in the SM's
   // instruction cache (with each role inlined twice, and the unpacking and the
@@ -696,7 +793,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp < kSoftmaxWarps) {
     softmax_role(c, warp, lane);
   } else if (warp == kMmaWarp) {
-    if (c.rank == 0 && lane == 0) mma_role(c);
+    if (c.rank == 0) mma_role(c);
+    settle(c);
   } else if (warp < 8 || warp == 9) {
     k_role(c, warp < 8 ? warp - 5 : 3, lane);
   } else if (warp == 8 || warp == 15) {

@@ -88,7 +88,7 @@ __device__ void divide(const Fp4DecodeArgs& a, Share& s, int worker) {
 // A worker's place in the chunk list.
 template <int kChunk>
 struct Walk {
-  int64_t left;   // chunks of this worker from the current one on
+  int64_t left;   // chunks of this worker from the current one on (none: <= 0)
   int64_t unit;   // t * (G * hb_per_group) + group * hb_per_group + head block
   int64_t t;
   int grp, hb;
