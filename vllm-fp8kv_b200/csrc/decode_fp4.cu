@@ -73,12 +73,6 @@ template <int kRegs>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegs));
 }
-// Bounded wait after which every lane has acquired the phase itself.
-__device__ __forceinline__ bool acquire(uint32_t bar, uint32_t parity, uint32_t where) {
-  const bool ok = warp_wait(bar, parity, where);
-  if (ok) (void)mbar_try_wait(bar, parity);
-  return ok;
-}
 // Barriers: all compute warps (id 1), one group (id 2 + group), and the same
 // with an "any of us" vote.
 __device__ __forceinline__ void compute_sync() {
@@ -145,7 +139,7 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
     for (int half = 0; half < 2; ++half) {
       if (g + half >= chunks) break;
       const int st = ring.st;
-      if (g + half >= kStages) ok = warp_wait(smem_u32(&s.raw_empty[st]), ring.ph ^ 1, 20);
+      if (g + half >= kStages) ok = wait(s.raw_empty[st], ring.ph ^ 1, 20);
       if (!ok) break;
       const uint32_t live = (live2 >> (16 * half)) & 0xFFFFu;
       const int n = __popc(live);
@@ -180,7 +174,7 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
   // the stages armed last have landed before the warp returns, even after a
   // failed wait
   for (int64_t x = armed > kStages ? armed - kStages : 0; x < armed; ++x)
-    (void)warp_wait(smem_u32(&s.raw_full[x % kStages]), (uint32_t)(x / kStages) & 1, 26);
+    (void)wait(s.raw_full[x % kStages], (uint32_t)(x / kStages) & 1, 26);
 }
 
 // ------------------------------------------------------------------ compute
@@ -374,7 +368,7 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int cw, int lane) {
     Ring ring = piece_at;
     ring.ahead(grp);
     for (int c = grp; c < nch; c += kGroups) {
-      if (ok) ok = acquire(smem_u32(&s.raw_full[ring.st]), ring.ph, 21);
+      if (ok) ok = wait(s.raw_full[ring.st], ring.ph, 21);
       const uint64_t live = *reinterpret_cast<const uint64_t*>(s.live[ring.st]);
       const uint8_t* raw = s.raw[ring.st];
       float x[2][4];

@@ -209,9 +209,9 @@ __device__ void mma_role(const Ctx& c) {
   // O of tile j - 1
   auto issue_o = [&]() {
     if (!ok) return;
-    if (first && piece > 0) ok = warp_wait_cluster(bar(s.oempty), (piece - 1) & 1, 45);
-    if (ok) ok = warp_wait_cluster(bar(s.pfull), (j - 1) & 1, 36);
-    if (ok) ok = warp_wait_cluster(bar(s.vfull), (j - 1) & 1, 38);
+    if (first && piece > 0) ok = wait(s.oempty, (piece - 1) & 1, 45);
+    if (ok) ok = wait(s.pfull, (j - 1) & 1, 36);
+    if (ok) ok = wait(s.vfull, (j - 1) & 1, 38);
     if (!ok) return;
     tc_fence_after();
 #pragma unroll 1
@@ -228,18 +228,17 @@ __device__ void mma_role(const Ctx& c) {
   };
   uint32_t p = 0;
   while (j < tiles && ok) {
-    ok = warp_wait_cluster(bar(s.qready), p & 1, 35);
+    ok = wait(s.qready, p & 1, 35);
     if (!ok) break;
-    (void)mbar_try_wait(bar(s.qready), p & 1);  // every lane acquires
     const int n = s.piece_tiles[p & 1];
     for (int i = 0; i < n && ok; ++i) {
-      if (j > 0) ok = warp_wait_cluster(bar(s.sempty), (j - 1) & 1, 34);
-      if (ok) ok = warp_wait_cluster(bar(s.kfull[0]), j & 1, 37);
+      if (j > 0) ok = wait(s.sempty, (j - 1) & 1, 34);
+      if (ok) ok = wait(s.kfull[0], j & 1, 37);
       if (!ok) break;
       tc_fence_after();
       issue_s_tmem(tS, tQ, kdesc0, 0, 4);
       commit(s.kempty[0]);
-      ok = warp_wait_cluster(bar(s.kfull[1]), j & 1, 39);
+      ok = wait(s.kfull[1], j & 1, 39);
       if (!ok) break;
       tc_fence_after();
       issue_s_tmem(tS, tQ, kdesc0, 4, 6);
@@ -268,11 +267,11 @@ __device__ void mma_role(const Ctx& c) {
 // is not signalled for the last unit.)
 __device__ void settle(const Ctx& c) {
   Smem& s = *c.s;
-  if (!warp_wait_cluster(bar(s.drain), 0, 46) || c.tiles == 0) return;
+  if (!wait(s.drain, 0, 46) || c.tiles == 0) return;
   const uint32_t par = (uint32_t)(c.tiles - 1) & 1;
-  (void)(warp_wait_cluster(bar(s.kempty[0]), par, 48) && warp_wait_cluster(bar(s.kempty[1]), par, 48) &&
-         warp_wait_cluster(bar(s.pvdone), par, 48) &&
-         (c.rank != 0 || warp_wait_cluster(bar(s.sempty), par, 48)));
+  (void)(wait(s.kempty[0], par, 48) && wait(s.kempty[1], par, 48) &&
+         wait(s.pvdone, par, 48) &&
+         (c.rank != 0 || wait(s.sempty, par, 48)));
 }
 
 // ------------------------------------------------------------------ producers
@@ -306,7 +305,7 @@ __device__ void produce(const Ctx& c, const CUtensorMap* tm, int pw, int lane) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int l0 = 16 * i + 8 * h, kw = 2 * pw + i;
-        if (ok && ring.round > 0) ok = warp_wait(bar(s.raw_empty[kw][ring.u]), (ring.round - 1) & 1, 40);
+        if (ok && ring.round > 0) ok = wait(s.raw_empty[kw][ring.u], (ring.round - 1) & 1, 40);
         if (!ok) break;
         const uint32_t live = (live4 >> l0) & 0xFFu;
         const int n = __popc(live);
@@ -341,7 +340,7 @@ __device__ void produce(const Ctx& c, const CUtensorMap* tm, int pw, int lane) {
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     for (int64_t x = armed[i] > kUnits ? armed[i] - kUnits : 0; x < armed[i]; ++x)
-      (void)warp_wait(bar(s.raw_full[2 * pw + i][x % kUnits]), (uint32_t)(x / kUnits) & 1, 41);
+      (void)wait(s.raw_full[2 * pw + i][x % kUnits], (uint32_t)(x / kUnits) & 1, 41);
 }
 
 // ------------------------------------------------------------------ K and V
@@ -382,10 +381,8 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
     uint32_t sc[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t full = bar(s.raw_full[kw][ring.u]);
-      if (ok) ok = warp_wait(full, ring.round & 1, 42);
+      if (ok) ok = wait(s.raw_full[kw][ring.u], ring.round & 1, 42);
       if (!ok) break;
-      (void)mbar_try_wait(full, ring.round & 1);  // every lane acquires
       const uint8_t* row = s.raw[kw][ring.u] + r8 * kFp4RowBytes;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -400,7 +397,7 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
     }
 #pragma unroll
     for (int g = 0; g < 2; ++g) {  // blocks [0,4): latent tiles 0, 1; blocks [4,9): 2, 3 and the rope
-      if (ok && j > 0) ok = warp_wait_cluster(bar(s.kempty[g]), (uint32_t)(j - 1) & 1, 43);
+      if (ok && j > 0) ok = wait(s.kempty[g], (uint32_t)(j - 1) & 1, 43);
       if (!ok) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -456,7 +453,7 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
       s.vmask[j % kMaskSlots][vw] = live;
       mbar_arrive(bar(s.mfull[j % kMaskSlots]));
     }
-    if (j > 0 && !warp_wait_cluster(bar(s.pvdone), (uint32_t)(j - 1) & 1, 44)) break;
+    if (j > 0 && !wait(s.pvdone, (uint32_t)(j - 1) & 1, 44)) break;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t r = 32 * vw + 8 * i + r8;
@@ -479,10 +476,7 @@ struct Meet {
   __device__ __forceinline__ bool operator()(Smem& s, int lane) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(s.meet));
-    const bool ok = warp_wait(bar(s.meet), n & 1, 47);
-    if (ok) (void)mbar_try_wait(bar(s.meet), n & 1);
-    ++n;
-    return ok;
+    return wait(s.meet, n++ & 1, 47);
   }
 };
 
@@ -599,11 +593,10 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
     const uint32_t masked = __float_as_uint(scale < 0.f ? INFINITY : -INFINITY);  // -inf after scaling
     for (int i = 0; i < n; ++i, ++j) {
       const uint32_t par = j & 1;
-      ok = warp_wait_cluster(bar(s.sfull), par, 31);
+      ok = wait(s.sfull, par, 31);
       const uint32_t mslot = j % kMaskSlots, mpar = (j / kMaskSlots) & 1;
-      if (ok) ok = warp_wait(bar(s.mfull[mslot]), mpar, 30);
+      if (ok) ok = wait(s.mfull[mslot], mpar, 30);
       if (!ok) break;
-      (void)mbar_try_wait(bar(s.mfull[mslot]), mpar);
       tc_fence_after();
       // two passes over the 64 scores, 32 at a time (half the code): the maximum ...
       float pm = -INFINITY;
@@ -658,7 +651,7 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
           pk[16 * h + e] = pack_f16x2(p0, p1);
         }
       }
-      if (j > 0) ok = warp_wait_cluster(bar(s.pvdone), (j - 1) & 1, 33);
+      if (j > 0) ok = wait(s.pvdone, (j - 1) & 1, 33);
       if (!ok) break;
       if (__any_sync(0xFFFFFFFFu, alpha != 1.f) && i > 0) {
         tc_fence_after();
@@ -696,7 +689,7 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
     const int64_t prow = (2 * (int64_t)c.worker + (w.c == 0 ? 1 : 0)) * a.rows + 64 * (int)c.rank + m;
     w.next_unit(a, n);
     if (w.left > 0) ok = load_q(c, w, L, piece + 1, meet, scale);
-    if (ok) ok = warp_wait_cluster(bar(s.ofull), piece & 1, 32);
+    if (ok) ok = wait(s.ofull, piece & 1, 32);
     if (!ok) break;
     tc_fence_after();
     const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);

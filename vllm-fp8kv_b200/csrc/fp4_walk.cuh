@@ -4,6 +4,7 @@
 #pragma once
 #include "common.cuh"
 #include "decode_fp4.h"
+#include "tc_ptx.cuh"
 
 namespace fp8mla {
 namespace fp4 {
@@ -207,6 +208,18 @@ struct Slots {
     return slot;
   }
 };
+
+// Bounded wait of a whole warp: every lane looks (so every lane has acquired the
+// phase) and the vote gives all of them one verdict.  A phase that is complete
+// costs 18 cycles; one lane looking for the others and passing the verdict on
+// costs 190.
+__device__ __forceinline__ bool wait(uint64_t& b, uint32_t parity, uint32_t where) {
+  const uint32_t at = smem_u32(&b);
+  for (uint32_t it = 0; it < tc::kMaxWaitIters; ++it)
+    if (__all_sync(0xFFFFFFFFu, tc::mbar_try_wait(at, parity))) return true;
+  if ((threadIdx.x & 31) == 0) atomicOr(&tc::g_device_status, tc::kStatusWaitTimeout | (where << 8));
+  return false;
+}
 
 __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
