@@ -500,7 +500,8 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, M
   // q times 2^k; returns the largest magnitudes (as bits) of the latents and of
   // the rope among what this thread converted
   auto convert = [&](int k, uint32_t& mx, uint32_t& mr) {
-    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+    // the sign of the softmax scale goes with q, so that scores scale by a positive factor
+    const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), a.scale_log2);
     auto f16 = [&](const uint4& v) {
       auto one = [&](uint32_t u) { return pack_f16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
       return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
@@ -571,9 +572,29 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, M
   tc_fence_before();
   __syncwarp();
   if ((L & 31) == 0) mbar_arrive_cluster(bar(s.qready), 0);
-  scale = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+  scale = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k) << 23);
   if (scale == 0.f) scale = 1.1754944e-38f;  // a masked score is an infinity times the scale
   return true;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two fp32 operations in one instruction, each rounded as on its own
+__device__ __forceinline__ float2 fma2(float2 v, float m, float a) {
+  const float2 m2 = make_float2(m, m), a2 = make_float2(a, a);
+  asm("fma.rn.f32x2 %0, %0, %1, %2;\n"
+      : "+l"(reinterpret_cast<uint64_t&>(v))
+      : "l"(reinterpret_cast<const uint64_t&>(m2)), "l"(reinterpret_cast<const uint64_t&>(a2)));
+  return v;
+}
+__device__ __forceinline__ float2 add2(float2 v, float2 w) {
+  asm("add.rn.f32x2 %0, %0, %1;\n"
+      : "+l"(reinterpret_cast<uint64_t&>(v))
+      : "l"(reinterpret_cast<const uint64_t&>(w)));
+  return v;
 }
 
 __device__ void softmax_role(const Ctx& c, int warp, int lane) {
@@ -590,30 +611,32 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
   while (w.left > 0 && ok) {
     const int n = w.here();
     float m_ref = -INFINITY, l = 0.f;
-    const uint32_t masked = __float_as_uint(scale < 0.f ? INFINITY : -INFINITY);  // -inf after scaling
     for (int i = 0; i < n; ++i, ++j) {
       const uint32_t par = j & 1;
       ok = wait(s.sfull, par, 31);
       const uint32_t mslot = j % kMaskSlots, mpar = (j / kMaskSlots) & 1;
       if (ok) ok = wait(s.mfull[mslot], mpar, 30);
       if (!ok) break;
+      const uint32_t live0 = s.vmask[mslot][2 * hh], live1 = s.vmask[mslot][2 * hh + 1];
       tc_fence_after();
-      // two passes over the 64 scores, 32 at a time (half the code): the maximum ...
-      float pm = -INFINITY;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        uint32_t sv[32];
-        tmem_ld32(trow + kColS + 32 * h, sv);
-        const uint32_t live = s.vmask[mslot][2 * hh + h];
-        tmem_wait_ld();
-        if (live != 0xFFFFFFFFu) {
+      uint32_t sv[64];
+      tmem_ld32(trow + kColS, reinterpret_cast<uint32_t(&)[32]>(sv[0]));
+      tmem_ld32(trow + kColS + 32, reinterpret_cast<uint32_t(&)[32]>(sv[32]));
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(bar(s.sempty), 0);  // S may be written again
+      if ((live0 & live1) != 0xFFFFFFFFu) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((live >> e) & 1u)) sv[e] = masked;
+        for (int e = 0; e < 32; ++e) {
+          if (!((live0 >> e) & 1u)) sv[e] = 0xFF800000u;  // -inf (the scale is positive)
+          if (!((live1 >> e) & 1u)) sv[32 + e] = 0xFF800000u;
         }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) pm = fmaxf(pm, __uint_as_float(sv[e]) * scale);
       }
+      float pm = __uint_as_float(sv[0]);
+#pragma unroll
+      for (int e = 1; e < 63; e += 2) pm = max3(pm, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+      pm = fmaxf(pm, __uint_as_float(sv[63])) * scale;
       s.half_max[par][L] = pm;
       ok = meet(s, lane);
       if (!ok) break;
@@ -625,32 +648,17 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
         l *= alpha;
       }
       const float sub = m_ref == -INFINITY ? 0.f : m_ref - kBias;
-      // ... then P, in registers until O of the tile before has read its P
+      // P, in registers until O of the tile before has read its P
       uint32_t pk[32];
+      float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t sv[32];
-        tmem_ld32(trow + kColS + 32 * h, sv);
-        const uint32_t live = s.vmask[mslot][2 * hh + h];
-        tmem_wait_ld();
-        if (h == 1) {  // S may be written again
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(bar(s.sempty), 0);
-        }
-        if (live != 0xFFFFFFFFu) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((live >> e) & 1u)) sv[e] = masked;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = ex2_approx(fmaf(__uint_as_float(sv[2 * e]), scale, -sub));
-          const float p1 = ex2_approx(fmaf(__uint_as_float(sv[2 * e + 1]), scale, -sub));
-          l += p0 + p1;
-          pk[16 * h + e] = pack_f16x2(p0, p1);
-        }
+      for (int e = 0; e < 32; ++e) {
+        const float2 x = fma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale, -sub);
+        const float2 p2 = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+        l2 = add2(l2, p2);
+        pk[e] = pack_f16x2(p2.x, p2.y);
       }
+      l += l2.x + l2.y;
       if (j > 0) ok = wait(s.pvdone, (j - 1) & 1, 33);
       if (!ok) break;
       if (__any_sync(0xFFFFFFFFu, alpha != 1.f) && i > 0) {
