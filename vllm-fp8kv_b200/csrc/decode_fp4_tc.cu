@@ -50,13 +50,14 @@
 //   warps 0-3         softmax, q, and the stores of O
 //   warp 4            tensor memory allocation; lane 0 of the even CTA issues
 //                     every MMA of the pair
-//   warps 5, 6, 7, 9  K: own rows [16i, +16) of every tile, raw ring -> K blocks
+//   warps 5, 6, 7, 9  K: own rows [16i, +16) of every tile: entries -> slots ->
+//                     TMA copies into the warp's raw ring -> K blocks
 //   warps 10, 11, 13, 14
 //                     V: entries [32i, +32) of every tile, the half's codes and
 //                     scales by register loads one tile ahead -> V blocks; and
 //                     the tile's live bits
-//   warps 8, 15       producers: entries -> slots -> TMA copies, 32 own rows each
-//   warp 12           idle
+//   warps 8, 12, 15   idle: sub-partition 0 runs the issuing warp and one softmax
+//                     warp alone
 // Barriers that gate the issuing thread live in the even CTA and count arrivals
 // of both CTAs; the completion of pair MMAs reaches both CTAs through a multicast
 // commit.  Every wait is bounded; after a failed wait a role stops, and the
@@ -67,7 +68,6 @@
 #include "fp4_walk.cuh"
 #include "tc_cluster.cuh"
 #include "tc_ptx.cuh"
-#include "tma_map.h"
 
 namespace fp8mla {
 namespace {
@@ -80,10 +80,6 @@ constexpr int kQBlockBytes = 64 * 128;
 constexpr int kKBlockBytes = kOwn * 128;   // 8 KB: 64 own rows of a 64-dim block
 constexpr int kVBlockBytes = kN * 128;     // 16 KB
 constexpr int kPBlockBytes = 64 * 128;     // 64 heads x 64 entries
-constexpr int kUnitRows = 8;               // rows of a raw unit: half of a K warp's rows of a tile
-constexpr int kUnitBytes = kUnitRows * kFp4RowBytes;  // 3328 = 26 * 128
-constexpr int kUnits = 3;                  // per K warp: a ring of its own, so that every
-                                           // waiter sees every phase of its barriers
 constexpr int kMaskSlots = 4;
 constexpr int kSoftmaxWarps = 4, kKWarps = 4, kVWarps = 4;
 constexpr int kMmaWarp = 4;
@@ -107,13 +103,11 @@ struct Smem {
   uint8_t k[9 * kKBlockBytes];
   uint8_t v[4 * kVBlockBytes];
   uint8_t p[2 * kPBlockBytes];
-  uint8_t raw[kKWarps][kUnits][kUnitBytes];
   float half_max[2][128];       // a tile's maxima per thread, by tile parity
   float lsum[128];
   uint32_t qmax[2][128];        // largest magnitudes of q's halves: latents, rope
   uint32_t vmask[kMaskSlots][4];  // a tile's live bits
   int piece_tiles[2];           // tiles of a piece, by its parity (softmax -> MMA)
-  uint64_t raw_full[kKWarps][kUnits], raw_empty[kKWarps][kUnits];
   uint64_t kfull[2], kempty[2];  // K blocks [0,4) and [4,9); kfull: even CTA
   uint64_t vfull, pfull, sempty, qready, oempty;  // even CTA, both CTAs arrive
   uint64_t sfull, pvdone, ofull, drain;           // commits
@@ -124,8 +118,7 @@ struct Smem {
 };
 static_assert(offsetof(Smem, k) % 1024 == 0 && offsetof(Smem, v) % 1024 == 0 && offsetof(Smem, p) % 1024 == 0,
               "swizzle atoms need 1024-B alignment");
-static_assert(offsetof(Smem, raw) % 128 == 0 && kUnitBytes % 128 == 0, "TMA destinations");
-static_assert(offsetof(Smem, raw_full) % 8 == 0, "");
+static_assert(offsetof(Smem, kfull) % 8 == 0, "");
 static_assert(sizeof(Smem) + 1024 <= 227 * 1024, "shared memory budget");
 
 __device__ __forceinline__ uint32_t swz(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
@@ -274,75 +267,6 @@ __device__ void settle(const Ctx& c) {
          (c.rank != 0 || wait(s.sempty, par, 48)));
 }
 
-// ------------------------------------------------------------------ producers
-// Place in a K warp's ring of units, and the times it was gone around.
-struct UnitRing {
-  int u = 0;
-  uint32_t round = 0;
-  __device__ __forceinline__ void next() {
-    if (++u == kUnits) {
-      u = 0;
-      ++round;
-    }
-  }
-};
-
-// Producer pw copies own rows [32 pw, +32) of every tile (lane = row) for K warps
-// 2 pw and 2 pw + 1: unit h of warp i holds the rows of lanes [16 i + 8 h, +8).
-__device__ void produce(const Ctx& c, const CUtensorMap* tm, int pw, int lane) {
-  const Fp4DecodeArgs& a = *c.a;
-  Smem& s = *c.s;
-  Slots<kN, 1> slots(a, s.share, c.worker, kOwn * (int)c.rank + 32 * pw + lane, 0);
-  bool ok = true;
-  int64_t armed[2] = {0, 0};
-  UnitRing ring;
-  for (int64_t j = 0; j < c.tiles && ok; ++j) {
-    const int32_t slot = slots.next(a);
-    const uint32_t live4 = __ballot_sync(0xFFFFFFFFu, slot >= 0);
-    const int32_t row = slot >= 0 ? slot : 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int l0 = 16 * i + 8 * h, kw = 2 * pw + i;
-        if (ok && ring.round > 0) ok = wait(s.raw_empty[kw][ring.u], (ring.round - 1) & 1, 40);
-        if (!ok) break;
-        const uint32_t live = (live4 >> l0) & 0xFFu;
-        const int n = __popc(live);
-        const int32_t s0 = __shfl_sync(0xFFFFFFFFu, slot, l0);
-        // consecutive slots: one bulk copy; else the groups of four rows with a live one
-        const bool run = (live & (live + 1)) == 0 &&
-                         __all_sync(0xFFFFFFFFu, (lane & 24) != l0 || slot < 0 || slot == s0 + (lane & 7));
-        const uint32_t grp = (live & 0xFu ? 1u : 0u) | (live & 0xF0u ? 2u : 0u);
-        const uint32_t full = bar(s.raw_full[kw][ring.u]);
-        const uint32_t dst = smem_u32(s.raw[kw][ring.u]);
-        if (lane == 0)
-          mbar_arrive_expect_tx(full, run ? (uint32_t)(n * kFp4RowBytes) : (uint32_t)(__popc(grp) * 4 * kFp4RowBytes));
-        __syncwarp();
-        if (run) {
-          if (lane == 0 && n > 0) bulk_g2s(dst, a.kv + (int64_t)s0 * kFp4RowBytes, (uint32_t)(n * kFp4RowBytes), full);
-        } else {
-          const int src = l0 + ((4 * lane) & 7);
-          const int32_t r0 = __shfl_sync(0xFFFFFFFFu, row, src);
-          const int32_t r1 = __shfl_sync(0xFFFFFFFFu, row, src + 1);
-          const int32_t r2 = __shfl_sync(0xFFFFFFFFu, row, src + 2);
-          const int32_t r3 = __shfl_sync(0xFFFFFFFFu, row, src + 3);
-          if (lane < 2 && ((grp >> lane) & 1u)) tma_gather4(dst + lane * 4 * kFp4RowBytes, tm, 0, r0, r1, r2, r3, full);
-        }
-        ++armed[i];
-      }
-      if (!ok) break;
-      ring.next();
-    }
-  }
-  // the units armed last have landed before the warp returns, even after a
-  // failed wait
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    for (int64_t x = armed[i] > kUnits ? armed[i] - kUnits : 0; x < armed[i]; ++x)
-      (void)wait(s.raw_full[2 * pw + i][x % kUnits], (uint32_t)(x / kUnits) & 1, 41);
-}
-
 // ------------------------------------------------------------------ K and V
 // Lane -> (row of 8, 32-dim quarter of a 128-dim latent tile): eight lanes that
 // store or load together cover four rows and two quarters, which touch every
@@ -368,33 +292,44 @@ __device__ __noinline__ void unpack32(uint4 w, uint32_t scales, uint32_t at) {
   }
 }
 
-// K warp kw: own rows [16 kw, +16) of every tile.  Rows that were not copied
-// (masked) leave what the ring held: their scores are replaced in the softmax.
+// K warp kw: own rows [16 kw, +16) of every tile, loaded into registers one tile
+// ahead.
 __device__ void k_role(const Ctx& c, int kw, int lane) {
+  const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
   const int r8 = lane_row(lane), q = lane_quarter(lane);
-  bool ok = true;
-  UnitRing ring;
-  for (int64_t j = 0; j < c.tiles && ok; ++j) {
-    // both units into registers, and back to the producer
-    uint4 w[2][4], rope[2][2];
-    uint32_t sc[2][4];
+  Slots<kN, 1> slots(a, s.share, c.worker, kOwn * (int)c.rank + 16 * kw + (lane & 15), 0);
+  uint4 w[2][4], rope[2][2];
+  uint32_t sc[2][4];
+  auto load = [&]() {
+    const int32_t slot = slots.next(a);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (ok) ok = wait(s.raw_full[kw][ring.u], ring.round & 1, 42);
-      if (!ok) break;
-      const uint8_t* row = s.raw[kw][ring.u] + r8 * kFp4RowBytes;
+      const int32_t sl = __shfl_sync(0xFFFFFFFFu, slot, 8 * h + r8);
+      if (sl >= 0) {  // a masked row keeps what the registers hold: its score is replaced
+        const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        w[h][t] = *reinterpret_cast<const uint4*>(row + 64 * t + 16 * q);
-        sc[h][t] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * t + 2 * q);
+        for (int t = 0; t < 4; ++t) {
+          w[h][t] = ldg_v4(row + 64 * t + 16 * q);
+          sc[h][t] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * t + 2 * q);
+        }
+        rope[h][0] = ldg_v4(row + kFp4RopeOff + 32 * q);
+        rope[h][1] = ldg_v4(row + kFp4RopeOff + 32 * q + 16);
       }
-      rope[h][0] = *reinterpret_cast<const uint4*>(row + kFp4RopeOff + 32 * q);
-      rope[h][1] = *reinterpret_cast<const uint4*>(row + kFp4RopeOff + 32 * q + 16);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(s.raw_empty[kw][ring.u]));
-      ring.next();
     }
+  };
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      w[h][t] = make_uint4(0, 0, 0, 0);
+      sc[h][t] = 0;
+    }
+    rope[h][0] = rope[h][1] = make_uint4(0, 0, 0, 0);
+  }
+  if (c.tiles > 0) load();
+  bool ok = true;
+  for (int64_t j = 0; j < c.tiles && ok; ++j) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {  // blocks [0,4): latent tiles 0, 1; blocks [4,9): 2, 3 and the rope
       if (ok && j > 0) ok = wait(s.kempty[g], (uint32_t)(j - 1) & 1, 43);
@@ -415,6 +350,7 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(bar(s.kfull[g]), 0);
     }
+    if (ok && j + 1 < c.tiles) load();  // behind the fences, so that none waits for loads
   }
 }
 
@@ -425,7 +361,7 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
   const int r8 = lane_row(lane), q = lane_quarter(lane), cr = (int)c.rank;
   Slots<kN, 1> slots(a, s.share, c.worker, 32 * vw + lane, 0);
   uint4 w[4][2];
-  uint32_t sc[4];  // the two scales of each tile half
+  uint32_t sc[4][2];  // (kept apart until they are used: combining them would wait for the loads)
   uint32_t live = 0;
   auto load = [&]() {
     const int32_t slot = slots.next(a);
@@ -437,11 +373,11 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
         const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
         w[i][0] = ldg_v4(row + 64 * cr + 16 * q);
         w[i][1] = ldg_v4(row + 64 * (cr + 2) + 16 * q);
-        sc[i] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * cr + 2 * q) |
-                ((uint32_t)*reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * (cr + 2) + 2 * q) << 16);
+        sc[i][0] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * cr + 2 * q);
+        sc[i][1] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * (cr + 2) + 2 * q);
       } else {  // zeros: P is 0 there, and nothing else may be
         w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
-        sc[i] = 0;
+        sc[i][0] = sc[i][1] = 0;
       }
     }
   };
@@ -458,8 +394,8 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
     for (int i = 0; i < 4; ++i) {
       const uint32_t r = 32 * vw + 8 * i + r8;
       const uint32_t at = smem_u32(s.v + (q >> 1) * kVBlockBytes + swz(r, 4 * (q & 1)));
-      unpack32(w[i][0], sc[i] & 0xFFFFu, at);
-      unpack32(w[i][1], sc[i] >> 16, at + 2 * kVBlockBytes);
+      unpack32(w[i][0], sc[i][0], at);
+      unpack32(w[i][1], sc[i][1], at + 2 * kVBlockBytes);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -740,7 +676,7 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    decode_fp4_tc_kernel(const Fp4DecodeArgs a, const __grid_constant__ CUtensorMap tm) {
+    decode_fp4_tc_kernel(const Fp4DecodeArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
   Smem& s = *reinterpret_cast<Smem*>(smem_raw + (((raw_base + 1023u) & ~1023u) - raw_base));
@@ -752,10 +688,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   c.rank = cluster_rank();  // == blockIdx.x & 1
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kKWarps * kUnits; ++i) {
-      mbar_init(bar(s.raw_full[0][i]), 1);
-      mbar_init(bar(s.raw_empty[0][i]), 1);
-    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(s.kfull[i]), 2 * kKWarps);
       mbar_init(bar(s.kempty[i]), 1);
@@ -798,9 +730,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     settle(c);
   } else if (warp < 8 || warp == 9) {
     k_role(c, warp < 8 ? warp - 5 : 3, lane);
-  } else if (warp == 8 || warp == 15) {
-    produce(c, &tm, warp == 8 ? 0 : 1, lane);
-  } else if (warp != 12) {
+  } else if (warp != 8 && warp < 15 && warp != 12) {
     v_role(c, warp < 12 ? warp - 10 : warp - 11, lane);
   }
 
@@ -818,14 +748,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }  // namespace
 
 int launch_decode_fp4_tc(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st) {
-  CUtensorMap tm{};
-  if (a.num_slots > 0)
-    if (int rc = encode_fp4_row_map(&tm, a.kv, a.num_slots)) return rc;
   const size_t smem = sizeof(Smem) + 1024;  // + alignment slack
   static SmemLimit limit;
   if (int rc = limit.raise(decode_fp4_tc_kernel, smem)) return rc;
   if (int rc = check_cuda(launch_pdl(decode_fp4_tc_kernel, dim3((unsigned)(2 * a.workers)), dim3(kThreads), smem, st,
-                                     a, tm),
+                                     a),
                           "decode_fp4_tc_kernel launch"))
     return rc;
   return cuts ? launch_merge_fp4(a, kBias, st) : FP8MLA_OK;
