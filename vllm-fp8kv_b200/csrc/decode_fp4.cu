@@ -127,13 +127,15 @@ struct Ring {
 // a time through gather4; masked rows are not read (a group with some fetches
 // row 0 for them) and their bits stay clear.
 __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, int pw, int lane) {
-  Slots<kBN, 2> slots(a, s.share, blockIdx.x, 16 * pw + (lane & 15), lane >> 4);
+  Slots<kBN, 2, 1> slots(a, s.share, blockIdx.x, 16 * pw + (lane & 15), lane >> 4);
   const int64_t chunks = Walk<kBN>(a, s.share, blockIdx.x).left;
   bool ok = true;
   int64_t armed = 0;
   Ring ring;
   for (int64_t g = 0; g < chunks && ok; g += 2) {
-    const int32_t slot = slots.next(a);
+    int32_t at[1];
+    slots.next(a, at);
+    const int32_t slot = at[0];
     const uint32_t live2 = __ballot_sync(0xFFFFFFFFu, slot >= 0);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {

@@ -50,19 +50,17 @@
 //   warps 0-3         softmax, q, and the stores of O
 //   warp 4            tensor memory allocation; lane 0 of the even CTA issues
 //                     every MMA of the pair
-//   warps 5, 6, 7, 9  K: own rows [16i, +16) of every tile: entries -> slots ->
-//                     TMA copies into the warp's raw ring -> K blocks
+//   warps 5, 6, 7, 9  K: own rows [16i, +16) of every tile, loaded into registers
+//                     a tile ahead -> K blocks
 //   warps 10, 11, 13, 14
-//                     V: entries [32i, +32) of every tile, the half's codes and
-//                     scales by register loads one tile ahead -> V blocks; and
-//                     the tile's live bits
-//   warps 8, 12, 15   idle: sub-partition 0 runs the issuing warp and one softmax
+//                     V: the half of entries [32i, +32) of every tile, likewise
+//   warp 15           scout: entries -> slots and live bits of all 128 entries
+//   warps 8, 12       idle: sub-partition 0 runs the issuing warp and one softmax
 //                     warp alone
 // Barriers that gate the issuing thread live in the even CTA and count arrivals
 // of both CTAs; the completion of pair MMAs reaches both CTAs through a multicast
-// commit.  Every wait is bounded; after a failed wait a role stops, and the
-// producers wait (with the full limit) for the copies they issued, so none
-// outlives the CTA.  No load uses cluster multicast.
+// commit.  Every wait is bounded, and a role stops after a failed one.  No load uses
+// cluster multicast; there are no copies that could outlive the CTA.
 #include "decode_fp4.h"
 #include "fp4.cuh"
 #include "fp4_walk.cuh"
@@ -80,7 +78,7 @@ constexpr int kQBlockBytes = 64 * 128;
 constexpr int kKBlockBytes = kOwn * 128;   // 8 KB: 64 own rows of a 64-dim block
 constexpr int kVBlockBytes = kN * 128;     // 16 KB
 constexpr int kPBlockBytes = 64 * 128;     // 64 heads x 64 entries
-constexpr int kMaskSlots = 4;
+constexpr int kScoutRing = 4;               // tiles of slots
 constexpr int kSoftmaxWarps = 4, kKWarps = 4, kVWarps = 4;
 constexpr int kMmaWarp = 4;
 constexpr int kThreads = 16 * 32;
@@ -106,12 +104,13 @@ struct Smem {
   float half_max[2][128];       // a tile's maxima per thread, by tile parity
   float lsum[128];
   uint32_t qmax[2][128];        // largest magnitudes of q's halves: latents, rope
-  uint32_t vmask[kMaskSlots][4];  // a tile's live bits
+  int32_t slot[kScoutRing][kN];   // a tile's slots, and its live bits
+  uint32_t vmask[kScoutRing][4];
   int piece_tiles[2];           // tiles of a piece, by its parity (softmax -> MMA)
   uint64_t kfull[2], kempty[2];  // K blocks [0,4) and [4,9); kfull: even CTA
   uint64_t vfull, pfull, sempty, qready, oempty;  // even CTA, both CTAs arrive
   uint64_t sfull, pvdone, ofull, drain;           // commits
-  uint64_t mfull[kMaskSlots];
+  uint64_t slots_full[kScoutRing], slots_empty[kScoutRing];
   uint64_t meet;                // the softmax warps of this CTA
   Share share;
   uint32_t tmem_base;
@@ -163,91 +162,83 @@ __device__ __forceinline__ void commit(uint64_t& b) {
       "h"((uint16_t)3)
       : "memory");
 }
-// The issue loops stay rolled, four MMAs a turn: straight-line code for all 52
-// MMAs of a tile is fetched anew for every tile.
-// K blocks [from, to) with q in tensor memory (blocks below 6) ...
-__device__ __forceinline__ void issue_s_tmem(uint32_t tS, uint32_t tQ, uint64_t kdesc, int from, int to) {
-#pragma unroll 1
-  for (int b = from; b < to; ++b) {
-    const uint64_t bd = kdesc + (uint64_t)((b * kKBlockBytes) >> 4);
-    const uint32_t aq = tQ + 32 * b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pair_ts(tS, aq + 8 * i, bd + (uint64_t)(2 * i), kIdescLatent, (b | i) ? 1u : 0u);
-  }
-}
-// ... and with q in shared memory (6 and 7 latents, 8 the rope)
-__device__ __forceinline__ void issue_s_smem(uint32_t tS, uint64_t qdesc, uint64_t kdesc) {
-#pragma unroll 1
-  for (int b = 6; b < 9; ++b) {
-    const uint64_t bd = kdesc + (uint64_t)((b * kKBlockBytes) >> 4);
-    const uint64_t ad = qdesc + (uint64_t)(((b - 6) * kQBlockBytes) >> 4);
-    const uint32_t id = b < 8 ? kIdescLatent : kIdescRope;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pair_ss(tS, ad + (uint64_t)(2 * i), bd + (uint64_t)(2 * i), id, 1u);
-  }
-}
-
+// The role is two short loops of four MMAs a turn, entered once a tile: code that
+// is met again only a tile later is fetched anew each time.
 __device__ void mma_role(const Ctx& c) {
   Smem& s = *c.s;
-  const uint32_t tQ = c.tmem + kColQ, tS = c.tmem + kColS;
-  const uint64_t qdesc0 = sdesc_sw128(smem_u32(s.q), 16, 1024);
-  const uint64_t kdesc0 = sdesc_sw128(smem_u32(s.k), 16, 1024);
-  const uint64_t pdesc0 = sdesc_sw128(smem_u32(s.p), 16, 1024);
-  const uint64_t vdesc0 = sdesc_sw128(smem_u32(s.v), kVBlockBytes, 1024);
-  bool ok = true;
+  const uint32_t tQ = c.tmem + kColQ, tS = c.tmem + kColS, tO = c.tmem + kColO;
+  const uint64_t qdesc = sdesc_sw128(smem_u32(s.q), 16, 1024);
+  const uint64_t kdesc = sdesc_sw128(smem_u32(s.k), 16, 1024);
+  const uint64_t pdesc = sdesc_sw128(smem_u32(s.p), 16, 1024);
+  const uint64_t vdesc = sdesc_sw128(smem_u32(s.v), kVBlockBytes, 1024);
   const uint32_t tiles = (uint32_t)c.tiles;
-  uint32_t j = 0;                     // tile of the run
+  uint32_t p = 0;                     // pieces opened
+  int left = 0;                       // tiles of the open piece still to come
   bool first = false, last = false;   // tile j - 1 opens / closes its piece
-  uint32_t piece = 0;                 // piece of tile j - 1
-  // O of tile j - 1
-  auto issue_o = [&]() {
-    if (!ok) return;
-    if (first && piece > 0) ok = wait(s.oempty, (piece - 1) & 1, 45);
-    if (ok) ok = wait(s.pfull, (j - 1) & 1, 36);
-    if (ok) ok = wait(s.vfull, (j - 1) & 1, 38);
-    if (!ok) return;
-    tc_fence_after();
+  auto ts_blocks = [&](int from, int to) {
 #pragma unroll 1
-    for (int x = 0; x < 4; ++x) {  // half x / 2 of the dims, entries [64 (x % 2), +64)
-      const uint64_t ad = pdesc0 + (uint64_t)(((x & 1) * kPBlockBytes) >> 4);
-      const uint64_t bd = vdesc0 + (uint64_t)(((x >> 1) * 2 * kVBlockBytes + (x & 1) * 64 * 128) >> 4);
+    for (int b = from; b < to; ++b) {
+      const uint64_t bd = kdesc + (uint64_t)((b * kKBlockBytes) >> 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        pair_ss(c.tmem + kColO + 128 * (x >> 1), ad + (uint64_t)(2 * i), bd + (uint64_t)((i * 16 * 128) >> 4),
-                    kIdescPV, ((x & 1) || i > 0 || !first) ? 1u : 0u);
+        pair_ts(tS, tQ + 32 * b + 8 * i, bd + (uint64_t)(2 * i), kIdescLatent, (b | i) ? 1u : 0u);
     }
-    commit(s.pvdone);  // P and V may be written again
-    if (last) commit(s.ofull);
   };
-  uint32_t p = 0;
-  while (j < tiles && ok) {
-    ok = wait(s.qready, p & 1, 35);
-    if (!ok) break;
-    const int n = s.piece_tiles[p & 1];
-    for (int i = 0; i < n && ok; ++i) {
-      if (j > 0) ok = wait(s.sempty, (j - 1) & 1, 34);
-      if (ok) ok = wait(s.kfull[0], j & 1, 37);
-      if (!ok) break;
+  // turn j: S of tile j, then O of tile j - 1
+  for (uint32_t j = 0; j <= tiles && tiles > 0; ++j) {
+    const bool has_s = j < tiles;
+    bool opens = false;
+    if (has_s) {
+      if (left == 0) {
+        if (!wait(s.qready, p & 1, 35)) return;
+        left = s.piece_tiles[p & 1];
+        ++p;
+        opens = true;
+      }
+      if (j > 0 && !wait(s.sempty, (j - 1) & 1, 34)) return;
+      if (!wait(s.kfull[0], j & 1, 37)) return;
       tc_fence_after();
-      issue_s_tmem(tS, tQ, kdesc0, 0, 4);
+      // K blocks 0-5: q in tensor memory
+      ts_blocks(0, 4);
       commit(s.kempty[0]);
-      ok = wait(s.kfull[1], j & 1, 39);
-      if (!ok) break;
+      if (!wait(s.kfull[1], j & 1, 39)) return;
       tc_fence_after();
-      issue_s_tmem(tS, tQ, kdesc0, 4, 6);
-      issue_s_smem(tS, qdesc0, kdesc0);
+      ts_blocks(4, 6);
+      // blocks 6, 7 (latents) and 8 (rope): q in shared memory
+#pragma unroll 1
+      for (int b = 0; b < 3; ++b) {
+        const uint64_t ad = qdesc + (uint64_t)((b * kQBlockBytes) >> 4);
+        const uint64_t bd = kdesc + (uint64_t)(((6 + b) * kKBlockBytes) >> 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          pair_ss(tS, ad + (uint64_t)(2 * i), bd + (uint64_t)(2 * i), b < 2 ? kIdescLatent : kIdescRope, 1u);
+      }
       commit(s.kempty[1]);
       commit(s.sfull);
-      if (j > 0) issue_o();
-      first = i == 0;
-      last = i == n - 1;
-      piece = p;
-      ++j;
     }
-    ++p;
+    if (j > 0) {
+      // (piece p - 1 - opens holds tile j - 1)
+      const uint32_t piece = p - 1 - (opens ? 1 : 0);
+      if (first && piece > 0 && !wait(s.oempty, (piece - 1) & 1, 45)) return;
+      if (!wait(s.pfull, (j - 1) & 1, 36)) return;
+      if (!wait(s.vfull, (j - 1) & 1, 38)) return;
+      tc_fence_after();
+#pragma unroll 1
+      for (int x = 0; x < 4; ++x) {  // dims half x / 2, entries [64 (x % 2), +64)
+        const uint64_t ad = pdesc + (uint64_t)(((x & 1) * kPBlockBytes) >> 4);
+        const uint64_t bd = vdesc + (uint64_t)(((x >> 1) * 2 * kVBlockBytes + (x & 1) * 64 * 128) >> 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          pair_ss(tO + 128 * (x >> 1), ad + (uint64_t)(2 * i), bd + (uint64_t)((i * 16 * 128) >> 4), kIdescPV,
+                  (x & 1) || i > 0 || !first ? 1u : 0u);
+      }
+      commit(s.pvdone);  // P and V may be written again
+      if (last) commit(s.ofull);
+    }
+    first = opens;
+    --left;
+    last = left == 0;
   }
-  if (j > 0) issue_o();
-  commit(s.drain);  // see settle()
 }
 
 // The MMA warp of both CTAs: every arrival that is still on its way to one of
@@ -260,11 +251,34 @@ __device__ void mma_role(const Ctx& c) {
 // is not signalled for the last unit.)
 __device__ void settle(const Ctx& c) {
   Smem& s = *c.s;
+  if (c.rank == 0) commit(s.drain);
   if (!wait(s.drain, 0, 46) || c.tiles == 0) return;
   const uint32_t par = (uint32_t)(c.tiles - 1) & 1;
   (void)(wait(s.kempty[0], par, 48) && wait(s.kempty[1], par, 48) &&
          wait(s.pvdone, par, 48) &&
          (c.rank != 0 || wait(s.sempty, par, 48)));
+}
+
+// ------------------------------------------------------------------ scout
+// Entries -> slots for all 128 entries of a tile, up to four tiles ahead.
+__device__ void scout(const Ctx& c, int lane) {
+  const Fp4DecodeArgs& a = *c.a;
+  Smem& s = *c.s;
+  Slots<kN, 1, 4> slots(a, s.share, c.worker, lane, 0);
+  for (int64_t j = 0; j < c.tiles; ++j) {
+    const int r = (int)(j % kScoutRing);
+    int32_t slot[4];
+    slots.next(a, slot);
+    if (j >= kScoutRing && !wait(s.slots_empty[r], (uint32_t)(j / kScoutRing + 1) & 1, 40)) break;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s.slot[r][32 * i + lane] = slot[i];
+      const uint32_t live = __ballot_sync(0xFFFFFFFFu, slot[i] >= 0);
+      if (lane == 0) s.vmask[r][i] = live;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(s.slots_full[r]));
+  }
 }
 
 // ------------------------------------------------------------------ K and V
@@ -298,14 +312,18 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
   const int r8 = lane_row(lane), q = lane_quarter(lane);
-  Slots<kN, 1> slots(a, s.share, c.worker, kOwn * (int)c.rank + 16 * kw + (lane & 15), 0);
   uint4 w[2][4], rope[2][2];
   uint32_t sc[2][4];
-  auto load = [&]() {
-    const int32_t slot = slots.next(a);
+  auto load = [&](uint32_t j) -> bool {
+    const uint32_t r = j % kScoutRing;
+    if (!wait(s.slots_full[r], (j / kScoutRing) & 1, 41)) return false;
+    const int32_t* at = s.slot[r] + kOwn * (int)c.rank + 16 * kw + r8;
+    const int32_t slot[2] = {at[0], at[8]};
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(s.slots_empty[r]));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int32_t sl = __shfl_sync(0xFFFFFFFFu, slot, 8 * h + r8);
+      const int32_t sl = slot[h];
       if (sl >= 0) {  // a masked row keeps what the registers hold: its score is replaced
         const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
 #pragma unroll
@@ -317,6 +335,7 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
         rope[h][1] = ldg_v4(row + kFp4RopeOff + 32 * q + 16);
       }
     }
+    return true;
   };
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -327,12 +346,12 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
     }
     rope[h][0] = rope[h][1] = make_uint4(0, 0, 0, 0);
   }
-  if (c.tiles > 0) load();
-  bool ok = true;
-  for (int64_t j = 0; j < c.tiles && ok; ++j) {
+  const uint32_t tiles = (uint32_t)c.tiles;
+  bool ok = tiles > 0 && load(0);
+  for (uint32_t j = 0; j < tiles && ok; ++j) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {  // blocks [0,4): latent tiles 0, 1; blocks [4,9): 2, 3 and the rope
-      if (ok && j > 0) ok = wait(s.kempty[g], (uint32_t)(j - 1) & 1, 43);
+      if (ok && j > 0) ok = wait(s.kempty[g], (j - 1) & 1, 43);
       if (!ok) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -350,7 +369,7 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(bar(s.kfull[g]), 0);
     }
-    if (ok && j + 1 < c.tiles) load();  // behind the fences, so that none waits for loads
+    if (ok && j + 1 < tiles) ok = load(j + 1);  // behind the fences, so that none waits for loads
   }
 }
 
@@ -359,16 +378,18 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
   const int r8 = lane_row(lane), q = lane_quarter(lane), cr = (int)c.rank;
-  Slots<kN, 1> slots(a, s.share, c.worker, 32 * vw + lane, 0);
   uint4 w[4][2];
   uint32_t sc[4][2];  // (kept apart until they are used: combining them would wait for the loads)
-  uint32_t live = 0;
-  auto load = [&]() {
-    const int32_t slot = slots.next(a);
-    live = __ballot_sync(0xFFFFFFFFu, slot >= 0);
+  auto load = [&](uint32_t j) -> bool {
+    const uint32_t r = j % kScoutRing;
+    if (!wait(s.slots_full[r], (j / kScoutRing) & 1, 42)) return false;
+    const int32_t* at = s.slot[r] + 32 * vw + r8;
+    const int32_t slot[4] = {at[0], at[8], at[16], at[24]};
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(s.slots_empty[r]));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int32_t sl = __shfl_sync(0xFFFFFFFFu, slot, 8 * i + r8);
+      const int32_t sl = slot[i];
       if (sl >= 0) {
         const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
         w[i][0] = ldg_v4(row + 64 * cr + 16 * q);
@@ -380,16 +401,12 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
         sc[i][0] = sc[i][1] = 0;
       }
     }
+    return true;
   };
-  if (c.tiles > 0) load();
-  for (int64_t j = 0; j < c.tiles; ++j) {
-    // The slot's reader of tile j - 4 is done: this warp saw O of tile j - 2
-    // complete before it wrote V of tile j - 1.
-    if (lane == 0) {
-      s.vmask[j % kMaskSlots][vw] = live;
-      mbar_arrive(bar(s.mfull[j % kMaskSlots]));
-    }
-    if (j > 0 && !wait(s.pvdone, (uint32_t)(j - 1) & 1, 44)) break;
+  const uint32_t tiles = (uint32_t)c.tiles;
+  bool ok = tiles > 0 && load(0);
+  for (uint32_t j = 0; j < tiles && ok; ++j) {
+    if (j > 0 && !wait(s.pvdone, (j - 1) & 1, 44)) break;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t r = 32 * vw + 8 * i + r8;
@@ -400,7 +417,7 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive_cluster(bar(s.vfull), 0);
-    if (j + 1 < c.tiles) load();  // behind the fence, so that it waits for no load
+    if (j + 1 < tiles) ok = load(j + 1);  // behind the fence, so that it waits for no load
   }
 }
 
@@ -550,10 +567,10 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
     for (int i = 0; i < n; ++i, ++j) {
       const uint32_t par = j & 1;
       ok = wait(s.sfull, par, 31);
-      const uint32_t mslot = j % kMaskSlots, mpar = (j / kMaskSlots) & 1;
-      if (ok) ok = wait(s.mfull[mslot], mpar, 30);
+      const uint32_t r = j % kScoutRing;
+      if (ok) ok = wait(s.slots_full[r], (j / kScoutRing) & 1, 30);
       if (!ok) break;
-      const uint32_t live0 = s.vmask[mslot][2 * hh], live1 = s.vmask[mslot][2 * hh + 1];
+      const uint32_t live0 = s.vmask[r][2 * hh], live1 = s.vmask[r][2 * hh + 1];
       tc_fence_after();
       uint32_t sv[64];
       tmem_ld32(trow + kColS, reinterpret_cast<uint32_t(&)[32]>(sv[0]));
@@ -561,7 +578,10 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(bar(s.sempty), 0);  // S may be written again
+      if (lane == 0) {
+        mbar_arrive_cluster(bar(s.sempty), 0);  // S may be written again
+        mbar_arrive(bar(s.slots_empty[r]));
+      }
       if ((live0 & live1) != 0xFFFFFFFFu) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
@@ -692,7 +712,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(bar(s.kfull[i]), 2 * kKWarps);
       mbar_init(bar(s.kempty[i]), 1);
     }
-    for (int i = 0; i < kMaskSlots; ++i) mbar_init(bar(s.mfull[i]), kVWarps);
+    for (int i = 0; i < kScoutRing; ++i) {
+      mbar_init(bar(s.slots_full[i]), 1);
+      mbar_init(bar(s.slots_empty[i]), kKWarps + kVWarps + kSoftmaxWarps);
+    }
     mbar_init(bar(s.vfull), 2 * kVWarps);
     mbar_init(bar(s.pfull), 2 * kSoftmaxWarps);
     mbar_init(bar(s.sempty), 2 * kSoftmaxWarps);
@@ -730,7 +753,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     settle(c);
   } else if (warp < 8 || warp == 9) {
     k_role(c, warp < 8 ? warp - 5 : 3, lane);
-  } else if (warp != 8 && warp < 15 && warp != 12) {
+  } else if (warp == 15) {
+    scout(c, lane);
+  } else if (warp != 8 && warp != 12) {
     v_role(c, warp < 12 ? warp - 10 : warp - 11, lane);
   }
 

@@ -153,16 +153,16 @@ __device__ __forceinline__ int32_t slot_of(const Fp4DecodeArgs& a, int32_t v, in
   return s >= 0 && s < a.num_slots ? (int32_t)s : -1;
 }
 
-// The slots of one row of every `kStride`-th chunk of a worker's run, entries
-// read three steps ahead of their use and block-table words two steps ahead,
-// so that neither latency is waited for.
-template <int kChunk, int kStride>
+// The slots of rows row, row + 32, .. (kRows of them) of every `kStride`-th chunk
+// of a worker's run, entries read three steps ahead of their use and block-table
+// words two steps ahead, so that neither latency is waited for.
+template <int kChunk, int kStride, int kRows>
 struct Slots {
   Walk<kChunk> ahead;
   int row;
   int32_t req = 0;
   const int32_t* idx_row = nullptr;
-  int32_t v[3], rq[3], pg[2];  // of the current step and the next ones
+  int32_t v[3][kRows], rq[3], pg[2][kRows];  // of the current step and the next ones
   __device__ __forceinline__ void at_unit(const Fp4DecodeArgs& a) {
     if (ahead.left <= 0) return;
     if (a.block_table != nullptr) req = a.req_id[ahead.t];
@@ -174,38 +174,47 @@ struct Slots {
       at_unit(a);
     }
   }
-  __device__ __forceinline__ int32_t fetch(const Fp4DecodeArgs& a) const {
-    const int pos = ahead.c * kChunk + row;
-    if (ahead.left <= 0 || pos >= ahead.entries) return -1;
-    return a.lens == nullptr ? idx_row[pos] : pos;
+  __device__ __forceinline__ void fetch(const Fp4DecodeArgs& a, int32_t (&e)[kRows]) const {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int pos = ahead.c * kChunk + row + 32 * i;
+      e[i] = ahead.left <= 0 || pos >= ahead.entries ? -1 : a.lens == nullptr ? idx_row[pos] : pos;
+    }
   }
-  // row `row` of chunks first, first + kStride, ... of the run
+  __device__ __forceinline__ void words(const Fp4DecodeArgs& a, int32_t r, const int32_t (&e)[kRows],
+                                        int32_t (&p)[kRows]) const {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) p[i] = table_word(a, r, e[i]);
+  }
+  // of chunks first, first + kStride, ... of the run
   __device__ __forceinline__ Slots(const Fp4DecodeArgs& a, const Share& s, int worker, int row_, int first)
       : ahead(a, s, worker), row(row_) {
     at_unit(a);
     for (int i = 0; i < first; ++i) step(a);
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      v[i] = fetch(a);
+      fetch(a, v[i]);
       rq[i] = req;
 #pragma unroll
       for (int k = 0; k < kStride; ++k) step(a);
     }
-    pg[0] = table_word(a, rq[0], v[0]);
-    pg[1] = table_word(a, rq[1], v[1]);
+    words(a, rq[0], v[0], pg[0]);
+    words(a, rq[1], v[1], pg[1]);
   }
-  __device__ __forceinline__ int32_t next(const Fp4DecodeArgs& a) {
-    const int32_t slot = slot_of(a, v[0], pg[0]);
-    v[0] = v[1];
-    v[1] = v[2];
+  __device__ __forceinline__ void next(const Fp4DecodeArgs& a, int32_t (&slot)[kRows]) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      slot[i] = slot_of(a, v[0][i], pg[0][i]);
+      v[0][i] = v[1][i];
+      v[1][i] = v[2][i];
+      pg[0][i] = pg[1][i];
+    }
     rq[1] = rq[2];
-    v[2] = fetch(a);
+    fetch(a, v[2]);
     rq[2] = req;
-    pg[0] = pg[1];
-    pg[1] = table_word(a, rq[1], v[1]);
+    words(a, rq[1], v[1], pg[1]);
 #pragma unroll
     for (int k = 0; k < kStride; ++k) step(a);
-    return slot;
   }
 };
 
