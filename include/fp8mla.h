@@ -386,7 +386,7 @@ FP8MLA_API int fp8mla_fp4_gather(const uint8_t* kv, int64_t num_slots, const int
                                  const int32_t* cu_seq_lens, int64_t B, const int32_t* seq_starts,
                                  int64_t n, uint16_t* out, int64_t out_stride, void* stream);
 
-/* Bytes of device workspace an attention call below needs (16-byte aligned;
+/* Bytes of device workspace an attention call below needs (32-byte aligned;
  * the contents need no initialisation and carry nothing from call to call;
  * calls that may run at once need one each).  topk: the index rows' width (0
  * bytes where whole rows go to single SMs), or -1 for whole contexts, which is

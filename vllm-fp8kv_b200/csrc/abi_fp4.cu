@@ -96,8 +96,9 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
 
   const int64_t hpg = H / G;
   const Plan p = plan_of(T, H, G, lens != nullptr ? -1 : topk, max_blocks * block_size);
-  if (p.cuts && (workspace == nullptr || workspace_bytes < workspace_of(p) || !aligned16(workspace)))
-    return set_error(FP8MLA_ERR_WORKSPACE, "needs %lld bytes of 16-B aligned workspace, got %lld",
+  if (p.cuts && (workspace == nullptr || workspace_bytes < workspace_of(p) ||
+                 (reinterpret_cast<uintptr_t>(workspace) & 31u) != 0))
+    return set_error(FP8MLA_ERR_WORKSPACE, "needs %lld bytes of 32-B aligned workspace, got %lld",
                      (long long)workspace_of(p), (long long)workspace_bytes);
   Fp4DecodeArgs a{};
   a.q = q;

@@ -566,15 +566,38 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------ merge
-// Block (w, y) joins the pieces of the unit that the border in front of worker
-// w cuts first, for one head: out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i.
-__global__ void __launch_bounds__(128) merge_fp4_kernel(const Fp4DecodeArgs a, float bias) {
-  if (threadIdx.x == 0) pdl_launch_dependents();
+// Joins the pieces of a cut unit for one head: out = sum 2^(m_i - m) O_i /
+// sum 2^(m_i - m) l_i.  A unit's first border is the one in front of a worker
+// that starts in it at most `per` chunks behind its start.
+//   kSplit 1  block (w - 1, head) joins the unit that worker w's border is the first
+//             to cut, if it is; most units have two or three pieces
+//   kSplit 4  block (unit, head), for calls of few units, which many workers share
+//             (74 or 148 pieces of one long context): each of four groups of 128
+//             threads takes every fourth piece, eight loads in flight
+//             (131071 positions, 128 heads: 6 instead of 20 us)
+template <int kSplit>
+__global__ void __launch_bounds__(128 * kSplit) merge_fp4_kernel(const Fp4DecodeArgs a, float bias) {
+  __shared__ int border;
+  __shared__ __align__(16) float part[kSplit][128][4];
+  if (threadIdx.x == 0) {
+    pdl_launch_dependents();
+    border = 0;
+  }
   pdl_wait();
-  const int w = blockIdx.x + 1;
+  int w = blockIdx.x + 1;
+  if (kSplit > 1) {
+    __syncthreads();
+    for (int i = threadIdx.x + 1; i < a.workers; i += 128 * kSplit) {
+      const int64_t* info = a.ws_info + 4 * (int64_t)i;
+      if (info[1] > 0 && info[1] <= info[3] && info[0] == blockIdx.x) border = i;
+    }
+    __syncthreads();
+    w = border;
+    if (w == 0) return;
+  }
   const int64_t* info = a.ws_info + 4 * (int64_t)w;
   const int64_t c = info[1], per = info[3];
-  if (c == 0 || c > per) return;  // no cut here, or cut by an earlier border too
+  if (c == 0 || c > per) return;  // no cut here, or an earlier border cuts the unit too
   const int64_t unit = info[0], n = info[2];
   const int pieces = 1 + (int)((n - c + per - 1) / per);
   const int per_tok = a.G * a.hb_per_group;
@@ -582,28 +605,47 @@ __global__ void __launch_bounds__(128) merge_fp4_kernel(const Fp4DecodeArgs a, f
   const int rest = (int)(unit - t * per_tok), grp = rest / a.hb_per_group, hb = rest - grp * a.hb_per_group;
   const int row = blockIdx.y;
   if (row >= min(a.rows, a.hpg - hb * a.rows)) return;
-  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)(w - 1) + 1 : 2 * (int64_t)(w - 1 + i); };
-  float m = -INFINITY;
-  for (int i = 0; i < pieces; ++i) m = fmaxf(m, a.ws_ml[slot(i) * a.rows + row].x);
+  // workspace row of piece i
+  auto at = [&](int i) -> int64_t { return (i == 0 ? 2 * (int64_t)w - 1 : 2 * (int64_t)(w - 1 + i)) * a.rows + row; };
+  const int lane = threadIdx.x & 31, g4 = threadIdx.x >> 7, d4 = threadIdx.x & 127;
+  // every warp: the maximum, then the sum
+  float m = -INFINITY, l = 0.f;
+  for (int i = lane; i < pieces; i += 32) m = fmaxf(m, a.ws_ml[at(i)].x);
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   const float ref = m == -INFINITY ? 0.f : m;
+  for (int i = lane; i < pieces; i += 32) {
+    const float2 ml = a.ws_ml[at(i)];
+    l += exp2f(ml.x - ref) * ml.y;
+  }
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < pieces; ++i) {
-    const float2 ml = a.ws_ml[slot(i) * a.rows + row];
-    const float4 o = reinterpret_cast<const float4*>(a.ws_o + (slot(i) * a.rows + row) * kNope)[threadIdx.x];
-    const float f = exp2f(ml.x - ref);
-    l += f * ml.y;
+#pragma unroll 8
+  for (int i = g4; i < pieces; i += kSplit) {
+    const float4 o = reinterpret_cast<const float4*>(a.ws_o + at(i) * kNope)[d4];
+    const float f = exp2f(a.ws_ml[at(i)].x - ref);
     acc.x += f * o.x;
     acc.y += f * o.y;
     acc.z += f * o.z;
     acc.w += f * o.w;
   }
+  if (kSplit > 1) {
+    *reinterpret_cast<float4*>(part[g4][d4]) = acc;
+    __syncthreads();
+    if (g4 != 0) return;
+#pragma unroll
+    for (int g = 1; g < kSplit; ++g) {
+      const float4 o = *reinterpret_cast<const float4*>(part[g][d4]);
+      acc.x += o.x;
+      acc.y += o.y;
+      acc.z += o.z;
+      acc.w += o.w;
+    }
+  }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const int64_t h = (int64_t)grp * a.hpg + hb * a.rows + row;
-  reinterpret_cast<uint2*>(a.out + t * a.out_st + h * a.out_sh)[threadIdx.x] =
+  reinterpret_cast<uint2*>(a.out + t * a.out_st + h * a.out_sh)[d4] =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  if (a.lse != nullptr && threadIdx.x == 0)
+  if (a.lse != nullptr && d4 == 0)
     a.lse[t * a.lse_st + h] = l == 0.f ? -INFINITY : (m - bias) * kLn2 + logf(l);
 }
 
@@ -611,9 +653,13 @@ __global__ void __launch_bounds__(128) merge_fp4_kernel(const Fp4DecodeArgs a, f
 
 int launch_merge_fp4(const Fp4DecodeArgs& a, float bias, cudaStream_t st) {
   if (a.workers < 2) return FP8MLA_OK;
-  return check_cuda(launch_pdl(merge_fp4_kernel, dim3((unsigned)(a.workers - 1), (unsigned)a.rows), dim3(128), 0, st,
-                               a, bias),
-                    "merge_fp4_kernel launch");
+  const int64_t units = (int64_t)a.T * a.G * a.hb_per_group;
+  const cudaError_t e =
+      units * 8 <= a.workers
+          ? launch_pdl(merge_fp4_kernel<4>, dim3((unsigned)units, (unsigned)a.rows), dim3(512), 0, st, a, bias)
+          : launch_pdl(merge_fp4_kernel<1>, dim3((unsigned)(a.workers - 1), (unsigned)a.rows), dim3(128), 0, st, a,
+                       bias);
+  return check_cuda(e, "merge_fp4_kernel launch");
 }
 
 int launch_decode_fp4(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st) {

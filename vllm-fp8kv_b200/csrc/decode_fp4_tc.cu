@@ -450,75 +450,60 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, M
     return __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
   };
   const uint32_t trow = c.tmem + ((uint32_t)((L >> 5) * 32) << 16);
-  // q times 2^k; returns the largest magnitudes (as bits) of the latents and of
-  // the rope among what this thread converted
-  auto convert = [&](int k, uint32_t& mx, uint32_t& mr) {
+  // First as it is, which is exact enough where the head's largest latent magnitude
+  // lies in [2^-2, 2^15] (an fp16 subnormal's error is below 2^-23 of it then).
+  // Else again times 2^k, which brings that magnitude to [2^8, 2^9), but the rope's at
+  // most to 2^101, where its products are still finite (1 for rows of zeros, inf
+  // or NaN).  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.  (Short
+  // loops: the code runs once a unit and comes from memory each time.)
+  int k = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
     // the sign of the softmax scale goes with q, so that scores scale by a positive factor
     const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), a.scale_log2);
-    auto f16 = [&](const uint4& v) {
-      auto one = [&](uint32_t u) { return pack_f16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
-      return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
-    };
-    auto bf = [&](const uint4& v) {
-      auto one = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
-      return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
-    };
-    mx = mr = 0;
-    {
-      uint4 x[12];
+    auto f16 = [&](uint32_t u) { return pack_f16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
+    auto bf = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
+    uint32_t mx = 0, mr = 0;
+    uint4 x[8], y[12];
 #pragma unroll
-      for (int b = 0; b < 3; ++b)
+    for (int i = 0; i < 12; ++i) y[i] = hv ? src[48 + 8 * (i >> 2) + 4 * hh + (i & 3)] : z4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * b + i] = hv ? src[48 + 8 * b + 4 * hh + i] : z4;
+    for (int i = 0; i < 8; ++i) x[i] = hv ? src[i] : z4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mx = __vmaxu2(mx, __vmaxu2(mag(x[i]), mag(x[4 + i])));
-        mr = __vmaxu2(mr, mag(x[8 + i]));
-        *reinterpret_cast<uint4*>(s.q + swz(m, 4 * hh + i)) = f16(x[i]);
-        *reinterpret_cast<uint4*>(s.q + kQBlockBytes + swz(m, 4 * hh + i)) = f16(x[4 + i]);
-        *reinterpret_cast<uint4*>(s.q + 2 * kQBlockBytes + swz(m, 4 * hh + i)) = bf(x[8 + i]);
+    for (int i = 0; i < 12; ++i) {
+      uint8_t* at = s.q + (i >> 2) * kQBlockBytes + swz(m, 4 * hh + (i & 3));
+      if (i < 8) {
+        mx = __vmaxu2(mx, mag(y[i]));
+        *reinterpret_cast<uint4*>(at) = make_uint4(f16(y[i].x), f16(y[i].y), f16(y[i].z), f16(y[i].w));
+      } else {
+        mr = __vmaxu2(mr, mag(y[i]));
+        *reinterpret_cast<uint4*>(at) = make_uint4(bf(y[i].x), bf(y[i].y), bf(y[i].z), bf(y[i].w));
       }
     }
 #pragma unroll 1
-    for (int c0 = 0; c0 < 192; c0 += 64) {
-      uint4 x[16];
+    for (int c0 = 0; c0 < 192; c0 += 32) {
+      uint32_t o[32];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = hv ? src[c0 / 4 + i] : z4;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t o[32];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          mx = __vmaxu2(mx, mag(x[8 * g + i]));
-          const uint4 v = f16(x[8 * g + i]);
-          o[4 * i] = v.x;
-          o[4 * i + 1] = v.y;
-          o[4 * i + 2] = v.z;
-          o[4 * i + 3] = v.w;
-        }
-        tmem_st32(trow + kColQ + c0 + 32 * g, o);
+      for (int i = 0; i < 8; ++i) {
+        mx = __vmaxu2(mx, mag(x[i]));
+        o[4 * i] = f16(x[i].x);
+        o[4 * i + 1] = f16(x[i].y);
+        o[4 * i + 2] = f16(x[i].z);
+        o[4 * i + 3] = f16(x[i].w);
+        if (c0 < 160) x[i] = hv ? src[c0 / 4 + 8 + i] : z4;  // the next turn's
       }
+      tmem_st32(trow + kColQ + c0, o);
     }
     tmem_wait_st();
-    mx = max(mx & 0xFFFFu, mx >> 16);
-    mr = max(mr & 0xFFFFu, mr >> 16);
-  };
-  // As it is where the head's largest latent magnitude lies in [2^-2, 2^15] (an
-  // fp16 subnormal's error is below 2^-23 of it then).  Else times 2^k, which
-  // brings that magnitude to [2^8, 2^9), but the rope's at most to 2^101, where
-  // its products are still finite (1 for rows of zeros, inf or NaN).  Exponents
-  // of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.
-  uint32_t mx, mr;
-  convert(0, mx, mr);
-  s.qmax[0][L] = mx;
-  s.qmax[1][L] = mr;
-  if (!meet(s, L & 31)) return false;
-  mx = max(mx, s.qmax[0][L ^ 64]);
-  mr = max(mr, s.qmax[1][L ^ 64]);
-  int k = 0;
-  if (mx != 0 && mx < 0x7F80u && (mx < 0x3E80u || mx > 0x4700u))
-    k = min(126, min(8 - ((int)(mx >> 7) - 127), 100 - ((int)(mr >> 7) - 127)));
-  if (__any_sync(0xFFFFFFFFu, k != 0)) convert(k, mx, mr);
+    if (pass == 1) break;
+    s.qmax[0][L] = max(mx & 0xFFFFu, mx >> 16);
+    s.qmax[1][L] = max(mr & 0xFFFFu, mr >> 16);
+    if (!meet(s, L & 31)) return false;
+    const int bm = (int)max(s.qmax[0][L], s.qmax[0][L ^ 64]), br = (int)max(s.qmax[1][L], s.qmax[1][L ^ 64]);
+    if (bm != 0 && bm < 0x7F80 && (bm < 0x3E80 || bm > 0x4700))
+      k = min(126, min(8 - ((bm >> 7) - 127), 100 - ((br >> 7) - 127)));
+    if (!__any_sync(0xFFFFFFFFu, k != 0)) break;
+  }
   // (the piece two before this one, whose place it takes, is past its last S)
   if (L == 0) s.piece_tiles[piece & 1] = w.here();
   fence_proxy_async_smem();
@@ -672,19 +657,24 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
       tmem_wait_ld();
       const int d = 256 * (c0 >> 7) + 128 * hh + (c0 & 127);
       if (hv && whole) {
-        uint4* dst = reinterpret_cast<uint4*>(a.out + t * a.out_st + hg * a.out_sh + d);
+        uint16_t* dst = a.out + t * a.out_st + hg * a.out_sh + d;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t v[4];
+        for (int e = 0; e < 2; ++e) {
+          uint32_t v[8];
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            v[x] = pack_bf16x2(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
-          dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
+          for (int x = 0; x < 8; ++x)
+            v[x] = pack_bf16x2(__uint_as_float(o[16 * e + 2 * x]) * inv, __uint_as_float(o[16 * e + 2 * x + 1]) * inv);
+          reinterpret_cast<uint4*>(dst)[2 * e] = make_uint4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<uint4*>(dst)[2 * e + 1] = make_uint4(v[4], v[5], v[6], v[7]);
         }
       } else if (hv) {
-        uint4* dst = reinterpret_cast<uint4*>(a.ws_o + prow * kNope + d);
+        float* dst = a.ws_o + prow * kNope + d;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        for (int e = 0; e < 4; ++e)  // 32-byte stores: whole sectors of the thread's own row
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + 8 * e), "r"(o[8 * e]),
+                       "r"(o[8 * e + 1]), "r"(o[8 * e + 2]), "r"(o[8 * e + 3]), "r"(o[8 * e + 4]), "r"(o[8 * e + 5]),
+                       "r"(o[8 * e + 6]), "r"(o[8 * e + 7])
+                       : "memory");
       }
     }
     tc_fence_before();

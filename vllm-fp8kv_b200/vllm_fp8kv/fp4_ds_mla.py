@@ -165,7 +165,7 @@ def _prepare(q, kv_cache, groups, topk, return_lse, workspace, *others):
     need = N.lib().fp8mla_fp4_workspace_bytes(T, H, groups, topk)
     if workspace is not None:
         assert workspace.is_contiguous(), "workspace must be contiguous"
-        if workspace.numel() * workspace.element_size() < need:
+        if workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 32:
             workspace = None
     if workspace is None and need:
         workspace = q.new_empty((need,), dtype=torch.uint8)
@@ -205,7 +205,8 @@ def fp4_ds_mla_sparse_decode(
     As ``fp8_ds_mla_sparse_decode``: entries < 0 or outside the pool are masked;
     returns ``out`` [T, H, 512] bf16, plus the natural-log ``lse`` [T, H] fp32
     when ``return_lse`` (-inf, and a zero row, where nothing is attended).
-    ``workspace``: a uint8 tensor of ``fp4_workspace_bytes`` to use."""
+    ``workspace``: a uint8 tensor of ``fp4_workspace_bytes``, 32-byte aligned, to
+    use (one that does not fit is replaced)."""
     indices = _with_groups(indices)
     G, topk = indices.shape[1], indices.shape[2]
     assert indices.shape[0] == q.shape[0], "one index row per query token"
