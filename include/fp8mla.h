@@ -393,8 +393,8 @@ FP8MLA_API int fp8mla_fp4_gather(const uint8_t* kv, int64_t num_slots, const int
  * also the most any topk needs. */
 FP8MLA_API int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t topk);
 
-/* Name of the attention kernel for H heads in G kv groups (introspection). */
-FP8MLA_API const char* fp8mla_fp4_kernel_name(int64_t H, int64_t G);
+/* Name of the attention kernel that a call takes (introspection); topk as above. */
+FP8MLA_API const char* fp8mla_fp4_kernel_name(int64_t T, int64_t H, int64_t G, int64_t topk);
 
 /*
  * Sparse MLA attention over fp4_ds_mla rows named by flat slots: arguments and

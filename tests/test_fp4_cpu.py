@@ -122,7 +122,12 @@ def test_workspace_and_names():
     assert F.fp4_workspace_bytes(3, 16, 1, 64) == 0            # whole rows: nothing to join
     for T, topk in ((1, 2048), (5, 100), (300, 777)):
         assert F.fp4_workspace_bytes(T, 16, 1, topk) <= F.fp4_workspace_bytes(T, 16)
-    assert F.fp4_kernel_name(16).startswith("decode_fp4")
+    # the kernel of many heads: from 33 heads a group, and enough work to fill its tiles
+    one, pair = "decode_fp4_kernel", "decode_fp4_tc_kernel"
+    assert F.fp4_kernel_name(16) == F.fp4_kernel_name(32) == F.fp4_kernel_name(128, 4, 64, 2048) == one
+    assert F.fp4_kernel_name(33) == F.fp4_kernel_name(128) == pair
+    assert F.fp4_kernel_name(128, 1, 1, 2048) == one and F.fp4_kernel_name(128, 1, 64, 2048) == pair
+    assert F.fp4_kernel_name(64, 1, 4, 2048) == one and F.fp4_kernel_name(40, 1, 64, 2048) == pair
 
 
 def test_header_constants_match_python_module():

@@ -11,6 +11,7 @@ from vllm_fp8kv.cache_writer import concat_and_cache_mla
 pytestmark = pytest.mark.gpu
 
 SCALE = 192 ** -0.5
+MANY = "decode_fp4_tc_kernel"
 
 
 def randn(seed, *shape):
@@ -203,13 +204,30 @@ def sparse_case(seed, T, H, topk, slots, G=1, mask=0.0):
     return randn(seed + 2, T, H, 576), idx
 
 
+def check_sparse(q, pool, idx, want, scale=SCALE):
+    """The call by itself and, where that does not take the kernel of many heads,
+    its rows repeated until it does."""
+    (T, H), (G, topk) = q.shape[:2], idx.shape[1:]
+    R.check(F.fp4_ds_mla_sparse_decode(q, pool, idx, scale, return_lse=True), want)
+    if F.fp4_kernel_name(H, G, T, topk) == MANY:
+        return
+    for reps in (16, 64, 256):
+        if F.fp4_kernel_name(H, G, T * reps, topk) == MANY:
+            out, lse = F.fp4_ds_mla_sparse_decode(q.repeat(reps, 1, 1), pool, idx.repeat(reps, 1, 1), scale,
+                                                  return_lse=True)
+            for i in range(0, reps, 5):
+                R.check((out[i * T:i * T + T], lse[i * T:i * T + T]), want)
+            return
+
+
 @pytest.mark.parametrize("H", [1, 3, 8, 16, 17, 24, 32, 40, 64, 65, 96, 128, 130, 256])
 @pytest.mark.parametrize("topk", [1, 63, 64, 65, 500])
 def test_sparse_heads_and_lengths(H, topk):
     pool = make_pool(30, 900)
     q, idx = sparse_case(31 + topk, 3, H, topk, 900, mask=0.2)
-    got = F.fp4_ds_mla_sparse_decode(q, pool, idx[:, 0], SCALE, return_lse=True)
-    R.check(got, R.attend(q, pool, idx, SCALE))
+    want = R.attend(q, pool, idx, SCALE)
+    R.check(F.fp4_ds_mla_sparse_decode(q, pool, idx[:, 0], SCALE, return_lse=True), want)
+    check_sparse(q, pool, idx, want)
     status_clean()
 
 
@@ -228,8 +246,7 @@ def test_sparse_division_of_work(H, T, topk):
 def test_sparse_groups(H, G):
     pool = make_pool(34, 400)
     q, idx = sparse_case(35, 4, H, 150, 400, G=G, mask=0.3)
-    got = F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True)
-    R.check(got, R.attend(q, pool, idx, SCALE, G))
+    check_sparse(q, pool, idx, R.attend(q, pool, idx, SCALE, G))
 
 
 @pytest.mark.parametrize("H", [16, 128])
@@ -249,8 +266,7 @@ def test_sparse_masks(H):
     idx[5, :, :256] = -(2 ** 31)
     idx[6, :, 3::4] = -1
     idx = torch.where(idx == 300, 100000, idx)
-    got = F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True)
-    R.check(got, R.attend(q, pool, idx, SCALE))
+    check_sparse(q, pool, idx, R.attend(q, pool, idx, SCALE))
 
 
 @pytest.mark.parametrize("H", [16, 128])
@@ -281,16 +297,29 @@ def test_scores_of_any_size(H):
     ramp = torch.linspace(0.05, 4.0, 2000, device="cuda")[:, None]
     pool = R.quantize((randn(42, 2000, 512).float() * ramp).to(torch.bfloat16), randn(43, 2000, 64))
     idx = torch.arange(2000, dtype=torch.int32, device="cuda").expand(2, 1, 2000)
-    got = F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True)
-    R.check(got, R.attend(q, pool, idx, SCALE))
+    check_sparse(q, pool, idx, R.attend(q, pool, idx, SCALE))
     size = 10.0 ** torch.linspace(-30, 30, H, device="cuda")
     q2 = (q.float() * size[:, None]).to(torch.bfloat16)
     # heads one at a time, each with the scale that makes its scores ordinary
+    if H > 32:  # enough rows for the kernel of many heads
+        q2, idx = q2.repeat(8, 1, 1), idx.repeat(8, 1, 1)
+        assert F.fp4_kernel_name(H, 1, 16, 2000) == MANY
     for h in range(0, H, max(1, H // 8)):
         sc = SCALE / float(size[h])
         got = F.fp4_ds_mla_sparse_decode(q2, pool, idx, sc, return_lse=True)
         want = R.attend(q2[:, h:h + 1], pool, idx, sc)
         R.check((got[0][:, h:h + 1], got[1][:, h:h + 1]), want)
+
+
+@pytest.mark.parametrize("H", [16, 128])
+@pytest.mark.parametrize("scale", [-0.07, 0.0, -0.0])
+def test_softmax_scale_of_any_sign(H, scale):
+    """A negative scale turns the order of the scores round; with 0 all live
+    entries weigh the same.  Masked entries stay out either way."""
+    pool = make_pool(46, 500)
+    q, idx = sparse_case(47, 3, H, 321, 500, mask=0.3)
+    idx[1] = -1
+    check_sparse(q, pool, idx, R.attend(q, pool, idx, scale), scale)
 
 
 @pytest.mark.parametrize("H", [16, 128])
@@ -302,7 +331,14 @@ def test_nan_in_an_attended_row_shows(H):
     idx[1, 17] = 150
     out, lse = F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True)
     assert out[0].isnan().all() and lse[0].isnan().all()
-    R.check((out[1:], lse[1:]), R.attend(q[1:], pool, idx[1:, None], SCALE))
+    want = R.attend(q[1:], pool, idx[1:, None], SCALE)
+    R.check((out[1:], lse[1:]), want)
+    if H > 32:
+        assert F.fp4_kernel_name(H, 1, 128, 100) == MANY
+        out, lse = F.fp4_ds_mla_sparse_decode(q.repeat(64, 1, 1), pool, idx.repeat(64, 1), SCALE, return_lse=True)
+        assert out[::2].isnan().all() and lse[::2].isnan().all()
+        R.check((out[1:2], lse[1:2]), want)
+        R.check((out[127:], lse[127:]), want)
 
 
 def paged_slots(table, req, tok, page, max_blocks):
@@ -321,8 +357,13 @@ def test_paged(H, page):
     req = torch.tensor([3, 0, 0, 2, 1], dtype=torch.int32, device="cuda")
     q = randn(52, 5, H, 576)
     tok = (ints(53, 430, (5, 1, 170)) - 5).to(torch.int32)  # some negative, some behind the table
-    got = F.fp4_ds_mla_sparse_decode_paged(q, pool, req, table, tok, SCALE, block_size=page, return_lse=True)
-    R.check(got, R.attend(q, pool, paged_slots(table, req, tok, page, blocks), SCALE))
+    want = R.attend(q, pool, paged_slots(table, req, tok, page, blocks), SCALE)
+    for reps in (1, 24) if H > 32 else (1,):
+        out, lse = F.fp4_ds_mla_sparse_decode_paged(q.repeat(reps, 1, 1), pool, req.repeat(reps), table,
+                                                    tok.repeat(reps, 1, 1), SCALE, block_size=page, return_lse=True)
+        for i in range(0, reps, 6):
+            R.check((out[5 * i:5 * i + 5], lse[5 * i:5 * i + 5]), want)
+    assert H <= 32 or F.fp4_kernel_name(H, 1, 5 * 24, 170) == MANY
 
 
 def dense_slots(table, req, lens, page):
@@ -384,8 +425,7 @@ def test_offsets_past_32_bits(H):
     pool[-2000:] = tail
     q = randn(68, 2, H, 576)
     idx = (slots - 1 - ints(69, 2000, (2, 1, 300))).to(torch.int32)
-    got = F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True)
-    R.check(got, R.attend(q, tail, idx.long() - (slots - 2000), SCALE))
+    check_sparse(q, pool, idx, R.attend(q, tail, idx.long() - (slots - 2000), SCALE))
     back = F.dequant_fp4_ds_mla_rows(pool, idx[0, 0])
     assert torch.equal(back.double(), R.values(pool[idx[0, 0].long()]))
     kv_c, k_pe = randn(70, 3, 512), randn(71, 3, 64)
@@ -393,12 +433,12 @@ def test_offsets_past_32_bits(H):
     assert torch.equal(pool[[slots - 1, 5_200_000, slots - 7]], R.quantize(kv_c, k_pe))
 
 
-@pytest.mark.parametrize("H", [16, 128])
-def test_q_layouts_and_workspace(H):
+@pytest.mark.parametrize("H,T", [(16, 4), (128, 4), (128, 80)])
+def test_q_layouts_and_workspace(H, T):
     pool = make_pool(72, 500)
-    q, idx = sparse_case(73, 4, H, 200, 500)
+    q, idx = sparse_case(73, T, H, 200, 500)
     want = F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True)
-    ws = torch.full((F.fp4_workspace_bytes(4, H) + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+    ws = torch.full((F.fp4_workspace_bytes(T, H) + 64,), 0xFF, dtype=torch.uint8, device="cuda")
     views = [q.transpose(0, 1).contiguous().transpose(0, 1),                       # head-major
              torch.cat([q, q], 2)[:, :, :576],                                     # padded rows
              torch.cat([q[..., :3], q], 2)[:, :, 3:]]                              # misaligned rows

@@ -11,9 +11,6 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 constexpr int64_t kMaxTopk = 1LL << 30, kMaxT = 1LL << 24, kMaxH = 1 << 16;
 
-// Heads per kv group from which the paired kernel is used.
-constexpr int64_t kTcHeads = 49;
-
 // How a call's units are dealt out (decode_fp4.h).
 struct Plan {
   int rows, workers, hb_per_group, chunk, min_per;
@@ -22,10 +19,10 @@ struct Plan {
   bool tc;      // the paired tensor-core kernel
 };
 // topk < 0: whole contexts, of at most max_len positions
-Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
+Plan plan_with(bool tc, int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
   Plan p;
   const int64_t hpg = H / G;
-  p.tc = hpg >= kTcHeads;
+  p.tc = tc;
   p.rows = p.tc ? kFp4TcRows : 16;
   p.workers = p.tc ? device_sm_count() / 2 : device_sm_count();
   p.hb_per_group = (int)((hpg + p.rows - 1) / p.rows);
@@ -51,6 +48,23 @@ Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
   if (!p.cuts) p.per = whole;
   p.workers = (int)((total + p.per - 1) / p.per);
   return p;
+}
+// Which kernel.  Up to 32 heads per group the paired one wastes three quarters of
+// its tile: not at any size.  Above, a run of n tiles costs it about 3 n us, a run of
+// n chunks costs the other 1.45 n, and the paired one takes 9 us more to get
+// going and to end.  Measured, us, the other one / the paired one, top-2048:
+//   heads     33-48          49-64          128            256
+//   T = 1     19.2 / 20.0    19.9 / 21.0    20.8 / 21.5    18.5 / 23.1
+//   T = 4     21.5 / 22.9    18.4 / 23.9    26.2 / 27.4    35.1 / 32.4
+//   T = 16    31.1 / 32.5    34.9 / 33.5    45.5 / 35.7    87.5 / 63.7
+//   T = 64    72.6 / 59.6    88.1 / 60.6     173 / 61.6     299 / 124
+// (17 to 32 heads at T = 64: 45.6 / 58.5).  Lengths that only the device knows are
+// taken for long ones.
+Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
+  const Plan one = plan_with(false, T, H, G, topk, max_len);
+  if (H / G <= 32) return one;
+  const Plan pair = plan_with(true, T, H, G, topk, max_len);
+  return topk < 0 || one.per >= 2 * pair.per + 6 ? pair : one;
 }
 int64_t info_bytes(const Plan& p) { return (int64_t)p.workers * 4 * 8; }
 int64_t part_bytes(const Plan& p) { return (int64_t)2 * p.workers * p.rows * FP8MLA_NOPE * 4; }
@@ -203,9 +217,9 @@ int64_t fp8mla_fp4_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t topk
   return workspace_of(plan_of(T, H, G, topk, INT32_MAX));
 }
 
-const char* fp8mla_fp4_kernel_name(int64_t H, int64_t G) {
-  if (H <= 0 || G <= 0 || H % G != 0) return "";
-  return H / G >= kTcHeads ? "decode_fp4_tc_kernel" : "decode_fp4_kernel";
+const char* fp8mla_fp4_kernel_name(int64_t T, int64_t H, int64_t G, int64_t topk) {
+  if (T <= 0 || T > kMaxT || H <= 0 || H > kMaxH || G <= 0 || H % G != 0 || topk < -1 || topk > kMaxTopk) return "";
+  return plan_of(T, H, G, topk, INT32_MAX).tc ? "decode_fp4_tc_kernel" : "decode_fp4_kernel";
 }
 
 int fp8mla_fp4_sparse_decode(const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t, int64_t q_stride_h,

@@ -67,7 +67,7 @@ struct SmemLimit {
 // One worker per SM, 16 heads per unit (decode_fp4.cu).  `cuts`: some unit may
 // be cut, so the merge follows.
 int launch_decode_fp4(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st);
-// One worker per SM pair, 128 heads per unit (decode_fp4_tc.cu).
+// One worker per SM pair, up to 128 heads per unit (decode_fp4_tc.cu).
 int launch_decode_fp4_tc(const Fp4DecodeArgs& a, bool cuts, cudaStream_t st);
 int read_device_status_fp4_tc(unsigned int* status, bool reset, cudaStream_t st);
 constexpr int kFp4TcRows = 128;

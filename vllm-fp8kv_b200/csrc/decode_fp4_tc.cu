@@ -11,14 +11,19 @@
 //   O    M=128 heads, N=256 dims (two MMAs for the 512), K=128 entries; CTA c
 //        supplies dims [128c, +128) of each MMA (latent tiles c and c + 2, its
 //        "half") of all 128 entries
-// An M=128 pair MMA costs about 45 cycles up to N=128 and 64 at N=256 (measured),
-// so the issuing thread's stream, not the arithmetic, is what bounds such a
-// kernel: 128-entry tiles need 52 MMAs per 128 entries, 64-entry tiles 88.  What
-// makes room for them in shared memory (K own rows 72 KB, V halves 64 KB, both
-// in fp16 and single) is the 4-bit rows, whose ring takes 39 KB, and letting each
-// buffer drain in parts: K in two groups of blocks, refilled for the next tile
-// while the other group and the O product of the tile before are still running; V while the
-// next tile's S runs.
+// A tile's 52 MMAs take 2200 cycles; 64-entry tiles would need 88 MMAs for the same
+// entries.  K (own rows, 72 KB) and V (halves, 64 KB) are single in shared memory,
+// in fp16; the 4-bit rows never lie there, they go from memory to registers a tile
+// ahead.  Each buffer drains in parts: K in two groups of blocks, refilled for the
+// next tile while the other group and the O product of the tile before are still
+// running; V while the next tile's S runs.
+//
+// Measured, us: 64 x 128 heads x top-2048, paged: 64.3 (16 tiles a pair); its
+// products take 22.5 at the rate of a large matrix product, its rows' bytes 8.3.  A tile takes 3.1 us, of which the
+// chain S -> softmax -> P -> O is the longest part: S and O of one tile cannot
+// overlap (one S, one P: tensor memory is full).  12 us go by before the first S
+// (cold code, and a chain of three memory latencies: entries, block table, rows)
+// and 5 behind the last P.  One context of 131072 x 128 heads: 72.5.
 //
 // The latents are exact in fp16 (fp4.cuh), so the 32 latent k-steps of S and the
 // O product are fp16 MMAs: q is scaled per head by a power of two to a largest
@@ -39,17 +44,17 @@
 //   [256,320)  S
 //   [320,512)  q dims [0,384), the A operand of 24 k-steps (lanes L and L^64
 //              hold the same head)
-// Shared memory (about 218 KB):
+// Shared memory (217 KB):
 //   q    dims [384,512) fp16, rope bf16: 3 x 64-dim swizzled blocks of 64 rows  24 KB
 //   k    own 64 entries x 576 dims, 9 blocks of 64 rows                         72 KB
 //   v    128 entries x this CTA's half, 4 blocks of 128 rows                    64 KB
 //   p    P of 64 heads x 128 entries, 2 blocks                                  16 KB
-//   raw  a ring of 3 units of 8 own rows per K warp, as copied by TMA            39 KB
+//   stage  half of q's latents on their way in                                  33 KB
 //
 // Warp roles (512 threads per CTA; warp w runs on SM sub-partition w % 4):
 //   warps 0-3         softmax, q, and the stores of O
-//   warp 4            tensor memory allocation; lane 0 of the even CTA issues
-//                     every MMA of the pair
+//   warp 4            tensor memory allocation; the even CTA's issues every MMA of
+//                     the pair
 //   warps 5, 6, 7, 9  K: own rows [16i, +16) of every tile, loaded into registers
 //                     a tile ahead -> K blocks
 //   warps 10, 11, 13, 14
@@ -101,9 +106,11 @@ struct Smem {
   uint8_t k[9 * kKBlockBytes];
   uint8_t v[4 * kVBlockBytes];
   uint8_t p[2 * kPBlockBytes];
+  uint8_t stage[64][528];       // half a latent of every head (rows 4 banks apart)
   float half_max[2][128];       // a tile's maxima per thread, by tile parity
   float lsum[128];
-  uint32_t qmax[2][128];        // largest magnitudes of q's halves: latents, rope
+  uint32_t qmax[128];           // largest latent magnitudes per thread
+  int qk[64], qagain[2];        // powers of two of the heads; any not 0 among 32
   int32_t slot[kScoutRing][kN];   // a tile's slots, and its live bits
   uint32_t vmask[kScoutRing][4];
   int piece_tiles[2];           // tiles of a piece, by its parity (softmax -> MMA)
@@ -117,7 +124,7 @@ struct Smem {
 };
 static_assert(offsetof(Smem, k) % 1024 == 0 && offsetof(Smem, v) % 1024 == 0 && offsetof(Smem, p) % 1024 == 0,
               "swizzle atoms need 1024-B alignment");
-static_assert(offsetof(Smem, kfull) % 8 == 0, "");
+static_assert(offsetof(Smem, kfull) % 8 == 0 && offsetof(Smem, stage) % 16 == 0, "");
 static_assert(sizeof(Smem) + 1024 <= 227 * 1024, "shared memory budget");
 
 __device__ __forceinline__ uint32_t swz(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
@@ -437,79 +444,110 @@ struct Meet {
 // L & 63), the rest -> swizzled shared memory (thread hh writes chunks [4 hh, +4)
 // of each block); padding rows are zero.  `scale` turns the head's accumulators
 // into scores in log2 units.
+// A thread needs its head's whole row, and 32 rows read 16 bytes at a time are 32
+// lines an instruction; so a warp reads 512 bytes of one row an instruction, and
+// the rows change hands in shared memory: 102 us
+// instead of 104.7 at 32 x 128 heads over contexts of up to 8192.
 __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, Meet& meet, float& scale) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
-  const int m = L & 63, hh = L >> 6;
-  const int head = w.hb * a.rows + 64 * (int)c.rank + m;  // of its group
-  const bool hv = 64 * (int)c.rank + m < a.rows && head < a.hpg;
-  const uint4* src = reinterpret_cast<const uint4*>(a.q + w.t * a.q_st +
-                                                    (int64_t)(w.grp * a.hpg + (hv ? head : 0)) * a.q_sh);
+  const int m = L & 63, hh = L >> 6, lane = L & 31, warp = L >> 5;
+  const int head0 = w.hb * a.rows + 64 * (int)c.rank;  // of its group
+  const int nh = max(0, min(64, min(a.rows - 64 * (int)c.rank, a.hpg - head0)));
+  const uint16_t* q0 = a.q + w.t * a.q_st + (int64_t)(w.grp * a.hpg + (nh > 0 ? head0 : 0)) * a.q_sh;
   const uint4 z4 = make_uint4(0, 0, 0, 0);
   auto mag = [](const uint4& v) {
     return __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
   };
-  const uint32_t trow = c.tmem + ((uint32_t)((L >> 5) * 32) << 16);
+  const uint32_t trow = c.tmem + ((uint32_t)(warp * 32) << 16);
   // First as it is, which is exact enough where the head's largest latent magnitude
   // lies in [2^-2, 2^15] (an fp16 subnormal's error is below 2^-23 of it then).
   // Else again times 2^k, which brings that magnitude to [2^8, 2^9), but the rope's at
   // most to 2^101, where its products are still finite (1 for rows of zeros, inf
-  // or NaN).  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.  (Short
-  // loops: the code runs once a unit and comes from memory each time.)
+  // or NaN).  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.
   int k = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     // the sign of the softmax scale goes with q, so that scores scale by a positive factor
     const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), a.scale_log2);
-    auto f16 = [&](uint32_t u) { return pack_f16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
-    auto bf = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
-    uint32_t mx = 0, mr = 0;
-    uint4 x[8], y[12];
-#pragma unroll
-    for (int i = 0; i < 12; ++i) y[i] = hv ? src[48 + 8 * (i >> 2) + 4 * hh + (i & 3)] : z4;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = hv ? src[i] : z4;
-#pragma unroll
-    for (int i = 0; i < 12; ++i) {
-      uint8_t* at = s.q + (i >> 2) * kQBlockBytes + swz(m, 4 * hh + (i & 3));
-      if (i < 8) {
-        mx = __vmaxu2(mx, mag(y[i]));
-        *reinterpret_cast<uint4*>(at) = make_uint4(f16(y[i].x), f16(y[i].y), f16(y[i].z), f16(y[i].w));
-      } else {
-        mr = __vmaxu2(mr, mag(y[i]));
-        *reinterpret_cast<uint4*>(at) = make_uint4(bf(y[i].x), bf(y[i].y), bf(y[i].z), bf(y[i].w));
-      }
-    }
+    auto f16 = [&](const uint4& v) {
+      auto one = [&](uint32_t u) { return pack_f16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
+      return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+    };
+    uint32_t mx = 0;
 #pragma unroll 1
-    for (int c0 = 0; c0 < 192; c0 += 32) {
-      uint32_t o[32];
+    for (int half = 0; half < 2; ++half) {  // latent dims [256 half, +256)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        mx = __vmaxu2(mx, mag(x[i]));
-        o[4 * i] = f16(x[i].x);
-        o[4 * i + 1] = f16(x[i].y);
-        o[4 * i + 2] = f16(x[i].z);
-        o[4 * i + 3] = f16(x[i].w);
-        if (c0 < 160) x[i] = hv ? src[c0 / 4 + 8 + i] : z4;  // the next turn's
+      for (int g = 0; g < 2; ++g) {
+        uint4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 16 * warp + 8 * g + i;
+          x[i] = r < nh ? reinterpret_cast<const uint4*>(q0 + r * a.q_sh + 256 * half)[lane] : z4;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(s.stage[16 * warp + 8 * g + i] + 16 * lane) = x[i];
       }
-      tmem_st32(trow + kColQ + c0, o);
+      if (!meet(s, lane)) return false;
+      const uint4* row = reinterpret_cast<const uint4*>(s.stage[m]);
+#pragma unroll 1
+      for (int c0 = 0; c0 < (half == 0 ? 128 : 64); c0 += 32) {  // to tensor memory
+        uint32_t o[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 x = row[c0 / 4 + i];
+          mx = __vmaxu2(mx, mag(x));
+          const uint4 v = f16(x);
+          o[4 * i] = v.x;
+          o[4 * i + 1] = v.y;
+          o[4 * i + 2] = v.z;
+          o[4 * i + 3] = v.w;
+        }
+        tmem_st32(trow + kColQ + 128 * half + c0, o);
+      }
+      if (half == 1) {  // dims [384,512) to shared memory
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 x = row[16 + 8 * (i >> 2) + 4 * hh + (i & 3)];
+          mx = __vmaxu2(mx, mag(x));
+          *reinterpret_cast<uint4*>(s.q + (i >> 2) * kQBlockBytes + swz(m, 4 * hh + (i & 3))) = f16(x);
+        }
+      }
+      s.qmax[L] = max(mx & 0xFFFFu, mx >> 16);
+      if (!meet(s, lane)) return false;  // the stage has been read (and the maxima are in place)
+    }
+    // the rope, four rows an instruction
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * warp + 4 * i + (lane >> 3);
+      const uint4 x = r < nh ? reinterpret_cast<const uint4*>(q0 + r * a.q_sh + kNope)[lane & 7] : z4;
+      const float ur = pass == 0 ? up : copysignf(__uint_as_float((uint32_t)(127 + s.qk[r]) << 23), a.scale_log2);
+      auto one = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * ur, bf16_hi(u) * ur); };
+      *reinterpret_cast<uint4*>(s.q + 2 * kQBlockBytes + swz(r, lane & 7)) = make_uint4(one(x.x), one(x.y), one(x.z), one(x.w));
     }
     tmem_wait_st();
     if (pass == 1) break;
-    s.qmax[0][L] = max(mx & 0xFFFFu, mx >> 16);
-    s.qmax[1][L] = max(mr & 0xFFFFu, mr >> 16);
-    if (!meet(s, L & 31)) return false;
-    const int bm = (int)max(s.qmax[0][L], s.qmax[0][L ^ 64]), br = (int)max(s.qmax[1][L], s.qmax[1][L ^ 64]);
-    if (bm != 0 && bm < 0x7F80 && (bm < 0x3E80 || bm > 0x4700))
+    const int bm = (int)max(s.qmax[L], s.qmax[L ^ 64]);
+    const bool again = bm != 0 && bm < 0x7F80 && (bm < 0x3E80 || bm > 0x4700);
+    if (again) {
+      uint32_t mr = 0;
+      for (int i = 0; i < 8; ++i) mr = __vmaxu2(mr, mag(reinterpret_cast<const uint4*>(q0 + m * a.q_sh + kNope)[i]));
+      const int br = (int)max(mr & 0xFFFFu, mr >> 16);
       k = min(126, min(8 - ((bm >> 7) - 127), 100 - ((br >> 7) - 127)));
-    if (!__any_sync(0xFFFFFFFFu, k != 0)) break;
+    }
+    if (hh == 0) s.qk[m] = k;
+    const bool any = __any_sync(0xFFFFFFFFu, again);
+    if (hh == 0 && lane == 0) s.qagain[warp] = any ? 1 : 0;
+    if (!meet(s, lane)) return false;
+    if (s.qagain[0] == 0 && s.qagain[1] == 0) break;
   }
   // (the piece two before this one, whose place it takes, is past its last S)
   if (L == 0) s.piece_tiles[piece & 1] = w.here();
   fence_proxy_async_smem();
   tc_fence_before();
   __syncwarp();
-  if ((L & 31) == 0) mbar_arrive_cluster(bar(s.qready), 0);
+  if (lane == 0) mbar_arrive_cluster(bar(s.qready), 0);
   scale = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k) << 23);
   if (scale == 0.f) scale = 1.1754944e-38f;  // a masked score is an infinity times the scale
   return true;
@@ -735,7 +773,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // one call per role: the loops of all roles together have to stay in the SM's
   // instruction cache (with each role inlined twice, and the unpacking and the
   // softmax unrolled in full, warps waited for instructions most of the time:
-  // 182 instead of TODO us at 64 x 128 heads x top-2048)
+  // 182 instead of 112 us, then, at 64 x 128 heads x top-2048)
   if (warp < kSoftmaxWarps) {
     softmax_role(c, warp, lane);
   } else if (warp == kMmaWarp) {

@@ -70,7 +70,7 @@ SIGNATURES = {
     "fp8mla_fp4_gather": (_I32, [_P, _I64, _P, _I64, _I64, _I64,  # kv, num_slots, block table, block_size
                                  _P, _I64, _P, _I64, _P, _I64, _P]),
     "fp8mla_fp4_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
-    "fp8mla_fp4_kernel_name": (ctypes.c_char_p, [_I64, _I64]),
+    "fp8mla_fp4_kernel_name": (ctypes.c_char_p, [_I64, _I64, _I64, _I64]),
     "fp8mla_fp4_sparse_decode": (_I32, [
         _P, _I64, _I64, _I64, _I64,            # q, T, H, q strides
         _P, _I64,                              # kv, num_slots

@@ -140,9 +140,10 @@ def fp4_workspace_bytes(T: int, H: int, G: int = 1, topk: int = -1) -> int:
     return int(N.lib().fp8mla_fp4_workspace_bytes(T, H, G, topk))
 
 
-def fp4_kernel_name(H: int, G: int = 1) -> str:
-    """The attention kernel for H query heads in G kv groups (introspection)."""
-    return N.lib().fp8mla_fp4_kernel_name(H, G).decode()
+def fp4_kernel_name(H: int, G: int = 1, T: int = 1, topk: int = -1) -> str:
+    """The attention kernel that a call with H query heads in G kv groups takes
+    (introspection); topk -1: whole contexts."""
+    return N.lib().fp8mla_fp4_kernel_name(T, H, G, topk).decode()
 
 
 def _prepare(q, kv_cache, groups, topk, return_lse, workspace, *others):
