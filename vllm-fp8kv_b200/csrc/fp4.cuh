@@ -47,10 +47,18 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// 2 exact fp16 products -> bf16x2 (exact: at most 6 significant bits)
-__device__ __forceinline__ uint32_t f16x2_to_bf16x2(uint32_t h) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  return pack_bf16x2(f.x, f.y);
+// Codes times scale in bf16, exact (at most 6 significant bits, and far from the
+// ends of the range).  An fp16 code (normal or zero) moved three bits to the right
+// under its sign is the bf16 code times 2^-112; the scale carries the 2^112.
+__device__ __forceinline__ uint32_t bf16_scale(uint32_t e4m3) {
+  const uint32_t h = e4m3x2_to_f16(e4m3);
+  const float s = __half2float(__ushort_as_half((unsigned short)(h & 0xFFFFu))) * 0x1p112f;
+  return pack_bf16x2(s, s);
+}
+__device__ __forceinline__ uint32_t scaled_bf16x2(uint32_t f16_codes, uint32_t scale) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(((f16_codes >> 3) & 0x0FFF0FFFu) | (f16_codes & 0x80008000u)), "r"(scale));
+  return r;
 }
 
 }  // namespace fp4

@@ -1,9 +1,11 @@
 // fp4_cache.cu -- the fp4_ds_mla cache around the attention: the writer, the
 // row read-back and the read-back of whole sequences.  All three move bytes:
-// 1152 in and 416 out per written token, 416 in and 1152 out per token read.
-// One warp owns one row and one lane one scale group (16 values: 8 code bytes,
-// one scale byte), so no value crosses a lane and every access of a warp is
-// one contiguous run.
+// 1152 in and 416 out per written token, 416 in and 1152 out per token read,
+// and run at 0.90 to 0.92 of a plain copy's rate (6.5 TB/s).  One warp owns one row
+// and one lane one scale group (16 values: 8 code bytes, one scale byte), so no
+// value crosses a lane and every access of a warp is one contiguous run.  What
+// held them at two thirds of that were instructions (conversions by way of fp32,
+// 64-bit divisions by every lane) and too few resident warps.
 #include "fp4.cuh"
 #include "decode.h"
 #include "decode_fp4.h"
@@ -39,13 +41,9 @@ __device__ __forceinline__ uint32_t f32x2_to_e2m1x2(float x0, float x1) {
   return r;
 }
 
-struct WriterIn {
-  int64_t slot;
-  uint32_t w[8];  // 16 bf16 latent values
-  uint4 rope;     // lanes 0..7: 8 bf16 rope values
-};
-__device__ __forceinline__ void load16(uint32_t (&w)[8], const uint16_t* src, bool vec) {
-  if (vec) {
+template <bool kVec>
+__device__ __forceinline__ void load16(uint32_t (&w)[8], const uint16_t* src) {
+  if (kVec) {
     const uint4 a = reinterpret_cast<const uint4*>(src)[0];
     const uint4 b = reinterpret_cast<const uint4*>(src)[1];
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
@@ -55,13 +53,18 @@ __device__ __forceinline__ void load16(uint32_t (&w)[8], const uint16_t* src, bo
     for (int j = 0; j < 8; ++j) w[j] = (uint32_t)src[2 * j] | ((uint32_t)src[2 * j + 1] << 16);
   }
 }
-__device__ __forceinline__ uint4 load8(const uint16_t* r, bool vec) {
-  if (vec) return *reinterpret_cast<const uint4*>(r);
+template <bool kVec>
+__device__ __forceinline__ uint4 load8(const uint16_t* r) {
+  if (kVec) return *reinterpret_cast<const uint4*>(r);
   return make_uint4((uint32_t)r[0] | ((uint32_t)r[1] << 16), (uint32_t)r[2] | ((uint32_t)r[3] << 16),
                     (uint32_t)r[4] | ((uint32_t)r[5] << 16), (uint32_t)r[6] | ((uint32_t)r[7] << 16));
 }
 
-__global__ void __launch_bounds__(kBlock) fp4_write_kernel(
+// kVec: rows of both inputs 16-byte aligned.  A row a warp with all of an SM's warps
+// resident: 17.3 us for 65536 rows, 6.0 TB/s (with the next row prefetched and half
+// the warps 19.0).
+template <bool kVec>
+__global__ void __launch_bounds__(kBlock, kVec ? 8 : 4) fp4_write_kernel(
     const uint16_t* __restrict__ kv_c, int64_t kv_c_stride, const uint16_t* __restrict__ k_pe,
     int64_t k_pe_stride, const int64_t* __restrict__ slot_mapping, int64_t N,
     uint8_t* __restrict__ cache, int64_t num_slots) {
@@ -69,24 +72,17 @@ __global__ void __launch_bounds__(kBlock) fp4_write_kernel(
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t warps_total = (int64_t)gridDim.x * kWarps;
-  const bool vec_c = (kv_c_stride % 8) == 0 && (reinterpret_cast<uintptr_t>(kv_c) & 15) == 0;
-  const bool vec_pe = (k_pe_stride % 8) == 0 && (reinterpret_cast<uintptr_t>(k_pe) & 15) == 0;
-  auto load = [&](WriterIn& in, int64_t tok) {
-    in.slot = slot_mapping[tok];
-    load16(in.w, kv_c + tok * kv_c_stride + lane * 16, vec_c);
-    in.rope = lane < 8 ? load8(k_pe + tok * k_pe_stride + lane * 8, vec_pe) : make_uint4(0, 0, 0, 0);
-  };
-  int64_t tok = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  WriterIn cur, nxt;
-  if (tok < N) load(cur, tok);
-  for (; tok < N; tok += warps_total) {
-    if (tok + warps_total < N) load(nxt, tok + warps_total);
-    const int64_t slot = cur.slot;
+  for (int64_t tok = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32; tok < N; tok += warps_total) {
+    const int64_t slot = slot_mapping[tok];
+    uint32_t in[8];  // 16 latent values
+    load16<kVec>(in, kv_c + tok * kv_c_stride + lane * 16);
+    uint4 rope = make_uint4(0, 0, 0, 0);
+    if (lane < 8) rope = load8<kVec>(k_pe + tok * k_pe_stride + lane * 8);
     if (slot >= 0 && slot < num_slots) {  // else a padding token
       // amax on the bf16 bits: magnitudes order as integers, NaN above inf
       uint32_t m2 = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m2 = __vmaxu2(m2, cur.w[j] & 0x7FFF7FFFu);
+      for (int j = 0; j < 8; ++j) m2 = __vmaxu2(m2, in[j] & 0x7FFF7FFFu);
       const uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
       const bool nan = m > 0x7F80u;
       const float want = fminf(fmaxf(__fdiv_rn(__uint_as_float(m << 16), 6.0f), 0.001953125f), 448.0f);
@@ -100,16 +96,15 @@ __global__ void __launch_bounds__(kBlock) fp4_write_kernel(
         q[h] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t w = cur.w[4 * h + j];
+          const uint32_t w = in[4 * h + j];
           q[h] |= f32x2_to_e2m1x2(snap12(bf16_lo(w) * inv), snap12(bf16_hi(w) * inv)) << (8 * j);
         }
       }
       uint8_t* row = cache + slot * (int64_t)kFp4RowBytes;
       reinterpret_cast<uint2*>(row)[lane] = make_uint2(q[0], q[1]);
       row[kFp4ScaleOff + lane] = nan ? (uint8_t)0x7F : (uint8_t)sb;
-      if (lane < 8) reinterpret_cast<uint4*>(row + kFp4RopeOff)[lane] = cur.rope;
+      if (lane < 8) reinterpret_cast<uint4*>(row + kFp4RopeOff)[lane] = rope;
     }
-    cur = nxt;
   }
 }
 
@@ -131,42 +126,46 @@ __device__ __forceinline__ void row_load(RowIn& in, const uint8_t* __restrict__ 
     in.rope = make_uint4(0, 0, 0, 0);
   }
 }
-__device__ __forceinline__ void row_store(const RowIn& in, uint16_t* __restrict__ dst, int lane) {
-  uint32_t s = e4m3x2_to_f16(in.scale * 0x0101u);
+// Rows that start at 32-byte sectors are stored a sector a lane.
+__device__ __forceinline__ bool whole_sectors(const uint16_t* out, int64_t out_stride) {
+  return out_stride % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0;
+}
+__device__ __forceinline__ void row_store(const RowIn& in, uint16_t* __restrict__ dst, int lane, bool sectors) {
+  const uint32_t s = bf16_scale(in.scale);
   uint32_t a[4], b[4];
   e2m1x8_to_f16(in.codes.x, a);
   e2m1x8_to_f16(in.codes.y, b);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    a[i] = f16x2_to_bf16x2(mul_f16x2(a[i], s));
-    b[i] = f16x2_to_bf16x2(mul_f16x2(b[i], s));
+    a[i] = scaled_bf16x2(a[i], s);
+    b[i] = scaled_bf16x2(b[i], s);
   }
-  uint4* o = reinterpret_cast<uint4*>(dst + 16 * lane);
-  o[0] = make_uint4(a[0], a[1], a[2], a[3]);
-  o[1] = make_uint4(b[0], b[1], b[2], b[3]);
+  uint16_t* o = dst + 16 * lane;
+  if (sectors) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(o), "r"(a[0]), "r"(a[1]),
+                 "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(o)[0] = make_uint4(a[0], a[1], a[2], a[3]);
+    reinterpret_cast<uint4*>(o)[1] = make_uint4(b[0], b[1], b[2], b[3]);
+  }
   if (lane < 8) reinterpret_cast<uint4*>(dst + kNope)[lane] = in.rope;
 }
 
-constexpr int kRowsPerStep = 4;  // rows of a warp in flight together
-
-__global__ void __launch_bounds__(kBlock) fp4_rows_kernel(const uint8_t* __restrict__ kv, int64_t num_slots,
+// A row a warp: 32 registers, so all of an SM's warps are resident, each with one
+// row in flight (17.3 us for 65536 rows; 20.8 with two rows a step, 22.1 with four).
+__global__ void __launch_bounds__(kBlock, 8) fp4_rows_kernel(const uint8_t* __restrict__ kv, int64_t num_slots,
                                                           const int64_t* __restrict__ slots, int64_t n,
                                                           uint16_t* __restrict__ out, int64_t out_stride) {
   if (threadIdx.x == 0) pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t step = (int64_t)gridDim.x * kWarps * kRowsPerStep;
-  for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + threadIdx.x / 32) * kRowsPerStep; r0 < n; r0 += step) {
-    RowIn in[kRowsPerStep];
-#pragma unroll
-    for (int i = 0; i < kRowsPerStep; ++i) {
-      int64_t s = r0 + i < n ? slots[r0 + i] : -1;
-      if (s >= num_slots) s = -1;
-      row_load(in[i], kv, s, lane);
-    }
-#pragma unroll
-    for (int i = 0; i < kRowsPerStep; ++i)
-      if (r0 + i < n) row_store(in[i], out + (r0 + i) * out_stride, lane);
+  const bool sectors = whole_sectors(out, out_stride);
+  for (int64_t r = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32; r < n; r += (int64_t)gridDim.x * kWarps) {
+    const int64_t s = slots[r];
+    RowIn in;
+    row_load(in, kv, s < num_slots ? s : -1, lane);
+    row_store(in, out + r * out_stride, lane, sectors);
   }
 }
 
@@ -187,6 +186,11 @@ __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int B
   return lo;
 }
 
+// A warp reads kRun consecutive rows: it looks for the first one's sequence, lane
+// i finds row i's slot, and the rows are in flight together.  196608 rows: 51.2 us,
+// 6.0 TB/s (runs of 8 in two halves the same, but 1.0 us more for few rows).
+constexpr int kRun = 4;
+
 __global__ void __launch_bounds__(kBlock) fp4_gather_kernel(
     const uint8_t* __restrict__ kv, int64_t num_slots, const int32_t* __restrict__ block_table,
     int64_t bt_stride, int64_t max_blocks, int block_size, const int32_t* __restrict__ cu, int B,
@@ -194,34 +198,35 @@ __global__ void __launch_bounds__(kBlock) fp4_gather_kernel(
   if (threadIdx.x == 0) pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t step = (int64_t)gridDim.x * kWarps * kRowsPerStep;
-  for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + threadIdx.x / 32) * kRowsPerStep; r0 < n; r0 += step) {
-    int b = sequence_of(cu, B, r0, lane);
-    if (b < 0 && r0 >= cu[0]) continue;  // behind the last sequence
-    int64_t slot[kRowsPerStep];
-    bool mine[kRowsPerStep];
-#pragma unroll
-    for (int i = 0; i < kRowsPerStep; ++i) {
-      const int64_t r = r0 + i;
-      if (b < 0 && r < n) b = sequence_of(cu, B, r, lane);  // in front of the first sequence
-      while (b >= 0 && r >= cu[b + 1]) b = b + 1 < B ? b + 1 : -1;
-      mine[i] = b >= 0 && r < n;
-      slot[i] = -1;
-      if (mine[i]) {
-        const int64_t p = r - cu[b] + (starts != nullptr ? starts[b] : 0);
-        const int64_t blk = p / block_size;
-        if (p >= 0 && blk < max_blocks) {
-          const int64_t s = (int64_t)block_table[b * bt_stride + blk] * block_size + (p - blk * block_size);
-          if (s >= 0 && s < num_slots) slot[i] = s;
-        }
+  const bool sectors = whole_sectors(out, out_stride);
+  const int64_t step = (int64_t)gridDim.x * kWarps * kRun;
+  const int64_t max_pos = max_blocks * block_size;  // below 2^31
+  const int first = cu[0], last = cu[B];
+  for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + threadIdx.x / 32) * kRun; r0 < n && r0 < last; r0 += step) {
+    if (r0 + kRun <= first) continue;
+    int b = sequence_of(cu, B, r0 < first ? first : r0, lane);  // (first < last, so there is one)
+    const int64_t r = r0 + lane;
+    int64_t slot = -2;  // not a row of any sequence
+    if (lane < kRun && r >= first && r < n && r < last) {
+      while (r >= cu[b + 1]) ++b;
+      slot = -1;
+      const int64_t p = r - cu[b] + (starts != nullptr ? starts[b] : 0);
+      if (p >= 0 && p < max_pos) {
+        const int64_t blk = (uint32_t)p / (uint32_t)block_size;
+        const int64_t s = (int64_t)block_table[b * bt_stride + blk] * block_size + (p - blk * block_size);
+        if (s >= 0 && s < num_slots) slot = s;
       }
     }
-    RowIn in[kRowsPerStep];
+    RowIn in[kRun];
+    int64_t s[kRun];
 #pragma unroll
-    for (int i = 0; i < kRowsPerStep; ++i) row_load(in[i], kv, slot[i], lane);
+    for (int i = 0; i < kRun; ++i) {
+      s[i] = __shfl_sync(0xFFFFFFFFu, slot, i);
+      row_load(in[i], kv, s[i], lane);
+    }
 #pragma unroll
-    for (int i = 0; i < kRowsPerStep; ++i)
-      if (mine[i]) row_store(in[i], out + (r0 + i) * out_stride, lane);
+    for (int i = 0; i < kRun; ++i)
+      if (s[i] >= -1) row_store(in[i], out + (r0 + i) * out_stride, lane, sectors);
   }
 }
 
@@ -237,14 +242,16 @@ int launch_fp4_write(const uint16_t* kv_c, int64_t kv_c_stride, const uint16_t* 
                      const int64_t* slot_mapping, int64_t N, uint8_t* cache, int64_t num_slots,
                      cudaStream_t st) {
   const int grid = grid_of((N + kWarps - 1) / kWarps, 16);
-  return check_cuda(launch_pdl(fp4_write_kernel, dim3(grid), dim3(kBlock), 0, st, kv_c, kv_c_stride, k_pe,
+  const bool vec = kv_c_stride % 8 == 0 && k_pe_stride % 8 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(kv_c) | reinterpret_cast<uintptr_t>(k_pe)) & 15) == 0;
+  return check_cuda(launch_pdl(vec ? fp4_write_kernel<true> : fp4_write_kernel<false>, dim3(grid), dim3(kBlock), 0, st, kv_c, kv_c_stride, k_pe,
                                k_pe_stride, slot_mapping, N, cache, num_slots),
                     "fp4_write_kernel launch");
 }
 
 int launch_fp4_rows(const uint8_t* kv, int64_t num_slots, const int64_t* slots, int64_t n, uint16_t* out,
                     int64_t out_stride, cudaStream_t st) {
-  const int grid = grid_of((n + kWarps * kRowsPerStep - 1) / (kWarps * kRowsPerStep), 16);
+  const int grid = grid_of((n + kWarps - 1) / kWarps, 16);
   return check_cuda(launch_pdl(fp4_rows_kernel, dim3(grid), dim3(kBlock), 0, st, kv, num_slots, slots, n, out,
                                out_stride),
                     "fp4_rows_kernel launch");
@@ -253,7 +260,7 @@ int launch_fp4_rows(const uint8_t* kv, int64_t num_slots, const int64_t* slots, 
 int launch_fp4_gather(const uint8_t* kv, int64_t num_slots, const int32_t* block_table, int64_t bt_stride,
                       int64_t max_blocks, int block_size, const int32_t* cu, int B, const int32_t* starts,
                       int64_t n, uint16_t* out, int64_t out_stride, cudaStream_t st) {
-  const int grid = grid_of((n + kWarps * kRowsPerStep - 1) / (kWarps * kRowsPerStep), 16);
+  const int grid = grid_of((n + kWarps * kRun - 1) / (kWarps * kRun), 16);
   return check_cuda(launch_pdl(fp4_gather_kernel, dim3(grid), dim3(kBlock), 0, st, kv, num_slots, block_table,
                                bt_stride, max_blocks, block_size, cu, B, starts, n, out, out_stride),
                     "fp4_gather_kernel launch");
