@@ -105,7 +105,8 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "q must be 16-byte aligned with row strides multiple of 16 bytes");
   if (!aligned16(out) || out_st % 8 || out_sh % 8)
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned with strides multiple of 8 elements");
-  if (!aligned16(kv)) return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "kv cache must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(kv) & 31u) != 0)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "kv cache must be 32-byte aligned");
   if (int rc = require_sm100()) return rc;
 
   const int64_t hpg = H / G;

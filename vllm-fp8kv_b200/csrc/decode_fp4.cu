@@ -132,16 +132,18 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
   bool ok = true;
   int64_t armed = 0;
   Ring ring;
-  for (int64_t g = 0; g < chunks && ok; g += 2) {
+#pragma unroll 1
+  for (int64_t g = -2 * slots.kAhead; g < chunks && ok; g += 2) {
     int32_t at[1];
     slots.next(a, at);
+    if (g < 0) continue;
     const int32_t slot = at[0];
     const uint32_t live2 = __ballot_sync(0xFFFFFFFFu, slot >= 0);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (g + half >= chunks) break;
       const int st = ring.st;
-      if (g + half >= kStages) ok = wait(s.raw_empty[st], ring.ph ^ 1, 20);
+      if (g + half >= kStages) ok = wait<4>(s.raw_empty[st], ring.ph ^ 1, 20);
       if (!ok) break;
       const uint32_t live = (live2 >> (16 * half)) & 0xFFFFu;
       const int n = __popc(live);
@@ -176,7 +178,7 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
   // the stages armed last have landed before the warp returns, even after a
   // failed wait
   for (int64_t x = armed > kStages ? armed - kStages : 0; x < armed; ++x)
-    (void)wait(s.raw_full[x % kStages], (uint32_t)(x / kStages) & 1, 26);
+    (void)wait<4>(s.raw_full[x % kStages], (uint32_t)(x / kStages) & 1, 26);
 }
 
 // ------------------------------------------------------------------ compute
@@ -370,7 +372,7 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int cw, int lane) {
     Ring ring = piece_at;
     ring.ahead(grp);
     for (int c = grp; c < nch; c += kGroups) {
-      if (ok) ok = wait(s.raw_full[ring.st], ring.ph, 21);
+      if (ok) ok = wait<4>(s.raw_full[ring.st], ring.ph, 21);
       const uint64_t live = *reinterpret_cast<const uint64_t*>(s.live[ring.st]);
       const uint8_t* raw = s.raw[ring.st];
       float x[2][4];

@@ -108,7 +108,8 @@ struct Smem {
   uint8_t p[2 * kPBlockBytes];
   uint8_t stage[64][528];       // half a latent of every head (rows 4 banks apart)
   float half_max[2][128];       // a tile's maxima per thread, by tile parity
-  float lsum[128];
+  float lsum[128];              // a finished piece: its sums per thread,
+  int done_t, done_head, done_heads, done_row;  // token, first head, heads, first row of partials (< 0: none)
   uint32_t qmax[128];           // largest latent magnitudes per thread
   int qk[64], qagain[2];        // powers of two of the heads; any not 0 among 32
   int32_t slot[kScoutRing][kN];   // a tile's slots, and its live bits
@@ -197,18 +198,18 @@ __device__ void mma_role(const Ctx& c) {
     bool opens = false;
     if (has_s) {
       if (left == 0) {
-        if (!wait(s.qready, p & 1, 35)) return;
+        if (!wait<1>(s.qready, p & 1, 35)) return;
         left = s.piece_tiles[p & 1];
         ++p;
         opens = true;
       }
-      if (j > 0 && !wait(s.sempty, (j - 1) & 1, 34)) return;
-      if (!wait(s.kfull[0], j & 1, 37)) return;
+      if (j > 0 && !wait<1>(s.sempty, (j - 1) & 1, 34)) return;
+      if (!wait<1>(s.kfull[0], j & 1, 37)) return;
       tc_fence_after();
       // K blocks 0-5: q in tensor memory
       ts_blocks(0, 4);
       commit(s.kempty[0]);
-      if (!wait(s.kfull[1], j & 1, 39)) return;
+      if (!wait<1>(s.kfull[1], j & 1, 39)) return;
       tc_fence_after();
       ts_blocks(4, 6);
       // blocks 6, 7 (latents) and 8 (rope): q in shared memory
@@ -226,18 +227,18 @@ __device__ void mma_role(const Ctx& c) {
     if (j > 0) {
       // (piece p - 1 - opens holds tile j - 1)
       const uint32_t piece = p - 1 - (opens ? 1 : 0);
-      if (first && piece > 0 && !wait(s.oempty, (piece - 1) & 1, 45)) return;
-      if (!wait(s.pfull, (j - 1) & 1, 36)) return;
-      if (!wait(s.vfull, (j - 1) & 1, 38)) return;
+      if (first && piece > 0 && !wait<1>(s.oempty, (piece - 1) & 1, 45)) return;
+      if (!wait<1>(s.pfull, (j - 1) & 1, 36)) return;
+      if (!wait<1>(s.vfull, (j - 1) & 1, 38)) return;
       tc_fence_after();
+      const uint32_t acc = first ? 0u : 1u;
 #pragma unroll 1
-      for (int x = 0; x < 4; ++x) {  // dims half x / 2, entries [64 (x % 2), +64)
-        const uint64_t ad = pdesc + (uint64_t)(((x & 1) * kPBlockBytes) >> 4);
-        const uint64_t bd = vdesc + (uint64_t)(((x >> 1) * 2 * kVBlockBytes + (x & 1) * 64 * 128) >> 4);
+      for (int h = 0; h < 2; ++h) {  // dims half h: entries [0,64) and [64,128)
+        const uint64_t bd = vdesc + (uint64_t)((h * 2 * kVBlockBytes) >> 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          pair_ss(tO + 128 * (x >> 1), ad + (uint64_t)(2 * i), bd + (uint64_t)((i * 16 * 128) >> 4), kIdescPV,
-                  (x & 1) || i > 0 || !first ? 1u : 0u);
+        for (int i = 0; i < 8; ++i)
+          pair_ss(tO + 128 * h, pdesc + (uint64_t)(((i >> 2) * kPBlockBytes + (i & 3) * 32) >> 4),
+                  bd + (uint64_t)((i * 16 * 128) >> 4), kIdescPV, i > 0 ? 1u : acc);
       }
       commit(s.pvdone);  // P and V may be written again
       if (last) commit(s.ofull);
@@ -259,11 +260,11 @@ __device__ void mma_role(const Ctx& c) {
 __device__ void settle(const Ctx& c) {
   Smem& s = *c.s;
   if (c.rank == 0) commit(s.drain);
-  if (!wait(s.drain, 0, 46) || c.tiles == 0) return;
+  if (!wait<1>(s.drain, 0, 46) || c.tiles == 0) return;
   const uint32_t par = (uint32_t)(c.tiles - 1) & 1;
-  (void)(wait(s.kempty[0], par, 48) && wait(s.kempty[1], par, 48) &&
-         wait(s.pvdone, par, 48) &&
-         (c.rank != 0 || wait(s.sempty, par, 48)));
+  (void)(wait<1>(s.kempty[0], par, 48) && wait<1>(s.kempty[1], par, 48) &&
+         wait<1>(s.pvdone, par, 48) &&
+         (c.rank != 0 || wait<1>(s.sempty, par, 48)));
 }
 
 // ------------------------------------------------------------------ scout
@@ -272,11 +273,14 @@ __device__ void scout(const Ctx& c, int lane) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
   Slots<kN, 1, 4> slots(a, s.share, c.worker, lane, 0);
-  for (int64_t j = 0; j < c.tiles; ++j) {
-    const int r = (int)(j % kScoutRing);
+  const int tiles = (int)c.tiles;
+#pragma unroll 1
+  for (int j = -slots.kAhead; j < tiles; ++j) {
     int32_t slot[4];
     slots.next(a, slot);
-    if (j >= kScoutRing && !wait(s.slots_empty[r], (uint32_t)(j / kScoutRing + 1) & 1, 40)) break;
+    if (j < 0) continue;
+    const int r = j % kScoutRing;
+    if (j >= kScoutRing && !wait<1>(s.slots_empty[r], (uint32_t)(j / kScoutRing + 1) & 1, 40)) break;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       s.slot[r][32 * i + lane] = slot[i];
@@ -285,15 +289,46 @@ __device__ void scout(const Ctx& c, int lane) {
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(s.slots_full[r]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int32_t sl = c.rank == 0 ? slot[i] : slot[2 + i];
+      if (sl >= 0) {
+        const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          asm volatile("prefetch.global.L2 [%0];\n" ::"l"(row + (x < 3 ? 128 * x : kFp4RowBytes - 1)));
+      }
+    }
   }
 }
 
 // ------------------------------------------------------------------ K and V
-// Lane -> (row of 8, 32-dim quarter of a 128-dim latent tile): eight lanes that
-// store or load together cover four rows and two quarters, which touch every
-// bank once in the swizzled blocks and in the 416-byte rows alike.
-__device__ __forceinline__ int lane_row(int lane) { return (lane & 3) + 4 * ((lane >> 3) & 1); }
-__device__ __forceinline__ int lane_quarter(int lane) { return ((lane >> 2) & 1) + 2 * ((lane >> 4) & 1); }
+// Four lanes read a row of 8 (lane / 4), lane q of them the 32 code bytes of one
+// 64-dim block: whole sectors, and one or two cache lines a row.  Stored in the same
+// order, the four lanes' chunks would lie in the same banks of their four blocks; so
+// lane q takes the block's two halves in the order i ^ (q & 1), and the words of each
+// in the order s ^ (q & 2).  With the swizzle of the row, eight lanes then touch every
+// bank once.
+__device__ __forceinline__ void load32(uint4 (&w)[2], const uint8_t* at) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+               : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y), "=r"(w[1].z),
+                 "=r"(w[1].w)
+               : "l"(at));
+}
+struct Codes {
+  uint4 w[2];    // halves of the block
+  uint32_t sc;   // its four scales
+  __device__ __forceinline__ void load(const uint8_t* row, int at) {
+    load32(w, row + at);
+    sc = *reinterpret_cast<const uint32_t*>(row + kFp4ScaleOff + at / 8);
+  }
+  __device__ __forceinline__ void zero() {
+    w[0] = w[1] = make_uint4(0, 0, 0, 0);
+    sc = 0;
+  }
+  // to the block's row at `block`, row r of it
+  __device__ __forceinline__ void store(uint32_t block, uint32_t r, int q) const;
+};
 
 // 32 codes and their two scales -> four 16-byte chunks of fp16 at `at` (the
 // shared address of the first, swizzled: the others differ from it in bits 4 and
@@ -313,17 +348,32 @@ __device__ __noinline__ void unpack32(uint4 w, uint32_t scales, uint32_t at) {
   }
 }
 
+__device__ __forceinline__ uint4 select(bool p, const uint4& x, const uint4& y) {
+  return make_uint4(p ? x.x : y.x, p ? x.y : y.y, p ? x.z : y.z, p ? x.w : y.w);
+}
+__device__ __forceinline__ void Codes::store(uint32_t block, uint32_t r, int q) const {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t half = i ^ (q & 1);
+    const bool turn = q & 2;
+    const uint4 v = select(half, w[1], w[0]);
+    // bytes 0 and 1: the scales of the words stored first and last
+    const uint32_t s2 = __byte_perm(sc, 0, (half ? 0x32u : 0x10u) ^ (turn ? 0x11u : 0u));
+    unpack32(select(turn, make_uint4(v.z, v.w, v.x, v.y), v), s2, (block + swz(r, 4 * half)) ^ (turn ? 32u : 0u));
+  }
+}
+
 // K warp kw: own rows [16 kw, +16) of every tile, loaded into registers one tile
 // ahead.
 __device__ void k_role(const Ctx& c, int kw, int lane) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
-  const int r8 = lane_row(lane), q = lane_quarter(lane);
-  uint4 w[2][4], rope[2][2];
-  uint32_t sc[2][4];
+  const int r8 = lane >> 2, q = lane & 3;
+  Codes w[2][2];  // [8 rows][group of blocks]
+  uint4 rope[2][2];
   auto load = [&](uint32_t j) -> bool {
     const uint32_t r = j % kScoutRing;
-    if (!wait(s.slots_full[r], (j / kScoutRing) & 1, 41)) return false;
+    if (!wait<1>(s.slots_full[r], (j / kScoutRing) & 1, 41)) return false;
     const int32_t* at = s.slot[r] + kOwn * (int)c.rank + 16 * kw + r8;
     const int32_t slot[2] = {at[0], at[8]};
     __syncwarp();
@@ -333,24 +383,17 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
       const int32_t sl = slot[h];
       if (sl >= 0) {  // a masked row keeps what the registers hold: its score is replaced
         const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          w[h][t] = ldg_v4(row + 64 * t + 16 * q);
-          sc[h][t] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * t + 2 * q);
-        }
-        rope[h][0] = ldg_v4(row + kFp4RopeOff + 32 * q);
-        rope[h][1] = ldg_v4(row + kFp4RopeOff + 32 * q + 16);
+        w[h][0].load(row, 32 * q);
+        w[h][1].load(row, 128 + 32 * q);
+        load32(rope[h], row + kFp4RopeOff + 32 * q);
       }
     }
     return true;
   };
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      w[h][t] = make_uint4(0, 0, 0, 0);
-      sc[h][t] = 0;
-    }
+    w[h][0].zero();
+    w[h][1].zero();
     rope[h][0] = rope[h][1] = make_uint4(0, 0, 0, 0);
   }
   const uint32_t tiles = (uint32_t)c.tiles;
@@ -358,15 +401,12 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
   for (uint32_t j = 0; j < tiles && ok; ++j) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {  // blocks [0,4): latent tiles 0, 1; blocks [4,9): 2, 3 and the rope
-      if (ok && j > 0) ok = wait(s.kempty[g], (j - 1) & 1, 43);
+      if (ok && j > 0) ok = wait<1>(s.kempty[g], (j - 1) & 1, 43);
       if (!ok) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t r = 16 * kw + 8 * h + r8;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          unpack32(w[h][2 * g + t], sc[h][2 * g + t],
-                   smem_u32(s.k + (4 * g + 2 * t + (q >> 1)) * kKBlockBytes + swz(r, 4 * (q & 1))));
+        w[h][g].store(smem_u32(s.k + (4 * g + q) * kKBlockBytes), r, q);
         if (g == 1) {
           *reinterpret_cast<uint4*>(s.k + 8 * kKBlockBytes + swz(r, 2 * q)) = rope[h][0];
           *reinterpret_cast<uint4*>(s.k + 8 * kKBlockBytes + swz(r, 2 * q + 1)) = rope[h][1];
@@ -384,12 +424,13 @@ __device__ void k_role(const Ctx& c, int kw, int lane) {
 __device__ void v_role(const Ctx& c, int vw, int lane) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
-  const int r8 = lane_row(lane), q = lane_quarter(lane), cr = (int)c.rank;
-  uint4 w[4][2];
-  uint32_t sc[4][2];  // (kept apart until they are used: combining them would wait for the loads)
+  const int r8 = lane >> 2, q = lane & 3;
+  // latent tiles rank and rank + 2, two 64-dim blocks of each
+  const int bytes = 64 * ((int)c.rank + 2 * (q >> 1)) + 32 * (q & 1);
+  Codes w[4];
   auto load = [&](uint32_t j) -> bool {
     const uint32_t r = j % kScoutRing;
-    if (!wait(s.slots_full[r], (j / kScoutRing) & 1, 42)) return false;
+    if (!wait<1>(s.slots_full[r], (j / kScoutRing) & 1, 42)) return false;
     const int32_t* at = s.slot[r] + 32 * vw + r8;
     const int32_t slot[4] = {at[0], at[8], at[16], at[24]};
     __syncwarp();
@@ -399,13 +440,9 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
       const int32_t sl = slot[i];
       if (sl >= 0) {
         const uint8_t* row = a.kv + (int64_t)sl * kFp4RowBytes;
-        w[i][0] = ldg_v4(row + 64 * cr + 16 * q);
-        w[i][1] = ldg_v4(row + 64 * (cr + 2) + 16 * q);
-        sc[i][0] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * cr + 2 * q);
-        sc[i][1] = *reinterpret_cast<const uint16_t*>(row + kFp4ScaleOff + 8 * (cr + 2) + 2 * q);
+        w[i].load(row, bytes);
       } else {  // zeros: P is 0 there, and nothing else may be
-        w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
-        sc[i][0] = sc[i][1] = 0;
+        w[i].zero();
       }
     }
     return true;
@@ -413,14 +450,9 @@ __device__ void v_role(const Ctx& c, int vw, int lane) {
   const uint32_t tiles = (uint32_t)c.tiles;
   bool ok = tiles > 0 && load(0);
   for (uint32_t j = 0; j < tiles && ok; ++j) {
-    if (j > 0 && !wait(s.pvdone, (j - 1) & 1, 44)) break;
+    if (j > 0 && !wait<1>(s.pvdone, (j - 1) & 1, 44)) break;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t r = 32 * vw + 8 * i + r8;
-      const uint32_t at = smem_u32(s.v + (q >> 1) * kVBlockBytes + swz(r, 4 * (q & 1)));
-      unpack32(w[i][0], sc[i][0], at);
-      unpack32(w[i][1], sc[i][1], at + 2 * kVBlockBytes);
-    }
+    for (int i = 0; i < 4; ++i) w[i].store(smem_u32(s.v + q * kVBlockBytes), 32 * vw + 8 * i + r8, q);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive_cluster(bar(s.vfull), 0);
@@ -436,11 +468,11 @@ struct Meet {
   __device__ __forceinline__ bool operator()(Smem& s, int lane) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(s.meet));
-    return wait(s.meet, n++ & 1, 47);
+    return wait<1>(s.meet, n++ & 1, 47);
   }
 };
 
-// q of the unit: dims [0,384) -> tensor memory (lanes L and L^64 both hold head
+// q of the unit (nh heads from q0 on): dims [0,384) -> tensor memory (lanes L and L^64 both hold head
 // L & 63), the rest -> swizzled shared memory (thread hh writes chunks [4 hh, +4)
 // of each block); padding rows are zero.  `scale` turns the head's accumulators
 // into scores in log2 units.
@@ -448,18 +480,15 @@ struct Meet {
 // lines an instruction; so a warp reads 512 bytes of one row an instruction, and
 // the rows change hands in shared memory: 102 us
 // instead of 104.7 at 32 x 128 heads over contexts of up to 8192.
-__device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, Meet& meet, float& scale) {
-  const Fp4DecodeArgs& a = *c.a;
-  Smem& s = *c.s;
-  const int m = L & 63, hh = L >> 6, lane = L & 31, warp = L >> 5;
-  const int head0 = w.hb * a.rows + 64 * (int)c.rank;  // of its group
-  const int nh = max(0, min(64, min(a.rows - 64 * (int)c.rank, a.hpg - head0)));
-  const uint16_t* q0 = a.q + w.t * a.q_st + (int64_t)(w.grp * a.hpg + (nh > 0 ? head0 : 0)) * a.q_sh;
+// Returns the scale, -1 after a failed wait.
+__device__ __forceinline__ float load_q(Smem& s, const uint16_t* q0, int64_t q_sh, int nh, float scale_log2,
+                                     uint32_t tmem, Meet meet) {
+  const int L = threadIdx.x, m = L & 63, hh = L >> 6, lane = L & 31, warp = L >> 5;
   const uint4 z4 = make_uint4(0, 0, 0, 0);
   auto mag = [](const uint4& v) {
     return __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
   };
-  const uint32_t trow = c.tmem + ((uint32_t)(warp * 32) << 16);
+  const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
   // First as it is, which is exact enough where the head's largest latent magnitude
   // lies in [2^-2, 2^15] (an fp16 subnormal's error is below 2^-23 of it then).
   // Else again times 2^k, which brings that magnitude to [2^8, 2^9), but the rope's at
@@ -469,7 +498,7 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, M
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     // the sign of the softmax scale goes with q, so that scores scale by a positive factor
-    const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), a.scale_log2);
+    const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), scale_log2);
     auto f16 = [&](const uint4& v) {
       auto one = [&](uint32_t u) { return pack_f16x2(bf16_lo(u) * up, bf16_hi(u) * up); };
       return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
@@ -478,18 +507,18 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, M
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {  // latent dims [256 half, +256)
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint4 x[8];
+      for (int g = 0; g < 4; ++g) {
+        uint4 x[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 16 * warp + 8 * g + i;
-          x[i] = r < nh ? reinterpret_cast<const uint4*>(q0 + r * a.q_sh + 256 * half)[lane] : z4;
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * warp + 4 * g + i;
+          x[i] = r < nh ? reinterpret_cast<const uint4*>(q0 + r * q_sh + 256 * half)[lane] : z4;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<uint4*>(s.stage[16 * warp + 8 * g + i] + 16 * lane) = x[i];
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(s.stage[16 * warp + 4 * g + i] + 16 * lane) = x[i];
       }
-      if (!meet(s, lane)) return false;
+      if (!meet(s, lane)) return -1.f;
       const uint4* row = reinterpret_cast<const uint4*>(s.stage[m]);
 #pragma unroll 1
       for (int c0 = 0; c0 < (half == 0 ? 128 : 64); c0 += 32) {  // to tensor memory
@@ -515,14 +544,14 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, M
         }
       }
       s.qmax[L] = max(mx & 0xFFFFu, mx >> 16);
-      if (!meet(s, lane)) return false;  // the stage has been read (and the maxima are in place)
+      if (!meet(s, lane)) return -1.f;  // the stage has been read (and the maxima are in place)
     }
     // the rope, four rows an instruction
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * warp + 4 * i + (lane >> 3);
-      const uint4 x = r < nh ? reinterpret_cast<const uint4*>(q0 + r * a.q_sh + kNope)[lane & 7] : z4;
-      const float ur = pass == 0 ? up : copysignf(__uint_as_float((uint32_t)(127 + s.qk[r]) << 23), a.scale_log2);
+      const uint4 x = r < nh ? reinterpret_cast<const uint4*>(q0 + r * q_sh + kNope)[lane & 7] : z4;
+      const float ur = pass == 0 ? up : copysignf(__uint_as_float((uint32_t)(127 + s.qk[r]) << 23), scale_log2);
       auto one = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * ur, bf16_hi(u) * ur); };
       *reinterpret_cast<uint4*>(s.q + 2 * kQBlockBytes + swz(r, lane & 7)) = make_uint4(one(x.x), one(x.y), one(x.z), one(x.w));
     }
@@ -532,26 +561,23 @@ __device__ bool load_q(const Ctx& c, const Walk<kN>& w, int L, uint32_t piece, M
     const bool again = bm != 0 && bm < 0x7F80 && (bm < 0x3E80 || bm > 0x4700);
     if (again) {
       uint32_t mr = 0;
-      for (int i = 0; i < 8; ++i) mr = __vmaxu2(mr, mag(reinterpret_cast<const uint4*>(q0 + m * a.q_sh + kNope)[i]));
+      for (int i = 0; i < 8; ++i) mr = __vmaxu2(mr, mag(reinterpret_cast<const uint4*>(q0 + m * q_sh + kNope)[i]));
       const int br = (int)max(mr & 0xFFFFu, mr >> 16);
       k = min(126, min(8 - ((bm >> 7) - 127), 100 - ((br >> 7) - 127)));
     }
     if (hh == 0) s.qk[m] = k;
     const bool any = __any_sync(0xFFFFFFFFu, again);
     if (hh == 0 && lane == 0) s.qagain[warp] = any ? 1 : 0;
-    if (!meet(s, lane)) return false;
+    if (!meet(s, lane)) return -1.f;
     if (s.qagain[0] == 0 && s.qagain[1] == 0) break;
   }
-  // (the piece two before this one, whose place it takes, is past its last S)
-  if (L == 0) s.piece_tiles[piece & 1] = w.here();
   fence_proxy_async_smem();
   tc_fence_before();
   __syncwarp();
-  if (lane == 0) mbar_arrive_cluster(bar(s.qready), 0);
-  scale = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k) << 23);
-  if (scale == 0.f) scale = 1.1754944e-38f;  // a masked score is an infinity times the scale
-  return true;
+  const float scale = fabsf(scale_log2) * __uint_as_float((uint32_t)(127 - k) << 23);
+  return scale == 0.f ? 1.1754944e-38f : scale;  // a masked score is an infinity times the scale
 }
+constexpr uint32_t kLoadMeets = 1;  // meetings of load_q, 5 or 9: only their parity counts
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -581,17 +607,78 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
   Walk<kN> w(a, s.share, c.worker);
   bool ok = true;
   uint32_t j = 0, piece = 0;
-  float scale = 0.f;
+  float scale = 0.f, m_ref = 0.f;
   Meet meet;
-  if (w.left > 0) ok = load_q(c, w, L, 0, meet, scale);
-  while (w.left > 0 && ok) {
+  // a turn: q of a piece, O of the piece before, the tiles of the piece
+  while (w.left > 0 || piece > 0) {
+    if (w.left > 0) {
+      const int h0 = 64 * (int)c.rank, head0 = w.hb * a.rows + h0;  // of its group
+      const int nh = max(0, min(64, min(a.rows - h0, a.hpg - head0)));
+      scale = load_q(s, a.q + w.t * a.q_st + (int64_t)(w.grp * a.hpg + (nh > 0 ? head0 : 0)) * a.q_sh, a.q_sh, nh,
+                     a.scale_log2, c.tmem, meet);
+      if (scale < 0.f) break;
+      meet.n += kLoadMeets;
+      // (the piece two before this one, whose place it takes, is past its last S)
+      if (L == 0) s.piece_tiles[piece & 1] = w.here();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(bar(s.qready), 0);
+    }
+    if (piece > 0) {
+      if (!wait<1>(s.ofull, (piece - 1) & 1, 32)) break;
+      tc_fence_after();
+      const int t = s.done_t, head = s.done_head + m, prow = s.done_row + m;
+      const bool hv = m < s.done_heads, whole = s.done_row < 0;
+      const float lt = s.lsum[L] + s.lsum[L ^ 64];
+      const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+      if (hv && hh == 0) {
+        if (whole) {
+          if (a.lse != nullptr)
+            a.lse[t * a.lse_st + head] = lt == 0.f ? -INFINITY : (m_ref - kBias) * kLn2 + logf(lt);
+        } else {
+          a.ws_ml[prow] = make_float2(m_ref, lt);
+        }
+      }
+#pragma unroll 1
+      for (int c0 = 0; c0 < 256; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32(trow + kColO + c0, o);
+        tmem_wait_ld();
+        const int d = 256 * (c0 >> 7) + 128 * hh + (c0 & 127);
+        if (hv && whole) {
+          uint16_t* dst = a.out + t * a.out_st + (int64_t)head * a.out_sh + d;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              v[x] = pack_bf16x2(__uint_as_float(o[16 * e + 2 * x]) * inv, __uint_as_float(o[16 * e + 2 * x + 1]) * inv);
+            reinterpret_cast<uint4*>(dst)[2 * e] = make_uint4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<uint4*>(dst)[2 * e + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+          }
+        } else if (hv) {
+          float* dst = a.ws_o + (int64_t)prow * kNope + d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)  // 32-byte stores: whole sectors of the thread's own row
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + 8 * e), "r"(o[8 * e]),
+                         "r"(o[8 * e + 1]), "r"(o[8 * e + 2]), "r"(o[8 * e + 3]), "r"(o[8 * e + 4]), "r"(o[8 * e + 5]),
+                         "r"(o[8 * e + 6]), "r"(o[8 * e + 7])
+                         : "memory");
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      // the next unit's O may begin (nobody waits behind the last one: see settle)
+      if (lane == 0 && w.left > 0) mbar_arrive_cluster(bar(s.oempty), 0);
+    }
+    if (w.left <= 0) break;
     const int n = w.here();
-    float m_ref = -INFINITY, l = 0.f;
+    float l = 0.f;
+    m_ref = -INFINITY;
     for (int i = 0; i < n; ++i, ++j) {
       const uint32_t par = j & 1;
-      ok = wait(s.sfull, par, 31);
+      ok = wait<1>(s.sfull, par, 31);
       const uint32_t r = j % kScoutRing;
-      if (ok) ok = wait(s.slots_full[r], (j / kScoutRing) & 1, 30);
+      if (ok) ok = wait<1>(s.slots_full[r], (j / kScoutRing) & 1, 30);
       if (!ok) break;
       const uint32_t live0 = s.vmask[r][2 * hh], live1 = s.vmask[r][2 * hh + 1];
       tc_fence_after();
@@ -638,7 +725,7 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
         pk[e] = pack_f16x2(p2.x, p2.y);
       }
       l += l2.x + l2.y;
-      if (j > 0) ok = wait(s.pvdone, (j - 1) & 1, 33);
+      if (j > 0) ok = wait<1>(s.pvdone, (j - 1) & 1, 33);
       if (!ok) break;
       if (__any_sync(0xFFFFFFFFu, alpha != 1.f) && i > 0) {
         tc_fence_after();
@@ -663,68 +750,23 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
       if (lane == 0) mbar_arrive_cluster(bar(s.pfull), 0);
     }
     if (!ok) break;
-    // ---- the piece: its sums, the next unit's q, then its O
+    // the piece's sums and place, for the stores of its O
     s.lsum[L] = l;
-    ok = meet(s, lane);
-    if (!ok) break;
-    const float lt = l + s.lsum[L ^ 64];
-    const bool whole = w.c == 0 && n == w.n;
-    const int64_t t = w.t;
-    const int head = w.hb * a.rows + 64 * (int)c.rank + m;
-    const bool hv = 64 * (int)c.rank + m < a.rows && head < a.hpg;
-    const int64_t hg = (int64_t)w.grp * a.hpg + head;
-    const int64_t prow = (2 * (int64_t)c.worker + (w.c == 0 ? 1 : 0)) * a.rows + 64 * (int)c.rank + m;
+    if (L == 0) {
+      const int h0 = 64 * (int)c.rank;  // of the unit
+      s.done_t = (int)w.t;
+      s.done_head = w.grp * a.hpg + w.hb * a.rows + h0;
+      s.done_heads = min(a.rows - h0, a.hpg - w.hb * a.rows - h0);
+      s.done_row = w.c == 0 && n == w.n ? -a.rows : (2 * c.worker + (w.c == 0 ? 1 : 0)) * a.rows + h0;
+    }
+    if (!meet(s, lane)) break;
     w.next_unit(a, n);
-    if (w.left > 0) ok = load_q(c, w, L, piece + 1, meet, scale);
-    if (ok) ok = wait(s.ofull, piece & 1, 32);
-    if (!ok) break;
-    tc_fence_after();
-    const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
-    if (hv && hh == 0) {
-      if (whole) {
-        if (a.lse != nullptr)
-          a.lse[t * a.lse_st + hg] = lt == 0.f ? -INFINITY : (m_ref - kBias) * kLn2 + logf(lt);
-      } else {
-        a.ws_ml[prow] = make_float2(m_ref, lt);
-      }
-    }
-#pragma unroll 1
-    for (int c0 = 0; c0 < 256; c0 += 32) {
-      uint32_t o[32];
-      tmem_ld32(trow + kColO + c0, o);
-      tmem_wait_ld();
-      const int d = 256 * (c0 >> 7) + 128 * hh + (c0 & 127);
-      if (hv && whole) {
-        uint16_t* dst = a.out + t * a.out_st + hg * a.out_sh + d;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t v[8];
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            v[x] = pack_bf16x2(__uint_as_float(o[16 * e + 2 * x]) * inv, __uint_as_float(o[16 * e + 2 * x + 1]) * inv);
-          reinterpret_cast<uint4*>(dst)[2 * e] = make_uint4(v[0], v[1], v[2], v[3]);
-          reinterpret_cast<uint4*>(dst)[2 * e + 1] = make_uint4(v[4], v[5], v[6], v[7]);
-        }
-      } else if (hv) {
-        float* dst = a.ws_o + prow * kNope + d;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)  // 32-byte stores: whole sectors of the thread's own row
-          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + 8 * e), "r"(o[8 * e]),
-                       "r"(o[8 * e + 1]), "r"(o[8 * e + 2]), "r"(o[8 * e + 3]), "r"(o[8 * e + 4]), "r"(o[8 * e + 5]),
-                       "r"(o[8 * e + 6]), "r"(o[8 * e + 7])
-                       : "memory");
-      }
-    }
-    tc_fence_before();
-    __syncwarp();
-    // the next unit's O may begin (nobody waits behind the last one: see settle)
-    if (lane == 0 && w.left > 0) mbar_arrive_cluster(bar(s.oempty), 0);
     ++piece;
   }
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    decode_fp4_tc_kernel(const Fp4DecodeArgs a) {
+    decode_fp4_tc_kernel(const __grid_constant__ Fp4DecodeArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
   Smem& s = *reinterpret_cast<Smem*>(smem_raw + (((raw_base + 1023u) & ~1023u) - raw_base));

@@ -20,6 +20,12 @@ __device__ __forceinline__ int chunks_of(int entries) {
   return entries > kChunk ? (entries + kChunk - 1) / kChunk : 1;
 }
 
+// u / d: nearly always in 32 bits (a 64-bit division is 1.6 KB of code).
+__device__ __forceinline__ int64_t quotient64(int64_t u, int d) { return u / d; }
+__device__ __forceinline__ int64_t quotient(int64_t u, int d) {
+  return (u >> 32) == 0 ? (int64_t)((uint32_t)u / (uint32_t)d) : quotient64(u, d);
+}
+
 struct Share {  // in shared memory: one worker's share of the chunk list
   int64_t total;       // chunks of the call
   int64_t per;         // chunks per worker
@@ -38,7 +44,7 @@ __device__ void divide(const Fp4DecodeArgs& a, Share& s, int worker) {
       const int64_t n = chunks_of<kChunk>(a.topk), at = (int64_t)worker * a.per;
       s.total = (int64_t)a.T * per_tok * n;
       s.per = a.per;
-      s.start_unit = at / n;
+      s.start_unit = quotient(at, n);
       s.start_chunk = (int)(at - s.start_unit * n);
     }
     __syncthreads();
@@ -53,7 +59,7 @@ __device__ void divide(const Fp4DecodeArgs& a, Share& s, int worker) {
   int64_t total = 0;
   for (int w = 0; w < kThreads / 32; ++w) total += s.scan[w];
   total *= per_tok;
-  int64_t per = (total + a.workers - 1) / a.workers;
+  int64_t per = quotient(total + a.workers - 1, a.workers);
   if (per < a.min_per) per = a.min_per;
   const int64_t at = (int64_t)worker * per;
   int64_t before = 0;  // chunks of the tokens in front of this pass
@@ -73,7 +79,7 @@ __device__ void divide(const Fp4DecodeArgs& a, Share& s, int worker) {
     for (int w = 0; w < warp; ++w) base += s.scan[w];
     const int64_t hi = base + inc, lo = hi - mine;
     if (t < a.T && at >= lo && at < hi) {
-      const int64_t u = (at - lo) / n;
+      const int64_t u = quotient(at - lo, n);
       s.start_unit = (int64_t)t * per_tok + u;
       s.start_chunk = (int)(at - lo - u * n);
     }
@@ -98,7 +104,7 @@ struct Walk {
   __device__ __forceinline__ void open(const Fp4DecodeArgs& a, int64_t u) {
     const int per_tok = a.G * a.hb_per_group;
     unit = u;
-    t = u / per_tok;
+    t = quotient(u, per_tok);
     const int r = (int)(u - t * per_tok);
     grp = r / a.hb_per_group;
     hb = r - grp * a.hb_per_group;
@@ -136,18 +142,22 @@ __device__ __forceinline__ void note_start(const Fp4DecodeArgs& a, const Share& 
   info[3] = s.per;
 }
 
+__device__ __forceinline__ int32_t block_by_division(int32_t v, int32_t block_size) { return v / block_size; }
+__device__ __forceinline__ int32_t block_of(const Fp4DecodeArgs& a, int32_t v) {
+  return a.block_shift >= 0 ? (v >> a.block_shift) : block_by_division(v, a.block_size);
+}
 // Block-table word of an entry (0 without a table), and the entry's slot given
 // that word; -1: masked, behind the table, or outside the pool.
 __device__ __forceinline__ int32_t table_word(const Fp4DecodeArgs& a, int32_t req, int32_t v) {
   if (a.block_table == nullptr || v < 0) return 0;
-  const int32_t blk = a.block_shift >= 0 ? (v >> a.block_shift) : v / a.block_size;
+  const int32_t blk = block_of(a, v);
   return blk < a.max_blocks ? a.block_table[(int64_t)req * a.bt_stride + blk] : -1;
 }
 __device__ __forceinline__ int32_t slot_of(const Fp4DecodeArgs& a, int32_t v, int32_t page) {
   int64_t s = v;
   if (a.block_table != nullptr) {
     if (v < 0 || page < 0) return -1;
-    const int32_t blk = a.block_shift >= 0 ? (v >> a.block_shift) : v / a.block_size;
+    const int32_t blk = block_of(a, v);
     s = (int64_t)page * a.block_size + (v - blk * a.block_size);
   }
   return s >= 0 && s < a.num_slots ? (int32_t)s : -1;
@@ -186,20 +196,19 @@ struct Slots {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) p[i] = table_word(a, r, e[i]);
   }
-  // of chunks first, first + kStride, ... of the run
+  // of chunks first, first + kStride, ... of the run; the first kAhead calls of
+  // next() only fill the pipeline
+  static constexpr int kAhead = 3;
   __device__ __forceinline__ Slots(const Fp4DecodeArgs& a, const Share& s, int worker, int row_, int first)
       : ahead(a, s, worker), row(row_) {
     at_unit(a);
-    for (int i = 0; i < first; ++i) step(a);
+    if (first) step(a);  // (0 or 1)
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      fetch(a, v[i]);
-      rq[i] = req;
-#pragma unroll
-      for (int k = 0; k < kStride; ++k) step(a);
+    for (int i = 0; i < kRows; ++i) {
+      v[0][i] = v[1][i] = v[2][i] = -1;
+      pg[0][i] = pg[1][i] = 0;
     }
-    words(a, rq[0], v[0], pg[0]);
-    words(a, rq[1], v[1], pg[1]);
+    rq[0] = rq[1] = rq[2] = 0;
   }
   __device__ __forceinline__ void next(const Fp4DecodeArgs& a, int32_t (&slot)[kRows]) {
 #pragma unroll
@@ -221,9 +230,11 @@ struct Slots {
 // Bounded wait of a whole warp: every lane looks (so every lane has acquired the
 // phase) and the vote gives all of them one verdict.  A phase that is complete
 // costs 18 cycles; one lane looking for the others and passing the verdict on
-// costs 190.
+// costs 190.  kUnroll: the compiler's choice would be 8 KB of code for every wait.
+template <int kUnroll>
 __device__ __forceinline__ bool wait(uint64_t& b, uint32_t parity, uint32_t where) {
   const uint32_t at = smem_u32(&b);
+#pragma unroll kUnroll
   for (uint32_t it = 0; it < tc::kMaxWaitIters; ++it)
     if (__all_sync(0xFFFFFFFFu, tc::mbar_try_wait(at, parity))) return true;
   if ((threadIdx.x & 31) == 0) atomicOr(&tc::g_device_status, tc::kStatusWaitTimeout | (where << 8));
