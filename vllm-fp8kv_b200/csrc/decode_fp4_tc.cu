@@ -180,9 +180,9 @@ __device__ void mma_role(const Ctx& c) {
   const uint64_t pdesc = sdesc_sw128(smem_u32(s.p), 16, 1024);
   const uint64_t vdesc = sdesc_sw128(smem_u32(s.v), kVBlockBytes, 1024);
   const uint32_t tiles = (uint32_t)c.tiles;
-  uint32_t p = 0;                     // pieces opened
-  int left = 0;                       // tiles of the open piece still to come
-  bool first = false, last = false;   // tile j - 1 opens / closes its piece
+  uint32_t p = 0;      // pieces opened
+  int left = 0;        // tiles of the open piece whose S is still to come
+  bool first = false;  // the next O begins its piece
   auto ts_blocks = [&](int from, int to) {
 #pragma unroll 1
     for (int b = from; b < to; ++b) {
@@ -192,24 +192,24 @@ __device__ void mma_role(const Ctx& c) {
         pair_ts(tS, tQ + 32 * b + 8 * i, bd + (uint64_t)(2 * i), kIdescLatent, (b | i) ? 1u : 0u);
     }
   };
-  // turn j: S of tile j, then O of tile j - 1
-  for (uint32_t j = 0; j <= tiles && tiles > 0; ++j) {
-    const bool has_s = j < tiles;
-    bool opens = false;
-    if (has_s) {
+  // S goes one tile ahead of O within a piece; a new piece, whose q may be long in
+  // coming, waits until the O's of the one before are on their way
+  uint32_t js = 0, jo = 0;  // next S, next O
+  while (jo < tiles) {
+    if (js < tiles && (js == jo || (js == jo + 1 && left > 0))) {
       if (left == 0) {
         if (!wait<1>(s.qready, p & 1, 35)) return;
         left = s.piece_tiles[p & 1];
         ++p;
-        opens = true;
+        first = true;
       }
-      if (j > 0 && !wait<1>(s.sempty, (j - 1) & 1, 34)) return;
-      if (!wait<1>(s.kfull[0], j & 1, 37)) return;
+      if (js > 0 && !wait<1>(s.sempty, (js - 1) & 1, 34)) return;
+      if (!wait<1>(s.kfull[0], js & 1, 37)) return;
       tc_fence_after();
       // K blocks 0-5: q in tensor memory
       ts_blocks(0, 4);
       commit(s.kempty[0]);
-      if (!wait<1>(s.kfull[1], j & 1, 39)) return;
+      if (!wait<1>(s.kfull[1], js & 1, 39)) return;
       tc_fence_after();
       ts_blocks(4, 6);
       // blocks 6, 7 (latents) and 8 (rope): q in shared memory
@@ -223,13 +223,12 @@ __device__ void mma_role(const Ctx& c) {
       }
       commit(s.kempty[1]);
       commit(s.sfull);
-    }
-    if (j > 0) {
-      // (piece p - 1 - opens holds tile j - 1)
-      const uint32_t piece = p - 1 - (opens ? 1 : 0);
-      if (first && piece > 0 && !wait<1>(s.oempty, (piece - 1) & 1, 45)) return;
-      if (!wait<1>(s.pfull, (j - 1) & 1, 36)) return;
-      if (!wait<1>(s.vfull, (j - 1) & 1, 38)) return;
+      ++js;
+      --left;
+    } else {
+      if (first && p > 1 && !wait<1>(s.oempty, p & 1, 45)) return;  // of piece p - 2
+      if (!wait<1>(s.pfull, jo & 1, 36)) return;
+      if (!wait<1>(s.vfull, jo & 1, 38)) return;
       tc_fence_after();
       const uint32_t acc = first ? 0u : 1u;
 #pragma unroll 1
@@ -241,11 +240,10 @@ __device__ void mma_role(const Ctx& c) {
                   bd + (uint64_t)((i * 16 * 128) >> 4), kIdescPV, i > 0 ? 1u : acc);
       }
       commit(s.pvdone);  // P and V may be written again
-      if (last) commit(s.ofull);
+      ++jo;
+      if (left == 0 && jo == js) commit(s.ofull);
+      first = false;
     }
-    first = opens;
-    --left;
-    last = left == 0;
   }
 }
 
@@ -507,17 +505,22 @@ __device__ __forceinline__ float load_q(Smem& s, const uint16_t* q0, int64_t q_s
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {  // latent dims [256 half, +256)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint4 x[4];
+      for (int i = 0; i < 16; ++i) {
+        const int r = 16 * warp + i;
+        cp_async16(smem_u32(s.stage[r] + 16 * lane), q0 + (r < nh ? r : 0) * q_sh + 256 * half + 8 * lane, r < nh ? 16 : 0);  // zeros past nh
+      }
+      if (half == 1) {  // the rope, four rows an instruction
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = 16 * warp + 4 * g + i;
-          x[i] = r < nh ? reinterpret_cast<const uint4*>(q0 + r * q_sh + 256 * half)[lane] : z4;
+          const int r = 16 * warp + 4 * i + (lane >> 3);
+          const uint4 x = r < nh ? reinterpret_cast<const uint4*>(q0 + r * q_sh + kNope)[lane & 7] : z4;
+          const float ur = pass == 0 ? up : copysignf(__uint_as_float((uint32_t)(127 + s.qk[r]) << 23), scale_log2);
+          auto one = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * ur, bf16_hi(u) * ur); };
+          *reinterpret_cast<uint4*>(s.q + 2 * kQBlockBytes + swz(r, lane & 7)) =
+              make_uint4(one(x.x), one(x.y), one(x.z), one(x.w));
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(s.stage[16 * warp + 4 * g + i] + 16 * lane) = x[i];
       }
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
       if (!meet(s, lane)) return -1.f;
       const uint4* row = reinterpret_cast<const uint4*>(s.stage[m]);
 #pragma unroll 1
@@ -545,15 +548,6 @@ __device__ __forceinline__ float load_q(Smem& s, const uint16_t* q0, int64_t q_s
       }
       s.qmax[L] = max(mx & 0xFFFFu, mx >> 16);
       if (!meet(s, lane)) return -1.f;  // the stage has been read (and the maxima are in place)
-    }
-    // the rope, four rows an instruction
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * warp + 4 * i + (lane >> 3);
-      const uint4 x = r < nh ? reinterpret_cast<const uint4*>(q0 + r * q_sh + kNope)[lane & 7] : z4;
-      const float ur = pass == 0 ? up : copysignf(__uint_as_float((uint32_t)(127 + s.qk[r]) << 23), scale_log2);
-      auto one = [&](uint32_t u) { return pack_bf16x2(bf16_lo(u) * ur, bf16_hi(u) * ur); };
-      *reinterpret_cast<uint4*>(s.q + 2 * kQBlockBytes + swz(r, lane & 7)) = make_uint4(one(x.x), one(x.y), one(x.z), one(x.w));
     }
     tmem_wait_st();
     if (pass == 1) break;
@@ -599,6 +593,13 @@ __device__ __forceinline__ float2 add2(float2 v, float2 w) {
   return v;
 }
 
+// A whole sector of the thread's own row.
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 __device__ void softmax_role(const Ctx& c, int warp, int lane) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
@@ -609,6 +610,7 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
   uint32_t j = 0, piece = 0;
   float scale = 0.f, m_ref = 0.f;
   Meet meet;
+  const bool sectors = ((reinterpret_cast<uintptr_t>(a.out) | (a.out_st * 2) | (a.out_sh * 2)) & 31) == 0;
   // a turn: q of a piece, O of the piece before, the tiles of the piece
   while (w.left > 0 || piece > 0) {
     if (w.left > 0) {
@@ -652,17 +654,17 @@ __device__ void softmax_role(const Ctx& c, int warp, int lane) {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
               v[x] = pack_bf16x2(__uint_as_float(o[16 * e + 2 * x]) * inv, __uint_as_float(o[16 * e + 2 * x + 1]) * inv);
-            reinterpret_cast<uint4*>(dst)[2 * e] = make_uint4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<uint4*>(dst)[2 * e + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+            if (sectors) {
+              store32(dst + 16 * e, v);
+            } else {
+              reinterpret_cast<uint4*>(dst)[2 * e] = make_uint4(v[0], v[1], v[2], v[3]);
+              reinterpret_cast<uint4*>(dst)[2 * e + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+            }
           }
         } else if (hv) {
           float* dst = a.ws_o + (int64_t)prow * kNope + d;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)  // 32-byte stores: whole sectors of the thread's own row
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + 8 * e), "r"(o[8 * e]),
-                         "r"(o[8 * e + 1]), "r"(o[8 * e + 2]), "r"(o[8 * e + 3]), "r"(o[8 * e + 4]), "r"(o[8 * e + 5]),
-                         "r"(o[8 * e + 6]), "r"(o[8 * e + 7])
-                         : "memory");
+          for (int e = 0; e < 4; ++e) store32(dst + 8 * e, reinterpret_cast<uint32_t(&)[8]>(o[8 * e]));
         }
       }
       tc_fence_before();
