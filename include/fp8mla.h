@@ -350,7 +350,8 @@ FP8MLA_API int fp8mla_indexer_topk(const float* logits, int64_t rows, int64_t lo
 
 /* ======================= fp4_ds_mla: the 4-bit cache =======================
  * No reference counterpart.  Rows as described at FP8MLA_FP4_ROW_BYTES; a
- * pool is [num_slots, 416] uint8, 16-byte aligned, num_slots < 2^31. */
+ * pool is [num_slots, 416] uint8, 16-byte aligned (32-byte for the attention),
+ * num_slots < 2^31. */
 
 /*
  * Cache writer: bf16 latent + rope -> 416-byte rows.  Per group of 16 values

@@ -88,7 +88,7 @@ def c_decode(**over):
     (dict(q=264), b"q must be 16-byte aligned"),
     (dict(q_sh=577), b"q must be 16-byte aligned"),
     (dict(out_st=8193), b"out must be 16-byte aligned"),
-    (dict(kv=257), b"kv cache must be 16-byte aligned"),
+    (dict(kv=272), b"kv cache must be 32-byte aligned"),
 ])
 def test_c_refusals(over, needle):
     assert c_decode(**over) == N.ERR_INVALID_ARGUMENT

@@ -17,7 +17,25 @@ struct Plan {
   int64_t per;  // 0: from the lengths, on the device
   bool cuts;    // some unit may be cut
   bool tc;      // the paired tensor-core kernel
+  double us;    // expected time (lengths known)
 };
+// Expected time, us, of a call whose workers take `per` chunks each of units of n
+// chunks; `cut`: units are cut, so there are partial results, a merge, and more
+// changes of unit than need be, unless n is a multiple of `per`.  Fitted to 560 calls of
+// either kernel (16 to 256 heads, 1 to 300 tokens, top-256 to top-4096), off by 3% on
+// average; choosing by it costs 0.1% against the best choice for each call.  For
+// instance, top-2048, 16-head kernel / paired kernel / chosen, measured:
+//   tokens   40 heads            64 heads            128 heads
+//   1        18.8 / 19 / 18.8    19.6 / 20 / 19.6    20.7 / 21 / 20.7
+//   8        24.3 / 25 / 24.3    25.7 / 27 / 25.7    34.6 / 31 / 31.0
+//   32       42.9 / 48 / 42.9    45.2 / 49 / 45.2    87 / 49.6 / 49.6
+//   160      151 / 142 / 142     204 / 139 / 141     384 / 146 / 146
+double cost(bool tc, int64_t per, int64_t n, bool cut) {
+  const double units = per > n ? (double)per / (double)n : 1.0;
+  if (tc) return 2.8 + 2.46 * (double)per + 8.6 * units + (!cut ? 0 : n % per == 0 ? 11.4 : 24.6);
+  return 1.6 + 1.21 * (double)per + 4.6 * units + (!cut ? 0 : n % per == 0 ? 6.3 : 9.6);
+}
+
 // topk < 0: whole contexts, of at most max_len positions
 Plan plan_with(bool tc, int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
   Plan p;
@@ -36,35 +54,28 @@ Plan plan_with(bool tc, int64_t T, int64_t H, int64_t G, int64_t topk, int64_t m
   if (topk < 0) {
     p.per = 0;
     p.cuts = n > 1;
+    p.us = 0;
     return p;
   }
   p.per = (total + p.workers - 1) / p.workers;
   if (p.per < p.min_per) p.per = p.min_per;
-  // whole units where that adds a sixth, or 256 entries, at most: there are no
-  // partials then and the merge's launch (4 us, the time of about four chunks)
-  // is saved
+  // whole units, or equal runs whose borders cut units
   const int64_t whole = (p.per + n - 1) / n * n;
-  p.cuts = whole * 6 > p.per * 7 && (whole - p.per) * chunk > 256;
-  if (!p.cuts) p.per = whole;
+  p.us = cost(tc, whole, n, false);
+  p.cuts = whole != p.per && 1.02 * cost(tc, p.per, n, true) < p.us;  // (near ties: no partials)
+  if (p.cuts)
+    p.us = cost(tc, p.per, n, true);
+  else
+    p.per = whole;
   p.workers = (int)((total + p.per - 1) / p.per);
   return p;
 }
-// Which kernel.  Up to 32 heads per group the paired one wastes three quarters of
-// its tile: not at any size.  Above, a run of n tiles costs it about 3 n us, a run of
-// n chunks costs the other 1.45 n, and the paired one takes 9 us more to get
-// going and to end.  Measured, us, the other one / the paired one, top-2048:
-//   heads     33-48          49-64          128            256
-//   T = 1     19.2 / 20.0    19.9 / 21.0    20.8 / 21.5    18.5 / 23.1
-//   T = 4     21.5 / 22.9    18.4 / 23.9    26.2 / 27.4    35.1 / 32.4
-//   T = 16    31.1 / 32.5    34.9 / 33.5    45.5 / 35.7    87.5 / 63.7
-//   T = 64    72.6 / 59.6    88.1 / 60.6     173 / 61.6     299 / 124
-// (17 to 32 heads at T = 64: 45.6 / 58.5).  Lengths that only the device knows are
-// taken for long ones.
+// Which kernel: the one that should be done first.  Lengths that only the device
+// knows are taken for long ones: there the paired kernel is ahead from 33 heads on
+// (with 17 to 32 it wastes three quarters of its tile).
 Plan plan_of(int64_t T, int64_t H, int64_t G, int64_t topk, int64_t max_len) {
-  const Plan one = plan_with(false, T, H, G, topk, max_len);
-  if (H / G <= 32) return one;
-  const Plan pair = plan_with(true, T, H, G, topk, max_len);
-  return topk < 0 || one.per >= 2 * pair.per + 6 ? pair : one;
+  const Plan one = plan_with(false, T, H, G, topk, max_len), pair = plan_with(true, T, H, G, topk, max_len);
+  return (topk < 0 ? H / G > 32 : pair.us < one.us) ? pair : one;
 }
 int64_t info_bytes(const Plan& p) { return (int64_t)p.workers * 4 * 8; }
 int64_t part_bytes(const Plan& p) { return (int64_t)2 * p.workers * p.rows * FP8MLA_NOPE * 4; }

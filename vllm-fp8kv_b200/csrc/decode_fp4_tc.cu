@@ -18,12 +18,16 @@
 // next tile while the other group and the O product of the tile before are still
 // running; V while the next tile's S runs.
 //
-// Measured, us: 64 x 128 heads x top-2048, paged: 64.3 (16 tiles a pair); its
-// products take 22.5 at the rate of a large matrix product, its rows' bytes 8.3.  A tile takes 3.1 us, of which the
-// chain S -> softmax -> P -> O is the longest part: S and O of one tile cannot
-// overlap (one S, one P: tensor memory is full).  12 us go by before the first S
-// (cold code, and a chain of three memory latencies: entries, block table, rows)
-// and 5 behind the last P.  One context of 131072 x 128 heads: 72.5.
+// Measured, us: 64 x 128 heads x top-2048, paged: 55.3 (16 tiles a pair); its
+// products take 22.5 at the rate of a large matrix product, its rows' bytes 8.3.
+// A tile takes 4400 cycles.  What bounds it is the traffic of shared memory, about 3000
+// cycles of it: K and V written (136 KB), read by the MMAs (192 KB), P, and the rows'
+// way through the L1; S runs at half its rate beside the unpacking.  About 11 us go by
+// before the first S (cold code, and a chain of three memory latencies: entries,
+// block table, rows) and 5 behind the last P; a change of unit costs 9 (q, O).
+// Steps on the way: 182 (64-entry tiles of mma.sync: 181), 112 one call per role, 79 waits
+// that vote, 67 rows by way of registers, 65 the scout, 62 waits not unrolled and rows
+// prefetched into L2, 56 rows read sector by sector.
 //
 // The latents are exact in fp16 (fp4.cuh), so the 32 latent k-steps of S and the
 // O product are fp16 MMAs: q is scaled per head by a power of two to a largest
@@ -476,8 +480,8 @@ struct Meet {
 // into scores in log2 units.
 // A thread needs its head's whole row, and 32 rows read 16 bytes at a time are 32
 // lines an instruction; so a warp reads 512 bytes of one row an instruction, and
-// the rows change hands in shared memory: 102 us
-// instead of 104.7 at 32 x 128 heads over contexts of up to 8192.
+// the rows change hands in shared memory.  The copies are asynchronous:
+// through registers, four rows at a time, each four waited for the ones before.
 // Returns the scale, -1 after a failed wait.
 __device__ __forceinline__ float load_q(Smem& s, const uint16_t* q0, int64_t q_sh, int nh, float scale_log2,
                                      uint32_t tmem, Meet meet) {
@@ -817,7 +821,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // one call per role: the loops of all roles together have to stay in the SM's
   // instruction cache (with each role inlined twice, and the unpacking and the
   // softmax unrolled in full, warps waited for instructions most of the time:
-  // 182 instead of 112 us, then, at 64 x 128 heads x top-2048)
+  // 182 instead of 112 us at 64 x 128 heads x top-2048)
   if (warp < kSoftmaxWarps) {
     softmax_role(c, warp, lane);
   } else if (warp == kMmaWarp) {
