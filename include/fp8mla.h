@@ -412,7 +412,7 @@ FP8MLA_API int fp8mla_fp4_sparse_decode(const uint16_t* q, int64_t T, int64_t H,
                                         int64_t workspace_bytes, void* stream);
 
 /* The same over request-local positions (block table as in
- * fp8mla_sparse_decode_paged). */
+ * fp8mla_sparse_decode_paged; req_id[t] < 0 masks all of token t). */
 FP8MLA_API int fp8mla_fp4_sparse_decode_paged(
     const uint16_t* q, int64_t T, int64_t H, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* kv,
     int64_t num_slots, const int32_t* req_id, const int32_t* block_table, int64_t bt_stride,
@@ -425,7 +425,7 @@ FP8MLA_API int fp8mla_fp4_sparse_decode_paged(
  * Attention over whole contexts: query token t attends to positions
  * [0, context_lens[t]) of request req_id[t] through the block table (lengths
  * below 0 count as 0, above max_blocks * block_size as that; positions whose
- * slot is outside the pool are masked).  Lengths are read on the device, so
+ * slot is outside the pool are masked, all of them where req_id[t] < 0).  Lengths are read on the device, so
  * one captured graph serves changing lengths.  With several query tokens of a
  * request, each one's own length makes the attention causal.
  */

@@ -103,11 +103,14 @@ def test_c_table_refusals():
                                    lens, 0.1, 256, 16 * 512, 512, None, 16, None, 0, None)
 
     for kw, needle in ((dict(block_size=0), b"bad block table"), (dict(stride=3), b"bad block table"),
-                       (dict(max_blocks=1 << 30, stride=1 << 30), b"positions"), (dict(req=None), b"required"),
+                       (dict(max_blocks=1 << 30, stride=1 << 30), b"positions"),
+                       (dict(max_blocks=1 << 58, stride=1 << 58), b"positions"), (dict(req=None), b"required"),
                        (dict(table=None), b"required"), (dict(lens=None), b"context_lens")):
         assert dense(**kw) == N.ERR_INVALID_ARGUMENT
         assert needle in L.fp8mla_last_error(), (kw, L.fp8mla_last_error())
     assert L.fp8mla_fp4_gather(256, 64, 256, 1, 2, 64, 256, 1, None, 4, 256, 576, None) == N.ERR_INVALID_ARGUMENT
+    assert L.fp8mla_fp4_gather(256, 64, 256, 1 << 58, 1 << 58, 64, 256, 1, None, 4, 256, 576,
+                               None) == N.ERR_INVALID_ARGUMENT
     assert L.fp8mla_fp4_gather(256, 64, 256, 2, 2, 64, 256, 1, None, 4, 256, 575, None) == N.ERR_INVALID_ARGUMENT
     assert L.fp8mla_fp4_write(256, 511, 256, 64, 256, 1, 256, 64, None) == N.ERR_INVALID_ARGUMENT
     assert L.fp8mla_fp4_write(256, 512, 256, 64, None, 1, 256, 64, None) == N.ERR_INVALID_ARGUMENT

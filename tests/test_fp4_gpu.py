@@ -366,6 +366,30 @@ def test_paged(H, page):
     assert H <= 32 or F.fp4_kernel_name(H, 1, 5 * 24, 170) == MANY
 
 
+@pytest.mark.parametrize("H", [16, 128])
+def test_padding_tokens(H):
+    """Tokens with a negative request attend to nothing, whatever their other
+    inputs hold, and leave the others' results alone."""
+    pool = make_pool(54, 640)
+    table = ints(55, 10, (3, 6)).to(torch.int32)
+    T = 80  # (both kernels at 128 heads: sparse calls of 80 and of 4 tokens)
+    req = (torch.arange(T, device="cuda") % 4 - 1).to(torch.int32)
+    q = randn(56, T, H, 576)
+    tok = ints(57, 384, (T, 1, 200)).to(torch.int32)
+    lens = ints(58, 384, (T,)).to(torch.int32)
+    at = table.clone()[req.long().clamp(0)]  # a row a token
+    rows = torch.arange(T, device="cuda")
+    masked = torch.where((req < 0)[:, None, None], -1, paged_slots(at, rows, tok, 64, 6))
+    want = R.attend(q, pool, masked, SCALE)
+    for n in (T, 4):
+        got = F.fp4_ds_mla_sparse_decode_paged(q[:n], pool, req[:n], table, tok[:n], SCALE, return_lse=True)
+        R.check(got, [w[:n] for w in want])
+    got = F.fp4_ds_mla_decode(q, pool, req, table, lens, SCALE, return_lse=True)
+    live = torch.where(req < 0, 0, lens)
+    R.check(got, R.attend(q, pool, dense_slots(at, rows, live, 64), SCALE))
+    status_clean()
+
+
 def dense_slots(table, req, lens, page):
     most = max(1, int(lens.max()))
     pos = torch.arange(most, device="cuda")
@@ -445,6 +469,10 @@ def test_q_layouts_and_workspace(H, T):
     for v in views:
         got = F.fp4_ds_mla_sparse_decode(v, pool, idx, SCALE, return_lse=True, workspace=ws)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    odd = q[:1].clone().as_strided((1, H, 576), (H * 576 + 4, 576, 1))  # a single token's stride is not used
+    assert odd.stride(0) % 8 == 4
+    assert torch.equal(F.fp4_ds_mla_sparse_decode(odd, pool, idx[:1], SCALE),
+                       F.fp4_ds_mla_sparse_decode(q[:1], pool, idx[:1], SCALE))
     wide = torch.cat([idx, idx], 2)[:, :, :200]
     assert torch.equal(F.fp4_ds_mla_sparse_decode(q, pool, wide, SCALE), want[0])
 

@@ -88,9 +88,10 @@ int check_table(const int32_t* req_id, const int32_t* block_table, int64_t bt_st
   if (block_size <= 0 || block_size > (1 << 20) || max_blocks < 0 || bt_stride < max_blocks)
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "bad block table: block_size=%lld max_blocks=%lld stride=%lld",
                      (long long)block_size, (long long)max_blocks, (long long)bt_stride);
-  if (max_blocks * block_size > INT32_MAX)
-    return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "a block-table row covers %lld positions; 2^31 - 1 at most",
-                     (long long)(max_blocks * block_size));
+  if (max_blocks > INT32_MAX / block_size)
+    return set_error(FP8MLA_ERR_INVALID_ARGUMENT,
+                     "a block-table row of %lld pages of %lld covers more than 2^31 - 1 positions", (long long)max_blocks,
+                     (long long)block_size);
   if (T > 0 && (req_id == nullptr || (max_blocks > 0 && block_table == nullptr)))
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "req_id and block_table are required");
   return FP8MLA_OK;
@@ -211,7 +212,7 @@ int fp8mla_fp4_gather(const uint8_t* kv, int64_t num_slots, const int32_t* block
                       const int32_t* seq_starts, int64_t n, uint16_t* out, int64_t out_stride, void* stream) {
   clear_error();
   if (n < 0 || num_slots < 0 || B < 0 || B > INT32_MAX || out_stride < kDqk || block_size <= 0 ||
-      block_size > (1 << 20) || max_blocks < 0 || bt_stride < max_blocks)
+      block_size > (1 << 20) || max_blocks < 0 || max_blocks > INT32_MAX || bt_stride < max_blocks)
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "bad gather sizes or strides");
   if (n == 0 || B == 0) return FP8MLA_OK;
   if ((num_slots > 0 && kv == nullptr) || cu_seq_lens == nullptr || out == nullptr ||

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kBlock) fp4_gather_kernel(
   const int lane = threadIdx.x & 31;
   const bool sectors = whole_sectors(out, out_stride);
   const int64_t step = (int64_t)gridDim.x * kWarps * kRun;
-  const int64_t max_pos = max_blocks * block_size;  // below 2^31
+  const int64_t max_pos = max_blocks * block_size;
   const int first = cu[0], last = cu[B];
   for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + threadIdx.x / 32) * kRun; r0 < n && r0 < last; r0 += step) {
     if (r0 + kRun <= first) continue;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kBlock) fp4_gather_kernel(
       while (r >= cu[b + 1]) ++b;
       slot = -1;
       const int64_t p = r - cu[b] + (starts != nullptr ? starts[b] : 0);
-      if (p >= 0 && p < max_pos) {
+      if (p >= 0 && p < max_pos) {  // (below 2^32: a row of the sequence plus its start)
         const int64_t blk = (uint32_t)p / (uint32_t)block_size;
         const int64_t s = (int64_t)block_table[b * bt_stride + blk] * block_size + (p - blk * block_size);
         if (s >= 0 && s < num_slots) slot = s;

@@ -20,10 +20,9 @@ __device__ __forceinline__ int chunks_of(int entries) {
   return entries > kChunk ? (entries + kChunk - 1) / kChunk : 1;
 }
 
-// u / d: nearly always in 32 bits (a 64-bit division is 1.6 KB of code).
-__device__ __forceinline__ int64_t quotient64(int64_t u, int d) { return u / d; }
+// u / d: nearly always in 32 bits.
 __device__ __forceinline__ int64_t quotient(int64_t u, int d) {
-  return (u >> 32) == 0 ? (int64_t)((uint32_t)u / (uint32_t)d) : quotient64(u, d);
+  return (u >> 32) == 0 ? (int64_t)((uint32_t)u / (uint32_t)d) : u / d;
 }
 
 struct Share {  // in shared memory: one worker's share of the chunk list
@@ -142,14 +141,14 @@ __device__ __forceinline__ void note_start(const Fp4DecodeArgs& a, const Share& 
   info[3] = s.per;
 }
 
-__device__ __forceinline__ int32_t block_by_division(int32_t v, int32_t block_size) { return v / block_size; }
 __device__ __forceinline__ int32_t block_of(const Fp4DecodeArgs& a, int32_t v) {
-  return a.block_shift >= 0 ? (v >> a.block_shift) : block_by_division(v, a.block_size);
+  return a.block_shift >= 0 ? (v >> a.block_shift) : v / a.block_size;
 }
 // Block-table word of an entry (0 without a table), and the entry's slot given
 // that word; -1: masked, behind the table, or outside the pool.
 __device__ __forceinline__ int32_t table_word(const Fp4DecodeArgs& a, int32_t req, int32_t v) {
   if (a.block_table == nullptr || v < 0) return 0;
+  if (req < 0) return -1;  // a padding token
   const int32_t blk = block_of(a, v);
   return blk < a.max_blocks ? a.block_table[(int64_t)req * a.bt_stride + blk] : -1;
 }

@@ -56,7 +56,8 @@ def _int64(t: torch.Tensor) -> torch.Tensor:
 def concat_and_cache_fp4_ds_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
                                 slot_mapping: torch.Tensor) -> None:
     """Quantize kv_c [N, 512] and k_pe [N, 64] (bf16) into the kv_cache [..., 416]
-    rows that slot_mapping [N] names; slots below 0 or behind the pool are skipped."""
+    rows that slot_mapping [N] names; slots below 0 or behind the pool are skipped.
+    A slot must not be named twice (its row could hold parts of both tokens)."""
     assert kv_c.dtype == torch.bfloat16 and k_pe.dtype == torch.bfloat16, "bf16 latent/rope"
     assert kv_c.dim() == 2 and kv_c.shape[1] == NOPE and kv_c.stride(1) == 1
     assert k_pe.dim() == 2 and k_pe.shape[1] == ROPE and k_pe.stride(1) == 1
@@ -157,10 +158,12 @@ def _prepare(q, kv_cache, groups, topk, return_lse, workspace, *others):
     assert H % groups == 0, f"h_q={H} not divisible by kv_groups={groups}"
     dev = N.require_cuda(q, kv_cache, workspace, *others)
     # the kernels read q in 16-byte vectors; re-lay a misaligned view once
-    if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+    # (a dimension of one token or head may have any stride, and contiguous() keeps it)
+    if q.data_ptr() % 16 or (q.stride(0) % 8 and T > 1) or (q.stride(1) % 8 and H > 1):
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
+    q_strides = (q.stride(0) if T > 1 else H * (NOPE + ROPE), q.stride(1) if H > 1 else NOPE + ROPE)
     out = q.new_empty((T, H, NOPE))
     lse = q.new_empty((T, H), dtype=torch.float32) if return_lse else None
     need = N.lib().fp8mla_fp4_workspace_bytes(T, H, groups, topk)
@@ -171,7 +174,7 @@ def _prepare(q, kv_cache, groups, topk, return_lse, workspace, *others):
     if workspace is None and need:
         workspace = q.new_empty((need,), dtype=torch.uint8)
     ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
-    return q, num_slots, out, lse, (lse.data_ptr(), H) if return_lse else (None, 0), ws, workspace, dev
+    return q, q_strides, num_slots, out, lse, (lse.data_ptr(), H) if return_lse else (None, 0), ws, workspace, dev
 
 
 def _check_table(req_id, block_table, T, block_size):
@@ -211,10 +214,11 @@ def fp4_ds_mla_sparse_decode(
     indices = _with_groups(indices)
     G, topk = indices.shape[1], indices.shape[2]
     assert indices.shape[0] == q.shape[0], "one index row per query token"
-    q, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace, indices)
+    q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace,
+                                                                        indices)
     with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_sparse_decode(
-            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv_cache.data_ptr(), num_slots,
+            q.data_ptr(), q.shape[0], q.shape[1], *q_strides, kv_cache.data_ptr(), num_slots,
             indices.data_ptr(), G, topk, indices.stride(0), indices.stride(1), float(sm_scale),
             out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
     N.check(rc, "fp4_ds_mla_sparse_decode")
@@ -234,17 +238,17 @@ def fp4_ds_mla_sparse_decode_paged(
     workspace: torch.Tensor | None = None,
 ):
     """``fp4_ds_mla_sparse_decode`` over request-local token positions: the
-    block-table conversion runs inside the gather (positions behind the table
-    are masked)."""
+    block-table conversion runs inside the gather (positions behind the table,
+    and all of a token with a negative req_id, are masked)."""
     token_indices = _with_groups(token_indices)
     G, topk = token_indices.shape[1], token_indices.shape[2]
     assert token_indices.shape[0] == q.shape[0], "one index row per query token"
     bt_stride = _check_table(req_id, block_table, q.shape[0], block_size)
-    q, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace, token_indices, req_id,
-                                                             block_table)
+    q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace,
+                                                                        token_indices, req_id, block_table)
     with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_sparse_decode_paged(
-            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv_cache.data_ptr(), num_slots,
+            q.data_ptr(), q.shape[0], q.shape[1], *q_strides, kv_cache.data_ptr(), num_slots,
             req_id.data_ptr(), block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
             token_indices.data_ptr(), G, topk, token_indices.stride(0), token_indices.stride(1), float(sm_scale),
             out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
@@ -265,7 +269,8 @@ def fp4_ds_mla_decode(
     workspace: torch.Tensor | None = None,
 ):
     """MLA attention of each query token over the first ``context_lens[t]``
-    positions of its request (at most max_blocks * block_size).
+    positions of its request (at most max_blocks * block_size; none where req_id
+    is negative, as in a padded batch).
 
     With several query tokens of one request (drafts, a prefill chunk) each
     token's own length makes the attention causal.  Lengths are read on the
@@ -274,11 +279,11 @@ def fp4_ds_mla_decode(
     assert context_lens.dtype == torch.int32 and context_lens.dim() == 1 and context_lens.is_contiguous()
     assert context_lens.shape[0] == q.shape[0], "one context length per query token"
     bt_stride = _check_table(req_id, block_table, q.shape[0], block_size)
-    q, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, 1, -1, return_lse, workspace, context_lens, req_id,
-                                                             block_table)
+    q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, 1, -1, return_lse, workspace,
+                                                                        context_lens, req_id, block_table)
     with N.on_device(dev):
         rc = N.lib().fp8mla_fp4_decode(
-            q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), kv_cache.data_ptr(), num_slots,
+            q.data_ptr(), q.shape[0], q.shape[1], *q_strides, kv_cache.data_ptr(), num_slots,
             req_id.data_ptr(), block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
             context_lens.data_ptr(), float(sm_scale),
             out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
