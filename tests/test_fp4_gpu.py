@@ -526,6 +526,49 @@ def test_graph_serves_new_lengths_and_tokens(H):
         R.check(got, R.attend(q, pool, dense_slots(table, req, lens, 64), SCALE))
 
 
+@pytest.mark.parametrize("H", [16, 128])
+def test_two_graphs_share_a_workspace(H):
+    """Nothing in the workspace outlives a call: graphs of different sizes replay in
+    turn over one."""
+    pool = make_pool(95, 3000)
+    cases = [sparse_case(96, 9, H, 1500, 3000, mask=0.1), sparse_case(97, 31, H, 700, 3000, mask=0.1)]
+    ws = torch.full((F.fp4_workspace_bytes(31, H),), 0xFF, dtype=torch.uint8, device="cuda")
+    want = [F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True) for q, idx in cases]
+    graphs, outs = [], []
+    for q, idx in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE, return_lse=True, workspace=ws))
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 1, 0):
+        outs[i][0].zero_()
+        graphs[i].replay()
+        assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
+
+
+@pytest.mark.parametrize("H", [16, 128])
+def test_calls_in_a_row_see_each_other(H):
+    """Launched without a pause, so that each kernel is on the SMs before the one in
+    front of it is done: rows that are written anew between reads of them."""
+    n, times = 256, 40
+    pool = make_pool(90, 640)
+    slots = torch.randperm(640, device="cuda")[:n]
+    idx = slots.to(torch.int32).view(1, n).repeat(40, 1)
+    q = randn(92, 40, H, 576)
+    kv_c, k_pe = randn(93, times, n, 512), randn(94, times, n, 64)
+    torch.cuda.synchronize()
+    got = []
+    for i in range(times):
+        F.concat_and_cache_fp4_ds_mla(kv_c[i], k_pe[i], pool, slots)
+        got.append((F.dequant_fp4_ds_mla_rows(pool, slots), F.fp4_ds_mla_sparse_decode(q, pool, idx, SCALE)))
+    for i in range(times):
+        rows = R.quantize(kv_c[i], k_pe[i])
+        assert torch.equal(got[i][0].double(), R.values(rows)), i
+        fresh = F.fp4_ds_mla_sparse_decode(q, rows, torch.arange(n, dtype=torch.int32, device="cuda").repeat(40, 1),
+                                           SCALE)
+        assert torch.equal(got[i][1], fresh), i
+
+
 def test_a_request_from_prompt_to_answer():
     """Together, as a server runs them: a prompt is written in two chunks, its
     cached part read back for prefill attention, then tokens are decoded, all

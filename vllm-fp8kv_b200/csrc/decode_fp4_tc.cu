@@ -312,7 +312,7 @@ __device__ void scout(const Ctx& c, int lane) {
 // in the order s ^ (q & 2).  With the swizzle of the row, eight lanes then touch every
 // bank once.
 __device__ __forceinline__ void load32(uint4 (&w)[2], const uint8_t* at) {
-  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
                : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y), "=r"(w[1].z),
                  "=r"(w[1].w)
                : "l"(at));

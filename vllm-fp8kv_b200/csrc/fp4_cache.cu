@@ -14,6 +14,9 @@ namespace fp8mla {
 namespace {
 using namespace fp8mla::fp4;
 
+// The kernels may start before the one in front of them is done (pdl_wait), so no
+// pointer is __restrict__: loads that the compiler takes for reads of constant
+// memory may be moved in front of the wait, or be served from before it.
 constexpr int kBlock = 256;
 constexpr int kWarps = kBlock / 32;
 
@@ -65,9 +68,9 @@ __device__ __forceinline__ uint4 load8(const uint16_t* r) {
 // the warps 19.0).
 template <bool kVec>
 __global__ void __launch_bounds__(kBlock, kVec ? 8 : 4) fp4_write_kernel(
-    const uint16_t* __restrict__ kv_c, int64_t kv_c_stride, const uint16_t* __restrict__ k_pe,
-    int64_t k_pe_stride, const int64_t* __restrict__ slot_mapping, int64_t N,
-    uint8_t* __restrict__ cache, int64_t num_slots) {
+    const uint16_t* kv_c, int64_t kv_c_stride, const uint16_t* k_pe,
+    int64_t k_pe_stride, const int64_t* slot_mapping, int64_t N,
+    uint8_t* cache, int64_t num_slots) {
   if (threadIdx.x == 0) pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -114,7 +117,7 @@ struct RowIn {
   uint32_t scale;
   uint4 rope;
 };
-__device__ __forceinline__ void row_load(RowIn& in, const uint8_t* __restrict__ kv, int64_t slot, int lane) {
+__device__ __forceinline__ void row_load(RowIn& in, const uint8_t* kv, int64_t slot, int lane) {
   if (slot >= 0) {
     const uint8_t* row = kv + slot * (int64_t)kFp4RowBytes;
     in.codes = reinterpret_cast<const uint2*>(row)[lane];
@@ -130,7 +133,7 @@ __device__ __forceinline__ void row_load(RowIn& in, const uint8_t* __restrict__ 
 __device__ __forceinline__ bool whole_sectors(const uint16_t* out, int64_t out_stride) {
   return out_stride % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0;
 }
-__device__ __forceinline__ void row_store(const RowIn& in, uint16_t* __restrict__ dst, int lane, bool sectors) {
+__device__ __forceinline__ void row_store(const RowIn& in, uint16_t* dst, int lane, bool sectors) {
   const uint32_t s = bf16_scale(in.scale);
   uint32_t a[4], b[4];
   e2m1x8_to_f16(in.codes.x, a);
@@ -154,9 +157,9 @@ __device__ __forceinline__ void row_store(const RowIn& in, uint16_t* __restrict_
 
 // A row a warp: 32 registers, so all of an SM's warps are resident, each with one
 // row in flight (17.3 us for 65536 rows; 20.8 with two rows a step, 22.1 with four).
-__global__ void __launch_bounds__(kBlock, 8) fp4_rows_kernel(const uint8_t* __restrict__ kv, int64_t num_slots,
-                                                          const int64_t* __restrict__ slots, int64_t n,
-                                                          uint16_t* __restrict__ out, int64_t out_stride) {
+__global__ void __launch_bounds__(kBlock, 8) fp4_rows_kernel(const uint8_t* kv, int64_t num_slots,
+                                                          const int64_t* slots, int64_t n,
+                                                          uint16_t* out, int64_t out_stride) {
   if (threadIdx.x == 0) pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(kBlock, 8) fp4_rows_kernel(const uint8_t* __re
 
 // Sequence b with cu[b] <= r < cu[b + 1] (-1 if there is none): a warp looks at
 // 32 evenly spaced entries at a time, so 1024 sequences take two rounds.
-__device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int B, int64_t r, int lane) {
+__device__ __forceinline__ int sequence_of(const int32_t* cu, int B, int64_t r, int lane) {
   int lo = 0, n = B;  // the answer, if any, is in [lo, lo + n)
   if (r < cu[0] || r >= cu[B]) return -1;
   while (n > 1) {
@@ -192,9 +195,9 @@ __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int B
 constexpr int kRun = 4;
 
 __global__ void __launch_bounds__(kBlock) fp4_gather_kernel(
-    const uint8_t* __restrict__ kv, int64_t num_slots, const int32_t* __restrict__ block_table,
-    int64_t bt_stride, int64_t max_blocks, int block_size, const int32_t* __restrict__ cu, int B,
-    const int32_t* __restrict__ starts, int64_t n, uint16_t* __restrict__ out, int64_t out_stride) {
+    const uint8_t* kv, int64_t num_slots, const int32_t* block_table,
+    int64_t bt_stride, int64_t max_blocks, int block_size, const int32_t* cu, int B,
+    const int32_t* starts, int64_t n, uint16_t* out, int64_t out_stride) {
   if (threadIdx.x == 0) pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
