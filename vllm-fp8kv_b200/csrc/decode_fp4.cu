@@ -142,11 +142,15 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
   bool ok = true;
   int64_t armed = 0;
   Ring ring;
+  int32_t early[2][1];
+  slots.start(a, early);
 #pragma unroll 1
-  for (int64_t g = -2 * slots.kAhead; g < chunks && ok; g += 2) {
+  for (int64_t g = 0; g < chunks && ok; g += 2) {
     int32_t at[1];
-    slots.next(a, at);
-    if (g < 0) continue;
+    if (g >= 4)
+      slots.next(a, at, g == 4);
+    else
+      at[0] = early[g >> 1][0];
     const int32_t slot = at[0];
     const uint32_t live2 = __ballot_sync(0xFFFFFFFFu, slot >= 0);
 #pragma unroll

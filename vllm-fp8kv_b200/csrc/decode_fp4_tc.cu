@@ -275,12 +275,21 @@ __device__ void scout(const Ctx& c, int lane) {
   const Fp4DecodeArgs& a = *c.a;
   Smem& s = *c.s;
   Slots<kN, 1, 4> slots(a, s.share, c.worker, lane, 0);
+  int32_t early[2][4];
+  slots.start(a, early);
   const int tiles = (int)c.tiles;
 #pragma unroll 1
-  for (int j = -slots.kAhead; j < tiles; ++j) {
+  for (int j = 0; j < tiles; ++j) {
     int32_t slot[4];
-    slots.next(a, slot);
-    if (j < 0) continue;
+    if (j >= 2) {
+      slots.next(a, slot, j == 2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        slot[i] = early[0][i];
+        early[0][i] = early[1][i];
+      }
+    }
     const int r = j % kScoutRing;
     if (j >= kScoutRing && !wait<1>(s.slots_empty[r], (uint32_t)(j / kScoutRing + 1) & 1, 40)) break;
 #pragma unroll

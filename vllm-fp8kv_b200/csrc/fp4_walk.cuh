@@ -195,9 +195,7 @@ struct Slots {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) p[i] = table_word(a, r, e[i]);
   }
-  // of chunks first, first + kStride, ... of the run; the first kAhead calls of
-  // next() only fill the pipeline
-  static constexpr int kAhead = 3;
+  // of chunks first, first + kStride, ... of the run
   __device__ __forceinline__ Slots(const Fp4DecodeArgs& a, const Share& s, int worker, int row_, int first)
       : ahead(a, s, worker), row(row_) {
     at_unit(a);
@@ -209,7 +207,31 @@ struct Slots {
     }
     rq[0] = rq[1] = rq[2] = 0;
   }
-  __device__ __forceinline__ void next(const Fp4DecodeArgs& a, int32_t (&slot)[kRows]) {
+  // The first kN steps, in one pass: two latencies.  (In next() the loads of a step
+  // are waited for when its registers move up, which is one latency a call.)
+  template <int kN>
+  __device__ __forceinline__ void start(const Fp4DecodeArgs& a, int32_t (&slot)[kN][kRows]) {
+    int32_t e[kN][kRows], p[kN][kRows], r[kN];
+#pragma unroll
+    for (int x = 0; x < kN; ++x) {
+      fetch(a, e[x]);
+      r[x] = req;
+#pragma unroll
+      for (int k = 0; k < kStride; ++k) step(a);
+    }
+#pragma unroll
+    for (int x = 0; x < kN; ++x) words(a, r[x], e[x], p[x]);
+#pragma unroll
+    for (int x = 0; x < kN; ++x)
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) slot[x][i] = slot_of(a, e[x][i], p[x][i]);
+  }
+  // The next step; the first call after start() fills the pipeline.
+  __device__ __forceinline__ void next(const Fp4DecodeArgs& a, int32_t (&slot)[kRows], bool fill) {
+#pragma unroll 1
+    for (int k = fill ? 0 : 3; k < 4; ++k) shift(a, slot);
+  }
+  __device__ __forceinline__ void shift(const Fp4DecodeArgs& a, int32_t (&slot)[kRows]) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       slot[i] = slot_of(a, v[0][i], pg[0][i]);
