@@ -17,7 +17,7 @@ __device__ __forceinline__ int entries_of(const Fp4DecodeArgs& a, int64_t t) {
 }
 template <int kChunk>
 __device__ __forceinline__ int chunks_of(int entries) {
-  return entries > kChunk ? (entries + kChunk - 1) / kChunk : 1;
+  return entries > kChunk ? (entries - 1) / kChunk + 1 : 1;  // (entries go up to 2^31 - 1)
 }
 
 // u / d: nearly always in 32 bits.
@@ -163,8 +163,8 @@ __device__ __forceinline__ int32_t slot_of(const Fp4DecodeArgs& a, int32_t v, in
 }
 
 // The slots of rows row, row + 32, .. (kRows of them) of every `kStride`-th chunk
-// of a worker's run, entries read three steps ahead of their use and block-table
-// words two steps ahead, so that neither latency is waited for.
+// of a worker's run: entries are read three steps ahead of their use and block-table
+// words two, so that a step waits for what is left of one latency.
 template <int kChunk, int kStride, int kRows>
 struct Slots {
   Walk<kChunk> ahead;
