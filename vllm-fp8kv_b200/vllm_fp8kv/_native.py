@@ -6,7 +6,6 @@ library is missing or the device is not sm_100, the call raises.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -136,17 +135,6 @@ def stream_ptr(device) -> int:
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
-
-
-_HERE_ALREADY = contextlib.nullcontext()
-
-
-def on_device(device):
-    """``torch.cuda.device(device)``, or nothing where it is current already
-    (entering the context costs more than the look)."""
-    import torch
-
-    return _HERE_ALREADY if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def raw_stream(device) -> int:

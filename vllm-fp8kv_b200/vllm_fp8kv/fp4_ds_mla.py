@@ -49,6 +49,19 @@ def _pool(kv_cache: torch.Tensor) -> int:
     return kv_cache.numel() // ROW_BYTES
 
 
+def _launch(what: str, fn: str, dev, *args) -> None:
+    """Calls C entry `fn` on the tensors' device and its current stream (entering
+    the device's context, where it is current already, costs more than the look)."""
+    call = getattr(N.lib(), fn)
+    if torch.cuda.current_device() == dev.index:
+        rc = call(*args, N.raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = call(*args, N.raw_stream(dev))
+    if rc:
+        N.check(rc, what)
+
+
 def _int64(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
@@ -69,15 +82,13 @@ def concat_and_cache_fp4_ds_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache
     st_pe = k_pe.stride(0) if k_pe.shape[0] > 1 else ROPE
     assert st_c >= NOPE and st_pe >= ROPE, "token rows must not overlap"
     slots = _int64(slot_mapping)
-    with N.on_device(dev):
-        rc = N.lib().fp8mla_fp4_write(kv_c.data_ptr(), st_c, k_pe.data_ptr(), st_pe, slots.data_ptr(),
-                                      slots.shape[0], kv_cache.data_ptr(), num_slots, N.raw_stream(dev))
-    N.check(rc, "concat_and_cache_fp4_ds_mla")
+    _launch("concat_and_cache_fp4_ds_mla", "fp8mla_fp4_write", dev, kv_c.data_ptr(), st_c, k_pe.data_ptr(), st_pe,
+            slots.data_ptr(), slots.shape[0], kv_cache.data_ptr(), num_slots)
 
 
-def _check_out(out: torch.Tensor | None, n: int, dev) -> torch.Tensor:
+def _check_out(out: torch.Tensor | None, n: int, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty((n, NOPE + ROPE), dtype=torch.bfloat16, device=dev)
+        return like.new_empty((n, NOPE + ROPE), dtype=torch.bfloat16)
     assert out.dtype == torch.bfloat16 and out.dim() == 2 and out.shape == (n, NOPE + ROPE) and out.stride(1) == 1, \
         f"out must be bf16 [{n}, {NOPE + ROPE}] with unit last stride"
     return out
@@ -95,11 +106,9 @@ def dequant_fp4_ds_mla_rows(kv_cache: torch.Tensor, slots: torch.Tensor,
     assert slots.dim() == 1 and slots.dtype in (torch.int32, torch.int64), "slots must be int32 or int64 [n]"
     dev = N.require_cuda(kv_cache, slots, out)
     sl = _int64(slots)
-    out = _check_out(out, sl.numel(), dev)
-    with N.on_device(dev):
-        rc = N.lib().fp8mla_fp4_dequant_rows(kv_cache.data_ptr(), num_slots, sl.data_ptr(), sl.numel(), out.data_ptr(),
-                                             _row_stride(out), N.raw_stream(dev))
-    N.check(rc, "dequant_fp4_ds_mla_rows")
+    out = _check_out(out, sl.numel(), kv_cache)
+    _launch("dequant_fp4_ds_mla_rows", "fp8mla_fp4_dequant_rows", dev, kv_cache.data_ptr(), num_slots,
+            sl.data_ptr(), sl.numel(), out.data_ptr(), _row_stride(out))
     return out
 
 
@@ -123,15 +132,12 @@ def gather_fp4_ds_mla(kv_cache: torch.Tensor, block_table: torch.Tensor, cu_seq_
                                   and seq_starts.is_contiguous()), "seq_starts must be contiguous int32 [B]"
     assert block_size > 0 and num_tokens >= 0
     dev = N.require_cuda(kv_cache, block_table, cu_seq_lens, seq_starts, out)
-    out = _check_out(out, num_tokens, dev)
+    out = _check_out(out, num_tokens, kv_cache)
     bt_stride = block_table.stride(0) if B > 1 else block_table.shape[1]
     assert bt_stride >= block_table.shape[1], "block_table rows must not overlap"
-    with N.on_device(dev):
-        rc = N.lib().fp8mla_fp4_gather(
-            kv_cache.data_ptr(), num_slots, block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
-            cu_seq_lens.data_ptr(), B, seq_starts.data_ptr() if seq_starts is not None else None, num_tokens,
-            out.data_ptr(), _row_stride(out), N.raw_stream(dev))
-    N.check(rc, "gather_fp4_ds_mla")
+    _launch("gather_fp4_ds_mla", "fp8mla_fp4_gather", dev, kv_cache.data_ptr(), num_slots, block_table.data_ptr(),
+            bt_stride, block_table.shape[1], int(block_size), cu_seq_lens.data_ptr(), B, seq_starts.data_ptr() if
+            seq_starts is not None else None, num_tokens, out.data_ptr(), _row_stride(out))
     return out
 
 
@@ -159,11 +165,13 @@ def _prepare(q, kv_cache, groups, topk, return_lse, workspace, *others):
     dev = N.require_cuda(q, kv_cache, workspace, *others)
     # the kernels read q in 16-byte vectors; re-lay a misaligned view once
     # (a dimension of one token or head may have any stride, and contiguous() keeps it)
-    if q.data_ptr() % 16 or (q.stride(0) % 8 and T > 1) or (q.stride(1) % 8 and H > 1):
+    st, sh, _ = q.stride()
+    if q.data_ptr() % 16 or (st % 8 and T > 1) or (sh % 8 and H > 1):
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-    q_strides = (q.stride(0) if T > 1 else H * (NOPE + ROPE), q.stride(1) if H > 1 else NOPE + ROPE)
+        st, sh, _ = q.stride()
+    q_strides = (st if T > 1 else H * (NOPE + ROPE), sh if H > 1 else NOPE + ROPE)
     out = q.new_empty((T, H, NOPE))
     lse = q.new_empty((T, H), dtype=torch.float32) if return_lse else None
     need = N.lib().fp8mla_fp4_workspace_bytes(T, H, groups, topk)
@@ -174,7 +182,7 @@ def _prepare(q, kv_cache, groups, topk, return_lse, workspace, *others):
     if workspace is None and need:
         workspace = q.new_empty((need,), dtype=torch.uint8)
     ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
-    return q, q_strides, num_slots, out, lse, (lse.data_ptr(), H) if return_lse else (None, 0), ws, workspace, dev
+    return T, H, q, q_strides, num_slots, out, lse, (lse.data_ptr(), H) if return_lse else (None, 0), ws, workspace, dev
 
 
 def _check_table(req_id, block_table, T, block_size):
@@ -214,14 +222,11 @@ def fp4_ds_mla_sparse_decode(
     indices = _with_groups(indices)
     G, topk = indices.shape[1], indices.shape[2]
     assert indices.shape[0] == q.shape[0], "one index row per query token"
-    q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace,
-                                                                        indices)
-    with N.on_device(dev):
-        rc = N.lib().fp8mla_fp4_sparse_decode(
-            q.data_ptr(), q.shape[0], q.shape[1], *q_strides, kv_cache.data_ptr(), num_slots,
-            indices.data_ptr(), G, topk, indices.stride(0), indices.stride(1), float(sm_scale),
-            out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
-    N.check(rc, "fp4_ds_mla_sparse_decode")
+    T, H, q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(
+        q, kv_cache, G, topk, return_lse, workspace, indices)
+    _launch("fp4_ds_mla_sparse_decode", "fp8mla_fp4_sparse_decode", dev, q.data_ptr(), T, H, *q_strides,
+            kv_cache.data_ptr(), num_slots, indices.data_ptr(), G, topk, indices.stride(0), indices.stride(1),
+            float(sm_scale), out.data_ptr(), H * NOPE, NOPE, *lse_at, *ws)
     return (out, lse) if return_lse else out
 
 
@@ -244,15 +249,12 @@ def fp4_ds_mla_sparse_decode_paged(
     G, topk = token_indices.shape[1], token_indices.shape[2]
     assert token_indices.shape[0] == q.shape[0], "one index row per query token"
     bt_stride = _check_table(req_id, block_table, q.shape[0], block_size)
-    q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, G, topk, return_lse, workspace,
-                                                                        token_indices, req_id, block_table)
-    with N.on_device(dev):
-        rc = N.lib().fp8mla_fp4_sparse_decode_paged(
-            q.data_ptr(), q.shape[0], q.shape[1], *q_strides, kv_cache.data_ptr(), num_slots,
-            req_id.data_ptr(), block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
-            token_indices.data_ptr(), G, topk, token_indices.stride(0), token_indices.stride(1), float(sm_scale),
-            out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
-    N.check(rc, "fp4_ds_mla_sparse_decode_paged")
+    T, H, q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(
+        q, kv_cache, G, topk, return_lse, workspace, token_indices, req_id, block_table)
+    _launch("fp4_ds_mla_sparse_decode_paged", "fp8mla_fp4_sparse_decode_paged", dev, q.data_ptr(), T, H, *q_strides,
+            kv_cache.data_ptr(), num_slots, req_id.data_ptr(), block_table.data_ptr(), bt_stride,
+            block_table.shape[1], int(block_size), token_indices.data_ptr(), G, topk, token_indices.stride(0),
+            token_indices.stride(1), float(sm_scale), out.data_ptr(), H * NOPE, NOPE, *lse_at, *ws)
     return (out, lse) if return_lse else out
 
 
@@ -279,13 +281,9 @@ def fp4_ds_mla_decode(
     assert context_lens.dtype == torch.int32 and context_lens.dim() == 1 and context_lens.is_contiguous()
     assert context_lens.shape[0] == q.shape[0], "one context length per query token"
     bt_stride = _check_table(req_id, block_table, q.shape[0], block_size)
-    q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(q, kv_cache, 1, -1, return_lse, workspace,
-                                                                        context_lens, req_id, block_table)
-    with N.on_device(dev):
-        rc = N.lib().fp8mla_fp4_decode(
-            q.data_ptr(), q.shape[0], q.shape[1], *q_strides, kv_cache.data_ptr(), num_slots,
-            req_id.data_ptr(), block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
-            context_lens.data_ptr(), float(sm_scale),
-            out.data_ptr(), out.stride(0), out.stride(1), *lse_at, *ws, N.raw_stream(dev))
-    N.check(rc, "fp4_ds_mla_decode")
+    T, H, q, q_strides, num_slots, out, lse, lse_at, ws, hold, dev = _prepare(
+        q, kv_cache, 1, -1, return_lse, workspace, context_lens, req_id, block_table)
+    _launch("fp4_ds_mla_decode", "fp8mla_fp4_decode", dev, q.data_ptr(), T, H, *q_strides, kv_cache.data_ptr(),
+            num_slots, req_id.data_ptr(), block_table.data_ptr(), bt_stride, block_table.shape[1], int(block_size),
+            context_lens.data_ptr(), float(sm_scale), out.data_ptr(), H * NOPE, NOPE, *lse_at, *ws)
     return (out, lse) if return_lse else out
