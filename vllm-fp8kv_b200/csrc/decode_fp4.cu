@@ -27,8 +27,8 @@
 // and spilling them made it three times slower.)
 //
 // Measured, us: 256 x 16 heads x top-2048 88.7 (two units on each of 128 SMs, 39% of
-// a plain copy's rate); 64 x 16 heads over up to 16384 positions 87.0; 4 x 16 heads x
-// top-256 10.8.  A chunk takes 2650 cycles of an SM, in which its MMAs take 1090, the
+// a plain copy's rate); 64 x 16 heads over up to 16384 positions 85.6; 4 x 16 heads x
+// top-256 10.7.  A chunk takes 2650 cycles of an SM, in which its MMAs take 1090, the
 // conversions 1020 and the issue slots of its 86 instructions a row 1440: no pipe
 // is full, and there are no registers for a fourth group.  Steps on the way:
 // 150 with warps that did S and warps that did O, 126 with warps that do both, 92 in

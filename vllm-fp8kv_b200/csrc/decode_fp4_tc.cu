@@ -18,7 +18,7 @@
 // next tile while the other group and the O product of the tile before are still
 // running; V while the next tile's S runs.
 //
-// Measured, us: 64 x 128 heads x top-2048, paged: 55.3 (16 tiles a pair); its
+// Measured, us: 64 x 128 heads x top-2048, paged: 54.6 (16 tiles a pair); its
 // products take 22.5 at the rate of a large matrix product, its rows' bytes 8.3.
 // A tile takes 4400 cycles.  What bounds it is the traffic of shared memory, about 3000
 // cycles of it: K and V written (136 KB), read by the MMAs (192 KB), P, and the rows'
