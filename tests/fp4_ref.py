@@ -54,7 +54,11 @@ def attend(q, pool, slots, sm_scale, G=1):
     rounded to fp16 (2^-11).  So each weight is off by e = 2^-11 + d relative with
     d = A (576 * 2^-23 + 2^-20) + 2^-20, the output by (e + d) * sum p |v| / l
     (numerator and sum) plus its own bf16 rounding 2^-8 |out|, the lse by d plus
-    its fp32 arithmetic 2^-20 (1 + |lse|)."""
+    its fp32 arithmetic 2^-20 (1 + |lse|).  P is stored times 2^6, so a weight
+    below fp16's normal range (2^-20 of the largest) is off by up to half its
+    smallest step, 2^-25 2^-6 = 2^-31 of the largest weight, instead of 2^-11 of
+    itself.  The reference maximum is never above the largest score met, so the
+    sum is at least the weight 1 that this is relative to: 2^-31 sum |v| more."""
     T, H, _ = q.shape
     out = torch.zeros(T, H, 512, dtype=torch.float64, device=q.device)
     lse = torch.full((T, H), float("-inf"), dtype=torch.float64, device=q.device)
@@ -77,6 +81,7 @@ def attend(q, pool, slots, sm_scale, G=1):
             d = a * (576 * 2.0 ** -23 + 2.0 ** -20) + 2.0 ** -20
             tol_l[t, hs] = d + 2.0 ** -20 * (1 + lse[t, hs].abs())
             tol_o[t, hs] = (2.0 ** -11 + 2 * d)[:, None] * (p @ k[:, :512].abs()) + 2.0 ** -8 * out[t, hs].abs()
+            tol_o[t, hs] += 2.0 ** -31 * k[:, :512].abs().sum(0)
     return out, lse, tol_o, tol_l
 
 

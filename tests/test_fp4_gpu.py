@@ -312,6 +312,17 @@ def test_scores_of_any_size(H):
 
 
 @pytest.mark.parametrize("H", [16, 128])
+@pytest.mark.parametrize("size", [30.0, 1e-3])
+def test_peaked_and_flat_rows(H, size):
+    """Scores of hundreds, where one entry takes nearly all the weight and the others'
+    lies below what P can hold, and scores that are nearly the same."""
+    pool = make_pool(48, 900)
+    q, idx = sparse_case(49, 9, H, 700, 900, mask=0.1)
+    q = q * size
+    check_sparse(q, pool, idx, R.attend(q, pool, idx, SCALE))
+
+
+@pytest.mark.parametrize("H", [16, 128])
 @pytest.mark.parametrize("scale", [-0.07, 0.0, -0.0])
 def test_softmax_scale_of_any_sign(H, scale):
     """A negative scale turns the order of the scores round; with 0 all live

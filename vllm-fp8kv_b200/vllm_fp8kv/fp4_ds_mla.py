@@ -23,7 +23,9 @@ reads back as NaN.
 * ``fp4_ds_mla_decode``               attention over whole contexts
 
 The attention takes bf16 q only: the latents enter the tensor cores exactly (as
-fp16, beside q scaled by a power of two), P in fp16, sums in fp32.  All calls
+fp16, beside q scaled by a power of two), the softmax's weights in fp16 (11 bits;
+below 2^-20 of a row's largest with an error of up to 2^-31 of it, so that those
+below 2^-31 count as 0), sums in fp32.  All calls
 run on the current stream of the tensors' device and never synchronise.
 """
 
