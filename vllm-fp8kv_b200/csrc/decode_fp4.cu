@@ -7,9 +7,10 @@
 // registers, straight into mma.sync fragments: a bf16 copy of a row in shared
 // memory would cost 1152 bytes written and twice read against 416 read twice.
 //   * latents are exact in fp16 (fp4.cuh), so the latent products are fp16
-//     MMAs: q is scaled per head by a power of two to a largest value in
-//     [2^8, 2^9) and converted (exact down to 2^-22 of that value, below it an
-//     error under 2^-33 of it), and P keeps 11 bits where bf16 keeps 8;
+//     MMAs: q is scaled per head by a power of two (q_power), to a largest value in
+//     [2^8, 2^9) where the softmax scale is of ordinary size, and converted (exact
+//     down to 2^-25 of that value, below it an error under 2^-33 of it), and P keeps
+//     11 bits where bf16 keeps 8;
 //   * the rope (bf16 as stored) and q's rope (times the same power of two)
 //     go through bf16 MMAs into the same accumulators.
 //
@@ -228,12 +229,7 @@ __device__ void load_q(const Fp4DecodeArgs& a, Smem& s, const Walk<kBN>& x, int 
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     mr = max(mr, __shfl_xor_sync(0xFFFFFFFFu, mr, o));
   }
-  // 2^k brings the latent part's largest value to [2^8, 2^9), but the rope's
-  // at most to 2^101, where its products are still finite; 1 for rows of
-  // zeros, inf or NaN.  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are
-  // normal.
-  int k = min(8 - ((int)(m >> 7) - 127), 100 - ((int)(mr >> 7) - 127));
-  k = (m == 0 || m >= 0x7F80u) ? 0 : min(126, k);
+  const int k = q_power((int)m, (int)mr, a.scale_log2);
   const float up = __uint_as_float((uint32_t)(127 + k) << 23);
   if (j16 == 0) s.qscale[row] = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
   const int r = row >> 3, gq = row & 7;

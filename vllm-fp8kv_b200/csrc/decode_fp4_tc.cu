@@ -30,8 +30,8 @@
 // prefetched into L2, 56 rows read sector by sector.
 //
 // The latents are exact in fp16 (fp4.cuh), so the 32 latent k-steps of S and the
-// O product are fp16 MMAs: q is scaled per head by a power of two to a largest
-// value in [2^8, 2^9) and converted, and P keeps 11 bits where bf16 keeps 8.  The
+// O product are fp16 MMAs: q is converted, scaled per head by a power of two where
+// it needs that (load_q), and P keeps 11 bits where bf16 keeps 8.  The
 // rope's four k-steps are bf16 MMAs (q's rope times the same power of two) into
 // the same accumulator.
 //
@@ -502,9 +502,7 @@ __device__ __forceinline__ float load_q(Smem& s, const uint16_t* q0, int64_t q_s
   const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
   // First as it is, which is exact enough where the head's largest latent magnitude
   // lies in [2^-2, 2^15] (an fp16 subnormal's error is below 2^-23 of it then).
-  // Else again times 2^k, which brings that magnitude to [2^8, 2^9), but the rope's at
-  // most to 2^101, where its products are still finite (1 for rows of zeros, inf
-  // or NaN).  Exponents of bf16 lie in [-127, 127]: 2^k and 2^-k are normal.
+  // Else again times 2^k (q_power).
   int k = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
@@ -570,7 +568,7 @@ __device__ __forceinline__ float load_q(Smem& s, const uint16_t* q0, int64_t q_s
       uint32_t mr = 0;
       for (int i = 0; i < 8; ++i) mr = __vmaxu2(mr, mag(reinterpret_cast<const uint4*>(q0 + m * q_sh + kNope)[i]));
       const int br = (int)max(mr & 0xFFFFu, mr >> 16);
-      k = min(126, min(8 - ((bm >> 7) - 127), 100 - ((br >> 7) - 127)));
+      k = q_power(bm, br, scale_log2);
     }
     if (hh == 0) s.qk[m] = k;
     const bool any = __any_sync(0xFFFFFFFFu, again);

@@ -47,6 +47,26 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// The power of two, k, that a head's q is taken times on its way to fp16 (its rope in
+// bf16 too: both products meet in one accumulator).  m and mr: the largest magnitudes
+// (bf16 bits) of its latent part and of its rope; scale_log2: the factor from q . k
+// to scores in log2 units.
+//   * It brings the latents' largest value to [2^8, 2^9): what is lost below 2^-17 of
+//     the scaled values is under 2^-33 of the largest.
+//   * It is held to 2^24 / scale_log2.  A latent's rounding error (2^-25 at most) then
+//     moves a score by less than 2^-48 a unit of cached latent, 2^-27 for a row full of
+//     its largest, 2688: further bits of tiny latents would say nothing.  And a score is
+//     at least 2^-24 of its accumulator, so sums are finite up to scores of 2^103,
+//     however tiny the latents beside whatever rope.
+//   * The rope itself stays below 2^127.
+// 0 for latents of zeros, inf or NaN.  Exponents of bf16 and fp32 lie in [-127, 128],
+// so k lies in [-119, 126]: 2^k and 2^-k are normal.
+__device__ __forceinline__ int q_power(int m, int mr, float scale_log2) {
+  const int em = (m >> 7) - 127, er = (mr >> 7) - 127;
+  const int es = (int)((__float_as_uint(scale_log2) >> 23) & 255u) - 127;
+  const int k = min(min(8 - em, es + 24), min(126, 126 - er));
+  return m == 0 || m >= 0x7F80 ? 0 : k;
+}
 // Codes times scale in bf16, exact (at most 6 significant bits, and far from the
 // ends of the range).  An fp16 code (normal or zero) moved three bits to the right
 // under its sign is the bf16 code times 2^-112; the scale carries the 2^112.
