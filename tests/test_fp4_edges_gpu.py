@@ -1,11 +1,11 @@
 """fp4_ds_mla attention where it can go wrong: queries whose parts differ in size by
-many orders of magnitude, against 64 bits."""
+many orders of magnitude, and calls that take long, against 64 bits."""
 
 import pytest
 import torch
 
 from tests import fp4_ref as R
-from tests.test_fp4_gpu import MANY, SCALE, check_sparse, ints, make_pool, randn, sparse_case, status_clean
+from tests.test_fp4_gpu import MANY, SCALE, check_sparse, dense_slots, make_pool, randn, sparse_case, status_clean
 from vllm_fp8kv import fp4_ds_mla as F
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +46,30 @@ def test_latents_decide_beside_cached_ropes_of_zero(H, latent):
     scale = SCALE * 2.0 ** -latent
     both(q, pool, idx, R.attend(q, pool, idx, scale), scale)
     status_clean()
+
+
+@pytest.mark.parametrize("H", [16, 128])
+def test_calls_longer_than_the_wait_limit(H):
+    """A wait gives up after about 0.4 s; a call may take longer without one that
+    does.  One token's q and one page table serve all rows (stride 0, the same 64
+    pages again and again), so that the call is long and its inputs small."""
+    page, times, own = 64, 64, 64
+    pool = make_pool(210, page * own)
+    table = torch.randperm(own, device="cuda").to(torch.int32).repeat(times).view(1, -1)
+    n = page * own * times  # 262144 positions, each row of the pool `times` times
+    T = 8192 if H == 128 else 20000
+    q = randn(211, 1, H, 576).expand(T, H, 576)
+    req = torch.zeros(T, dtype=torch.int32, device="cuda")
+    lens = torch.full((T,), n, dtype=torch.int32, device="cuda")
+    lens[1::7] = n - 1000
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    out, lse = F.fp4_ds_mla_decode(q, pool, req, table, lens, SCALE, block_size=page, return_lse=True)
+    b.record()
+    status_clean()
+    assert a.elapsed_time(b) > 450  # ms: else this shows nothing
+    slots = dense_slots(table, req[:2], lens[:2], page)
+    want = R.attend(q[:2], pool, slots, SCALE)
+    for t in (0, T // 2 // 7 * 7, (T - 2) // 7 * 7):
+        R.check((out[t:t + 1], lse[t:t + 1]), [w[:1] for w in want])
+        R.check((out[t + 1:t + 2], lse[t + 1:t + 2]), [w[1:] for w in want])

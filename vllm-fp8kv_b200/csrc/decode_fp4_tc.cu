@@ -251,7 +251,10 @@ __device__ void mma_role(const Ctx& c) {
   }
 }
 
-// The MMA warp of both CTAs: every arrival that is still on its way to one of
+// One warp of each CTA, when the last MMA has been issued: the even CTA's issuing warp,
+// and in the odd CTA, where nobody issues, a softmax warp that has seen the last O (a
+// warp that came here at the start would have to wait for as long as the call takes).
+// Every arrival that is still on its way to one of
 // this CTA's barriers is seen in before the CTA may exit (one that finds its
 // target gone is an illegal access; the closing cluster barrier alone does not
 // hold it back).  The drain commit arrives once every MMA is done.  Of the last
@@ -833,7 +836,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     softmax_role(c, warp, lane);
   } else if (warp == kMmaWarp) {
     if (c.rank == 0) mma_role(c);
-    settle(c);
   } else if (warp < 8 || warp == 9) {
     k_role(c, warp < 8 ? warp - 5 : 3, lane);
   } else if (warp == 15) {
@@ -841,6 +843,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp != 8 && warp != 12) {
     v_role(c, warp < 12 ? warp - 10 : warp - 11, lane);
   }
+
+  if (warp == (c.rank == 0 ? kMmaWarp : 0)) settle(c);
 
   // both CTAs: no MMA of the pair may still run, no arrival may still target the
   // other CTA, before tensor memory is freed and the CTAs exit

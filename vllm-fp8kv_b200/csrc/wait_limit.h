@@ -5,7 +5,8 @@
 namespace fp8mla {
 // try_wait suspends for a hardware-chosen interval per call (about 87 ns on
 // B200, so 2^22 calls take about 0.4 s): well beyond the longest legitimate
-// wait of a CTA (its whole MMA chain, tens of microseconds), yet a broken
-// protocol ends in under a second with the timeout recorded.
+// wait, which spans a few tiles or one change of unit (tens of microseconds)
+// and never a whole call, yet a broken protocol ends in under a second with
+// the timeout recorded.
 constexpr uint32_t kMaxWaitIters = 1u << 22;
 }  // namespace fp8mla
