@@ -85,13 +85,15 @@ FP8MLA_API int fp8mla_device_status(unsigned int* status, int reset, void* strea
 FP8MLA_API uint32_t fp8mla_wait_limit(void);
 
 /*
- * Exercises the error path of the decode kernels' bounded on-chip waits: a
- * one-warp kernel runs their wait loop on an mbarrier that nothing arrives
- * on, gives up after `iters` (1 .. fp8mla_wait_limit()) try_wait calls and
+ * Exercises the error path of the decode kernels' bounded on-chip waits: for
+ * each of their two wait loops a one-warp kernel runs it on an mbarrier that
+ * nothing arrives on, gives up after `iters` (1 .. fp8mla_wait_limit())
+ * try_wait calls (a 64th of them in the fp4_ds_mla kernels' loop, in which
+ * every lane looks: such a call suspends the warp about 50 times as long) and
  * returns, leaving bit 0 and "which wait" = 63 in the device status word
- * (fp8mla_device_status).  *elapsed_ns (if not NULL) receives the loop's
- * duration, so a caller can see how long a full-limit timeout takes.  No GPU
- * fault is involved and the context stays usable.  Synchronises `stream`.
+ * (fp8mla_device_status).  *elapsed_ns (if not NULL) receives the longer
+ * loop's duration, so a caller can see how long a full-limit timeout takes.
+ * No GPU fault is involved and the context stays usable.  Synchronises `stream`.
  * For tests and health checks; no reference counterpart.
  */
 FP8MLA_API int fp8mla_selftest_wait_timeout(uint32_t iters, uint64_t* elapsed_ns, void* stream);

@@ -94,3 +94,13 @@ def test_small_head_decode_timeout_path_returns_and_reports(cuda_device):
     U.assert_close(out.float().cpu().numpy(), ref)
     U.assert_lse_close(lse.cpu().numpy(), ref_lse)
     assert N.device_status(reset=True) == 0
+
+
+def test_every_wait_loop_gives_up_within_a_second(cuda_device):
+    """Also the loop of the fp4_ds_mla kernels, in which all lanes of a warp look and
+    a look suspends the warp for microseconds."""
+    N.device_status(reset=True)
+    ns = _selftest(N.lib().fp8mla_wait_limit())
+    assert 0 < ns < 1e9
+    assert N.device_status(reset=True) == 1 | (SELFTEST_WHERE << 8)
+    assert _selftest(1) > 0 and N.device_status(reset=True) == 1 | (SELFTEST_WHERE << 8)

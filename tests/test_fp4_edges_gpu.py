@@ -50,7 +50,7 @@ def test_latents_decide_beside_cached_ropes_of_zero(H, latent):
 
 @pytest.mark.parametrize("H", [16, 128])
 def test_calls_longer_than_the_wait_limit(H):
-    """A wait gives up after about 0.4 s; a call may take longer without one that
+    """A wait gives up after less than 0.4 s; a call may take longer without one that
     does.  One token's q and one page table serve all rows (stride 0, the same 64
     pages again and again), so that the call is long and its inputs small."""
     page, times, own = 64, 64, 64

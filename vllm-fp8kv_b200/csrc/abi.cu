@@ -148,7 +148,12 @@ int fp8mla_selftest_wait_timeout(uint32_t iters, uint64_t* elapsed_ns, void* str
   if (iters == 0 || iters > fp8mla_wait_limit())
     return set_error(FP8MLA_ERR_INVALID_ARGUMENT, "iters must be in [1, %u]", fp8mla_wait_limit());
   if (int rc = require_sm100()) return rc;
-  return launch_wait_timeout_selftest(iters, elapsed_ns, static_cast<cudaStream_t>(stream));
+  uint64_t one = 0, all = 0;  // a lane that looks for its warp, and all lanes
+  int rc = launch_wait_timeout_selftest(iters, &one, static_cast<cudaStream_t>(stream));
+  if (rc == FP8MLA_OK)
+    rc = launch_wait_timeout_selftest_fp4((iters + 63) / 64, &all, static_cast<cudaStream_t>(stream));
+  if (elapsed_ns != nullptr) *elapsed_ns = one > all ? one : all;
+  return rc;
 }
 
 uint32_t fp8mla_wait_limit(void) { return kMaxWaitIters; }

@@ -676,7 +676,34 @@ __global__ void __launch_bounds__(128 * kSplit) merge_fp4_kernel(const Fp4Decode
     a.lse[t * a.lse_st + h] = l == 0.f ? -INFINITY : (m - bias) * kLn2 + logf(l);
 }
 
+// Self-test of the error path of fp4::wait: as wait_timeout_selftest_kernel, the same
+// code (63) in this file's status word.
+__device__ unsigned long long g_selftest_ns = 0;
+__global__ void __launch_bounds__(32) wait_timeout_selftest_fp4_kernel(uint32_t looks) {
+  __shared__ uint64_t bar;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar), 1);
+    mbar_init_fence();
+  }
+  __syncwarp();
+  unsigned long long t0, t1;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  (void)wait<1>(bar, 0, 63, looks);
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+  if (threadIdx.x == 0) g_selftest_ns = t1 - t0;
+}
+
 }  // namespace
+
+int launch_wait_timeout_selftest_fp4(uint32_t looks, uint64_t* elapsed_ns, cudaStream_t st) {
+  wait_timeout_selftest_fp4_kernel<<<1, 32, 0, st>>>(looks);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  unsigned long long ns = 0;
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&ns, g_selftest_ns, sizeof(ns));
+  *elapsed_ns = ns;
+  return check_cuda(e, "wait timeout self-test");
+}
 
 int launch_merge_fp4(const Fp4DecodeArgs& a, float bias, cudaStream_t st) {
   if (a.workers < 2) return FP8MLA_OK;

@@ -76,6 +76,8 @@ int launch_merge_fp4(const Fp4DecodeArgs& a, float bias, cudaStream_t st);
 constexpr int kFp4Chunk = 64;   // entries per chunk
 constexpr int kFp4MinPer = 3;   // a worker's three groups of warps take a chunk each
 int read_device_status_fp4(unsigned int* status, bool reset, cudaStream_t st);
+// launch_wait_timeout_selftest for the wait loop of these kernels.
+int launch_wait_timeout_selftest_fp4(uint32_t looks, uint64_t* elapsed_ns, cudaStream_t st);
 
 int launch_fp4_write(const uint16_t* kv_c, int64_t kv_c_stride, const uint16_t* k_pe, int64_t k_pe_stride,
                      const int64_t* slot_mapping, int64_t N, uint8_t* cache, int64_t num_slots,

@@ -251,13 +251,17 @@ struct Slots {
 // Bounded wait of a whole warp: every lane looks (so every lane has acquired the
 // phase) and the vote gives all of them one verdict.  A phase that is complete
 // costs 18 cycles; one lane looking for the others and passing the verdict on
-// costs 190.  kUnroll: the compiler's choice would be 8 KB of code for every wait.
+// costs 190.  `limit` counts looks, rounded up to kUnroll.  kUnroll: the compiler's
+// choice would be 8 KB of code for every wait.
 template <int kUnroll>
-__device__ __forceinline__ bool wait(uint64_t& b, uint32_t parity, uint32_t where) {
+__device__ __forceinline__ bool wait(uint64_t& b, uint32_t parity, uint32_t where,
+                                     uint32_t limit = kMaxWaitLooks) {
   const uint32_t at = smem_u32(&b);
-#pragma unroll kUnroll
-  for (uint32_t it = 0; it < tc::kMaxWaitIters; ++it)
-    if (__all_sync(0xFFFFFFFFu, tc::mbar_try_wait(at, parity))) return true;
+#pragma unroll 1
+  for (uint32_t it = 0; it < limit; it += kUnroll)
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (__all_sync(0xFFFFFFFFu, tc::mbar_try_wait(at, parity))) return true;
   if ((threadIdx.x & 31) == 0) atomicOr(&tc::g_device_status, tc::kStatusWaitTimeout | (where << 8));
   return false;
 }
