@@ -99,13 +99,15 @@ FP8MLA_API uint32_t fp8mla_wait_limit(void);
 FP8MLA_API int fp8mla_selftest_wait_timeout(uint32_t iters, uint64_t* elapsed_ns, void* stream);
 
 /*
- * Lowers the limit of the hand-off waits of the small-head decode kernel
+ * Lowers the limit of the hand-off waits of the small-head decode kernels
  * (decode_ws_kernel: raw rows, key rows and Q between its producer, dequant
- * and compute warps) to `iters` try_wait calls for the decode calls that
+ * and compute warps; decode_fp4_kernel: rows between its producers and
+ * compute warps) to `iters` try_wait calls (in decode_fp4_kernel a 64th of
+ * them, below 64 one call that does not suspend) for the decode calls that
  * follow in this process; 0 restores fp8mla_wait_limit().  With a limit of a
  * few calls the waits give up while the copies they wait for are still
  * arriving, so a test can drive the kernel's error path without a fault:
- * the producer stops issuing copies, waits (with the full limit) for those it
+ * the producers stop issuing copies, wait (with the full limit) for those they
  * issued, every warp returns, and the status word carries the timeout.
  * Results of such calls are meaningless.  For tests; no reference
  * counterpart.  Returns FP8MLA_ERR_INVALID_ARGUMENT above the full limit.

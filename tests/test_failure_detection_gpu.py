@@ -14,8 +14,10 @@ import pytest
 import torch
 
 from oracle import oracle as O
+from tests import fp4_ref as R
 from tests import gpu_util as U
 from vllm_fp8kv import _native as N
+from vllm_fp8kv import fp4_ds_mla as F
 from vllm_fp8kv import synthetic
 from vllm_fp8kv.fp8_ds_mla_sparse_decode import fp8_ds_mla_sparse_decode
 
@@ -104,3 +106,33 @@ def test_every_wait_loop_gives_up_within_a_second(cuda_device):
     assert 0 < ns < 1e9
     assert N.device_status(reset=True) == 1 | (SELFTEST_WHERE << 8)
     assert _selftest(1) > 0 and N.device_status(reset=True) == 1 | (SELFTEST_WHERE << 8)
+
+
+@pytest.mark.parametrize("topk", [2048, 300])
+def test_fp4_decode_timeout_path_returns_and_reports(cuda_device, topk):
+    """The same for decode_fp4_kernel: with a limit of two calls its compute warps
+    give up on rows that are still arriving.  They release no stage after that, so
+    the producers give up too and wait for the copies they issued; the call
+    completes, the status word carries the kernel's wait codes (20, 21, 26), and the
+    next call is right."""
+    L = N.lib()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(22)
+    pool = R.quantize(*(torch.randn(4000, n, generator=g, device="cuda").to(torch.bfloat16) for n in (512, 64)))
+    q = torch.randn(160, 16, 576, generator=g, device="cuda").to(torch.bfloat16)
+    idx = torch.randint(0, 4000, (160, 1, topk), generator=g, device="cuda").to(torch.int32)
+    assert F.fp4_kernel_name(16, 1, 160, topk) == "decode_fp4_kernel"
+    N.device_status(reset=True)
+    N.check(L.fp8mla_selftest_set_wait_limit(2), "set wait limit")
+    try:
+        F.fp4_ds_mla_sparse_decode(q, pool, idx, 0.07)
+        torch.cuda.synchronize()
+        st = N.device_status(reset=True)
+    finally:
+        N.check(L.fp8mla_selftest_set_wait_limit(0), "restore wait limit")
+    assert st & 1, f"no timeout recorded (status {st:#x})"
+    assert 16 <= (st >> 8) < 32, f"unexpected wait code in status {st:#x}"
+    got = F.fp4_ds_mla_sparse_decode(q, pool, idx, 0.07, return_lse=True)
+    R.check([x[:4] for x in got], R.attend(q[:4], pool, idx[:4], 0.07))
+    R.check([x[-4:] for x in got], R.attend(q[-4:], pool, idx[-4:], 0.07))
+    assert N.device_status(reset=True) == 0

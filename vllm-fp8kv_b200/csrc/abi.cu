@@ -31,7 +31,7 @@ int check_cuda(cudaError_t e, const char* what) {
 }
 
 namespace {
-// Hand-off wait limit of the small-head kernel (fp8mla_selftest_set_wait_limit).
+// Hand-off wait limit of the small-head kernels (fp8mla_selftest_set_wait_limit).
 std::atomic<uint32_t> g_handoff_wait_iters{kMaxWaitIters};
 
 constexpr int kMaxDevices = 64;
@@ -101,6 +101,8 @@ int64_t ws_bytes(int64_t T, int64_t H, int S, int elem_bytes) {
 }  // namespace
 
 void clear_error() { g_last_error[0] = 0; }
+
+uint32_t handoff_wait_iters() { return g_handoff_wait_iters.load(); }
 
 int require_sm100() {
   const DevInfo* d = dev_info();
@@ -285,7 +287,7 @@ int decode_impl(const void* q, int q_dtype, int64_t T, int64_t H, int64_t q_stri
   a.lse_st = lse_stride_t;
   a.num_splits = S;
   a.split_len = (int)((topk + S - 1) / S);
-  a.wait_iters = g_handoff_wait_iters.load();
+  a.wait_iters = handoff_wait_iters();
   if (S > 1) {
     const int elem = q_dtype == FP8MLA_DTYPE_BF16 ? 2 : 4;  // partials in the output dtype
     const int64_t need = ws_bytes(T, H, S, elem);

@@ -2,6 +2,7 @@
 // argument checks, the division of work, workspace layout and dispatch.
 #include "common.cuh"
 #include "decode_fp4.h"
+#include "wait_limit.h"
 
 using namespace fp8mla;
 
@@ -164,6 +165,7 @@ int attend(const uint16_t* q, int64_t T, int64_t H, int64_t q_st, int64_t q_sh, 
   for (int k = 0; k < 31; ++k)
     if (block_table != nullptr && (int64_t)1 << k == block_size) a.block_shift = k;
   a.max_len = max_blocks * block_size;
+  a.wait_looks = handoff_wait_iters() / (kMaxWaitIters / kMaxWaitLooks);
   if (p.cuts) {
     char* ws = static_cast<char*>(workspace);
     a.ws_o = reinterpret_cast<float*>(ws);

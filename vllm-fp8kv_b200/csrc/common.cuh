@@ -36,6 +36,7 @@ int check_cuda(cudaError_t e, const char* what);
 void clear_error();
 int require_sm100();  // FP8MLA_OK when the current device is sm_100
 int device_sm_count();
+uint32_t handoff_wait_iters();  // limit of the small-head kernels' hand-off waits
 int device_arch(int* major, int* minor);
 
 // ---------------------------------------------------------------- PTX helpers

@@ -131,6 +131,15 @@ struct Ring {
   }
 };
 
+// A wait between producers and compute warps.  A limit of 0 looks (a test's) stands for
+// one that does not suspend the warp.
+__device__ __forceinline__ bool hand_off(const Fp4DecodeArgs& a, uint64_t& b, uint32_t parity, uint32_t where) {
+  if (a.wait_looks != 0) return wait<4>(b, parity, where, a.wait_looks);
+  if (__all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&b), parity))) return true;
+  if ((threadIdx.x & 31) == 0) atomicOr(&g_device_status, kStatusWaitTimeout | (where << 8));
+  return false;
+}
+
 // ------------------------------------------------------------------ producers
 // Warp pw owns rows [16 pw, +16) of every chunk: lanes 0-15 those of the even
 // chunks of the worker's run, lanes 16-31 of the odd ones.  A run of consecutive
@@ -158,7 +167,7 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
     for (int half = 0; half < 2; ++half) {
       if (g + half >= chunks) break;
       const int st = ring.st;
-      if (g + half >= kStages) ok = wait<4>(s.raw_empty[st], ring.ph ^ 1, 20);
+      if (g + half >= kStages) ok = hand_off(a, s.raw_empty[st], ring.ph ^ 1, 20);
       if (!ok) break;
       const uint32_t live = (live2 >> (16 * half)) & 0xFFFFu;
       const int n = __popc(live);
@@ -197,6 +206,11 @@ __device__ void produce(const Fp4DecodeArgs& a, Smem& s, const CUtensorMap* tm, 
 }
 
 // ------------------------------------------------------------------ compute
+// After a failed wait a warp goes on to the end, for the barriers that it shares with
+// others, on whatever its stages hold, and releases no stage any more: a stage is
+// armed anew only when all that it was armed with before has landed, so that the
+// producers' last waits name their last copies.
+//
 // Fragment coordinates: lane = 4 gq + q4.  Thread q4 of a quad owns latent
 // dims [128 q4, +128) of a row and rope dims [16 q4, +16); it walks its four
 // 32-dim pieces in the order i ^ (q4 >> 1) and its two rope halves in the order
@@ -382,7 +396,7 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int cw, int lane) {
     Ring ring = piece_at;
     ring.ahead(grp);
     for (int c = grp; c < nch; c += kGroups) {
-      if (ok) ok = wait<4>(s.raw_full[ring.st], ring.ph, 21);
+      if (ok) ok = hand_off(a, s.raw_full[ring.st], ring.ph, 21);
       const uint64_t live = *reinterpret_cast<const uint64_t*>(s.live[ring.st]);
       const uint8_t* raw = s.raw[ring.st];
       float x[2][4];
@@ -451,7 +465,7 @@ __device__ void compute(const Fp4DecodeArgs& a, Smem& s, int cw, int lane) {
       }
       output_step(raw, s.p[grp][pb], live, lane, code_at, scale_at, ra, rb, acc);
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.raw_empty[ring.st]));
+      if (ok && lane == 0) mbar_arrive(smem_u32(&s.raw_empty[ring.st]));
       ring.ahead(kGroups);
       pb ^= 1;
     }

@@ -48,6 +48,7 @@ struct Fp4DecodeArgs {
   float* ws_o;           // [2 * workers][rows][512] unnormalised partials
   float2* ws_ml;         // [2 * workers][rows] (reference max in log2 units, sum)
   int64_t* ws_info;      // [workers][4]: unit, first chunk in it, its chunks, per
+  uint32_t wait_looks;   // limit of decode_fp4_kernel's hand-off waits
 };
 
 // Raises a kernel's dynamic shared memory limit, once per device.
