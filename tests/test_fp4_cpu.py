@@ -151,3 +151,15 @@ def test_reference_round_trips_and_rounds_to_even():
     g = torch.tensor([6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, -0.25, -5, 0, 0, 0, 0, 0, 0], dtype=torch.float64)
     back = R.values(R.quantize(g.repeat(32).view(1, 512).to(torch.bfloat16), bf(1, 64)))[0, :16]
     assert back.tolist() == [6, 0, 1, 1, 2, 2, 4, 4, -0.0, -4, 0, 0, 0, 0, 0, 0]
+
+
+def test_short_rows_of_few_heads_go_to_the_kernel_of_few_heads():
+    """Units of one or two chunks need no more than one SM each: nothing there is for
+    128-row tiles to gain at up to 32 heads."""
+    for H in (1, 8, 16, 17, 32):
+        for T in (1, 2, 7, 37, 64, 74, 75, 148, 256):
+            for topk in (0, 1, 63, 64, 65, 100, 127, 128):
+                assert F.fp4_kernel_name(H, 1, T, topk) == "decode_fp4_kernel", (H, T, topk)
+                if topk <= 64:
+                    assert F.fp4_workspace_bytes(T, H, 1, topk) == 0
+    assert F.fp4_kernel_name(128, 1, 148, 64) == "decode_fp4_tc_kernel"

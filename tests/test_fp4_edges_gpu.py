@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import fp4_ref as R
-from tests.test_fp4_gpu import MANY, SCALE, check_sparse, dense_slots, make_pool, randn, sparse_case, status_clean
+from tests.test_fp4_gpu import MANY, SCALE, check_sparse, dense_slots, ints, make_pool, randn, sparse_case, status_clean
 from vllm_fp8kv import fp4_ds_mla as F
 
 pytestmark = pytest.mark.gpu
@@ -73,3 +73,25 @@ def test_calls_longer_than_the_wait_limit(H):
     for t in (0, T // 2 // 7 * 7, (T - 2) // 7 * 7):
         R.check((out[t:t + 1], lse[t:t + 1]), [w[:1] for w in want])
         R.check((out[t + 1:t + 2], lse[t + 1:t + 2]), [w[1:] for w in want])
+
+
+@pytest.mark.parametrize("H", [1, 16, 40, 128])
+@pytest.mark.parametrize("T", [3, 64, 150, 400])
+def test_dense_short_contexts(H, T):
+    """Contexts of one or two chunks, by themselves and beside a longer one: fewer
+    chunks a worker than pieces of a cut unit have."""
+    pool = make_pool(220, 3200)
+    table = torch.randperm(50, device="cuda")[:40].to(torch.int32).view(4, 10)
+    q = randn(221, T, H, 576)
+    req = (torch.arange(T, device="cuda") % 4).to(torch.int32)
+    rows = torch.arange(T, device="cuda")
+    for most, long in ((64, 64), (130, 130), (64, 600)):
+        lens = ints(222 + most, most + 1, (T,)).to(torch.int32)
+        lens[T // 2] = long
+        got = F.fp4_ds_mla_decode(q, pool, req, table, lens, SCALE, return_lse=True)
+        R.check(got, R.attend(q, pool, dense_slots(table[req.long()], rows, lens, 64), SCALE))
+        tight = table[:, :(most + 63) // 64].contiguous()  # (the longest row the table holds is short, too)
+        if long == most:
+            again = F.fp4_ds_mla_decode(q, pool, req, tight, lens, SCALE, return_lse=True)
+            R.check(again, R.attend(q, pool, dense_slots(table[req.long()], rows, lens, 64), SCALE))
+    status_clean()

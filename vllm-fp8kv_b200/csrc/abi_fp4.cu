@@ -23,14 +23,16 @@ struct Plan {
 // Expected time, us, of a call whose workers take `per` chunks each of units of n
 // chunks; `cut`: units are cut, so there are partial results, a merge, and more
 // changes of unit than need be, unless n is a multiple of `per`.  Fitted to 560 calls of
-// either kernel (16 to 256 heads, 1 to 300 tokens, top-256 to top-4096), off by 3% on
-// average; choosing by it costs 0.1% against the best choice for each call.  For
-// instance, top-2048, 16-head kernel / paired kernel / chosen, measured:
-//   tokens   40 heads            64 heads            128 heads
-//   1        18.8 / 19 / 18.8    19.6 / 20 / 19.6    20.7 / 21 / 20.7
-//   8        24.3 / 25 / 24.3    25.7 / 27 / 25.7    34.6 / 31 / 31.0
-//   32       42.9 / 48 / 42.9    45.2 / 49 / 45.2    87 / 49.6 / 49.6
-//   160      151 / 142 / 142     204 / 139 / 141     384 / 146 / 146
+// either kernel; on 1755 shapes (8 to 128 heads, 1 to 256 tokens, top-1 to top-4096:
+// profiles/fp4_cost_model.txt) it is off by 5% in the 16-head kernel and by 18% in the
+// paired one, mostly above it, and choosing by it costs 0.3% on average against the
+// best choice for each call, at worst 24% (top-512, 1 token, 8 heads: 15.0 us whole, 12.1
+// cut).  For instance, 16-head kernel / paired kernel / chosen, measured:
+//   tokens   top-64, 16 heads    top-64, 128 heads    top-2048, 40        top-2048, 64        top-2048, 128
+//   1        7.3 / 10.9 / 7.3    7.2 / 12.7 / 7.2     18.4 / 17.7 / 18.4  18.9 / 19.3 / 18.9  19.3 / 20.1 / 19.3
+//   8        7.3 / 11.4 / 7.3    7.9 / 13.0 / 7.9     23.7 / 26.1 / 23.7  25.5 / 29.2 / 25.5  34.1 / 34.1 / 34.1
+//   32       7.7 / 11.8 / 7.7    13.7 / 13.4 / 13.7   42.9 / 48.5 / 42.9  45.7 / 51.0 / 45.7  88 / 52.1 / 52.1
+//   148      8.5 / 19.9 / 8.5    46 / 23.0 / 23.0     133 / 100 / 100     176 / 102 / 102     346 / 104 / 104
 double cost(bool tc, int64_t per, int64_t n, bool cut) {
   const double units = per > n ? (double)per / (double)n : 1.0;
   if (tc) return 2.8 + 2.46 * (double)per + 8.6 * units + (!cut ? 0 : n % per == 0 ? 11.4 : 24.6);
@@ -46,10 +48,10 @@ Plan plan_with(bool tc, int64_t T, int64_t H, int64_t G, int64_t topk, int64_t m
   p.workers = p.tc ? device_sm_count() / 2 : device_sm_count();
   p.hb_per_group = (int)((hpg + p.rows - 1) / p.rows);
   p.chunk = p.tc ? kFp4TcChunk : kFp4Chunk;
-  p.min_per = p.tc ? 1 : kFp4MinPer;
   const int64_t chunk = p.chunk, units = T * G * p.hb_per_group;
   const int64_t len = topk < 0 ? max_len : topk;
   const int64_t n = len > chunk ? (len + chunk - 1) / chunk : 1;  // chunks of a unit (at most)
+  p.min_per = p.tc ? 1 : (int)(n < kFp4MinPer ? n : kFp4MinPer);
   const int64_t total = units * n;
   if (total < p.workers) p.workers = (int)total;
   if (topk < 0) {

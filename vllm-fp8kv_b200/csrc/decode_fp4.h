@@ -43,7 +43,7 @@ struct Fp4DecodeArgs {
   int block_shift;       // log2(block_size) when it is a power of two, else -1
   int64_t max_len;       // max_blocks * block_size (lens set)
   int64_t per;           // chunks per worker; 0 = from the lengths, on the device
-  int min_per;           // ... but at least this many
+  int min_per;           // ... but at least this many, or a mean unit's
   int workers;
   float* ws_o;           // [2 * workers][rows][512] unnormalised partials
   float2* ws_ml;         // [2 * workers][rows] (reference max in log2 units, sum)
@@ -75,7 +75,7 @@ constexpr int kFp4TcRows = 128;
 constexpr int kFp4TcChunk = 128;
 int launch_merge_fp4(const Fp4DecodeArgs& a, float bias, cudaStream_t st);
 constexpr int kFp4Chunk = 64;   // entries per chunk
-constexpr int kFp4MinPer = 3;   // a worker's three groups of warps take a chunk each
+constexpr int kFp4MinPer = 3;   // chunks of a piece of a cut unit: three groups of warps take one each
 int read_device_status_fp4(unsigned int* status, bool reset, cudaStream_t st);
 // launch_wait_timeout_selftest for the wait loop of these kernels.
 int launch_wait_timeout_selftest_fp4(uint32_t looks, uint64_t* elapsed_ns, cudaStream_t st);

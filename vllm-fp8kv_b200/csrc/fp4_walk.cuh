@@ -59,7 +59,13 @@ __device__ void divide(const Fp4DecodeArgs& a, Share& s, int worker) {
   for (int w = 0; w < kThreads / 32; ++w) total += s.scan[w];
   total *= per_tok;
   int64_t per = quotient(total + a.workers - 1, a.workers);
-  if (per < a.min_per) per = a.min_per;
+  // pieces of a cut unit have min_per chunks at least, but units that are shorter on
+  // average are not lined up behind one another for that while SMs stand idle
+  if (per < a.min_per) {
+    const int64_t mean = quotient(total, a.T * per_tok);
+    const int64_t least = mean < a.min_per ? mean : a.min_per;
+    if (per < least) per = least;
+  }
   const int64_t at = (int64_t)worker * per;
   int64_t before = 0;  // chunks of the tokens in front of this pass
   for (int t0 = 0; t0 < a.T; t0 += kThreads) {
