@@ -1,5 +1,6 @@
 """fp4_ds_mla attention where it can go wrong: queries whose parts differ in size by
-many orders of magnitude, and calls that take long, against 64 bits."""
+many orders of magnitude, special values, lengths around the borders of a chunk in both
+kernels, and calls that take long, against 64 bits."""
 
 import pytest
 import torch
@@ -9,6 +10,8 @@ from tests.test_fp4_gpu import MANY, SCALE, check_sparse, dense_slots, ints, mak
 from vllm_fp8kv import fp4_ds_mla as F
 
 pytestmark = pytest.mark.gpu
+
+FEW = "decode_fp4_kernel"
 
 
 def both(q, pool, idx, want, scale):
@@ -94,4 +97,64 @@ def test_dense_short_contexts(H, T):
         if long == most:
             again = F.fp4_ds_mla_decode(q, pool, req, tight, lens, SCALE, return_lse=True)
             R.check(again, R.attend(q, pool, dense_slots(table[req.long()], rows, lens, 64), SCALE))
+    status_clean()
+
+
+def copies(kernel, q, topk, times=400):
+    """How many copies of q's rows a call needs to go to `kernel`."""
+    T, H, _ = q.shape
+    for r in range(1, times):
+        if F.fp4_kernel_name(H, 1, T * r, topk) == kernel:
+            return r
+    raise AssertionError(f"no call of {H} heads and top-{topk} goes to {kernel}")
+
+
+@pytest.mark.parametrize("H", [1, 16, 17, 32, 33, 48, 64, 65, 128, 130])
+@pytest.mark.parametrize("topk", [1, 63, 64, 65, 127, 128, 129, 192, 193, 500])
+def test_every_length_in_every_kernel(H, topk):
+    """Around the borders of a chunk of either kernel: all head counts in the kernel
+    of few heads, those above 32 in the other one too, where it is chosen at all."""
+    pool = make_pool(230, 900)
+    q, idx = sparse_case(231 + topk, 3, H, topk, 900, mask=0.2)
+    idx[1, :, -1] = -1
+    idx[2, :, 0] = -1
+    want = R.attend(q, pool, idx, SCALE)
+    for kernel in (FEW, MANY) if H >= 64 or (H > 32 and topk > 64) else (FEW,):
+        r = copies(kernel, q, topk)
+        out, lse = F.fp4_ds_mla_sparse_decode(q.repeat(r, 1, 1), pool, idx.repeat(r, 1, 1), SCALE, return_lse=True)
+        for i in {0, r // 2, r - 1}:
+            R.check((out[3 * i:3 * i + 3], lse[3 * i:3 * i + 3]), want)
+    status_clean()
+
+
+@pytest.mark.parametrize("kernel,H", [("few", 16), ("few", 40), ("many", 64), ("many", 128)])
+@pytest.mark.parametrize("topk", [100, 700])
+def test_special_values_in_attended_rows(kernel, H, topk):
+    """NaN scales, NaN ropes and infinite scores show in the rows (and heads) that
+    attend to them and in no other; an entry whose score is -inf weighs nothing."""
+    kernel = FEW if kernel == "few" else MANY
+    pool = make_pool(240, 800)
+    q, _ = sparse_case(241, 6, H, topk, 800)
+    q[..., 512] = q[..., 512].abs() + 0.5
+    pool[790, 256 + 31] = 0x7F                                     # the last group of the latents
+    pool[791, 288:290] = torch.tensor([0xC0, 0x7F], device="cuda")  # rope: NaN
+    pool[792, 288:290] = torch.tensor([0x80, 0x7F], device="cuda")  # +inf
+    pool[793, 288:290] = torch.tensor([0x80, 0xFF], device="cuda")  # -inf
+    idx = ints(242, 780, (6, 1, topk)).to(torch.int32)
+    for t, at in ((1, 790), (2, 791), (3, 792), (4, 793)):
+        idx[t, 0, topk - 7 * t] = at
+    masked = idx.clone()
+    masked[4, 0, topk - 28] = -1
+    r = copies(kernel, q, topk)
+    out, lse = F.fp4_ds_mla_sparse_decode(q.repeat(r, 1, 1), pool, idx.repeat(r, 1, 1), SCALE, return_lse=True)
+    clean = [0, 4, 5]
+    want = [w[clean] for w in R.attend(q, pool, torch.where(masked >= 790, -1, masked), SCALE)]
+    for i in {0, r // 2, r - 1}:
+        o, l = out[6 * i:6 * i + 6], lse[6 * i:6 * i + 6]
+        assert o[1:4].isnan().all() and l[1:4].isnan().all()
+        R.check((o[clean], l[clean]), want)
+    nothing = torch.full_like(idx[:1], 793)  # scores of -inf alone: as nothing to attend
+    rows = q[5:].repeat(6 * r, 1, 1)
+    out, lse = F.fp4_ds_mla_sparse_decode(rows, pool, nothing.repeat(6 * r, 1, 1), SCALE, return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
     status_clean()
