@@ -89,6 +89,25 @@ def test_bf16_path_stays_upstream_on_cpu(vllm):
     assert impl.bf16_indices[0, :4].tolist() == [192, 193, 64, -1]
 
 
+def test_fp4_layers_and_pools_are_refused(vllm):
+    """Not upstream's bf16 path over 4-bit rows, nor a pool of its shape."""
+    backend_patch.apply()
+    impl = vllm.impl(kv_cache_dtype="fp4_ds_mla", softmax_scale=1 / 24.0)
+    impl.topk_indices_buffer = torch.zeros(1, 128, dtype=torch.int32)
+
+    class Md:
+        req_id_per_token = torch.zeros(1, dtype=torch.int32)
+        block_table = torch.zeros(1, 4, dtype=torch.int32)
+        block_size = 64
+        topk_tokens = 128
+
+    with pytest.raises(NotImplementedError, match="fp4_ds_mla"):
+        impl.forward_mqa(torch.randn(1, 16, 576), torch.zeros(4, 64, 416, dtype=torch.uint8), Md, None)
+    assert impl.bf16_calls == 0
+    with pytest.raises(NotImplementedError, match="fp4_ds_mla"):
+        vllm.backend.get_kv_cache_shape(8, 64, 1, 576, "fp4_ds_mla")
+
+
 # ------------------------------------------------------------------- GPU paths
 def _pool(n_slots=512, seed=3):
     rng = np.random.default_rng(seed)

@@ -13,6 +13,8 @@ Behaviour matches the reference's backend_patch (vllm_fp8kv/backend_patch.py:50-
 * ``_get_kv_cache_shape_fp8_aware`` -- 656-byte rows for fp8_ds_mla
 * ``_patch_mla_spec_quant_mode`` -- the MLA KV-cache spec of an fp8_ds_mla pool
                                     declares itself quantized
+* a layer or pool of ``fp4_ds_mla`` is refused: vLLM has no such cache dtype, and
+  upstream's bf16 path would misread its rows
 * ``apply()``                    -- installs all of it into a live vLLM; idempotent
 """
 
@@ -25,9 +27,15 @@ from vllm_fp8kv.fp8_ds_mla_sparse_decode import (
 )
 
 FP8_DS_MLA = "fp8_ds_mla"
+FP4_DS_MLA = "fp4_ds_mla"
 _CLI_FP8_NAMES = ("fp8", "fp8_e4m3")
 _MARK = "_vllm_fp8kv_b200"
 _CONVERT_BLOCK_N = 128  # entries per program of vLLM's index converter
+
+
+def _refuse_fp4(dtype) -> None:
+    if dtype == FP4_DS_MLA:
+        raise NotImplementedError(f"{FP4_DS_MLA} is not served through vLLM; call vllm_fp8kv.fp4_ds_mla")
 
 
 def _as_single_q(q):
@@ -71,6 +79,7 @@ def _forward_fp8_kv_paged(self, q, kv_c_and_k_pe_cache, topk_indices, attn_metad
 
 def _forward_mqa_fp8_aware(self, q, kv_c_and_k_pe_cache, attn_metadata, layer):
     """Replacement ``forward_mqa`` that accepts fp8_ds_mla KV."""
+    _refuse_fp4(self.kv_cache_dtype)
     q = _as_single_q(q)
     n_tok = q.shape[0]
     assert self.topk_indices_buffer is not None
@@ -93,6 +102,7 @@ def _forward_mqa_fp8_aware(self, q, kv_c_and_k_pe_cache, attn_metadata, layer):
 def _get_kv_cache_shape_fp8_aware(num_blocks: int, block_size: int, num_kv_heads: int,
                                   head_size: int, cache_dtype_str: str = "auto") -> tuple:
     """fp8_ds_mla pools are (num_blocks, block_size, 656) bytes; others head_size wide."""
+    _refuse_fp4(cache_dtype_str)
     if cache_dtype_str == FP8_DS_MLA:
         return (num_blocks, block_size, ROW_BYTES)
     return (num_blocks, block_size, head_size)
