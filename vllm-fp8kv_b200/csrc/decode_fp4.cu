@@ -4,8 +4,8 @@
 //
 // A persistent CTA per SM walks its run of 64-entry chunks (decode_fp4.h).
 // The 416-byte rows stay 4-bit in shared memory; both products unpack them in
-// registers, straight into mma.sync fragments: a bf16 copy of a row in shared
-// memory would cost 1152 bytes written and twice read against 416 read twice.
+// registers, straight into mma.sync fragments.  Shared memory sees 416 bytes of a row
+// written and twice read, and 1152 of q (18 KB for every 16 entries).
 //   * latents are exact in fp16 (fp4.cuh), so the latent products are fp16
 //     MMAs: q is scaled per head by a power of two (q_power), to a largest value in
 //     [2^8, 2^9) where the softmax scale is of ordinary size, and converted (exact

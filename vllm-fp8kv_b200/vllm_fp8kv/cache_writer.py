@@ -44,7 +44,8 @@ def concat_and_cache_ds_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: to
 def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
                          slot_mapping: torch.Tensor, kv_cache_dtype: str,
                          scale: torch.Tensor | float | None = None) -> None:
-    """vLLM-signature wrapper: the fp8_ds_mla format, and this library's fp4_ds_mla."""
+    """vLLM-signature wrapper: the fp8_ds_mla format, and this library's fp4_ds_mla.
+    ``scale`` is not used: rows of both formats carry their own."""
     if kv_cache_dtype == "fp4_ds_mla":
         concat_and_cache_fp4_ds_mla(kv_c, k_pe, kv_cache, slot_mapping)
         return

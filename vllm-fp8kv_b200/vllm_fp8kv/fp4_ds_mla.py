@@ -23,7 +23,7 @@ reads back as NaN.
 * ``fp4_ds_mla_decode``               attention over whole contexts
 
 The attention takes bf16 q only: the latents enter the tensor cores exactly (as
-fp16, beside q scaled by a power of two), the softmax's weights in fp16 (11 bits;
+fp16, beside q in fp16, scaled by a power of two per head), the softmax's weights in fp16 (11 bits;
 below 2^-20 of a row's largest with an error of up to 2^-31 of it, so that those
 below 2^-31 count as 0), sums in fp32.  All calls
 run on the current stream of the tensors' device and never synchronise.
@@ -122,8 +122,9 @@ def gather_fp4_ds_mla(kv_cache: torch.Tensor, block_table: torch.Tensor, cu_seq_
     Row r of sequence b (cu_seq_lens[b] <= r < cu_seq_lens[b + 1]) is position
     seq_starts[b] + r - cu_seq_lens[b] of it; block_table [B, max_blocks] int32
     holds its pages.  Positions behind the table, or on pages outside the pool,
-    give zero rows.  num_tokens is cu_seq_lens[-1]; where it (or `out`) has more
-    rows, those behind the last sequence are left as they were."""
+    give zero rows.  num_tokens, the rows of `out`, is cu_seq_lens[-1]; where it is
+    more, the rows behind the last sequence are left as they were (whatever the
+    allocator gave, without `out`)."""
     num_slots = _pool(kv_cache)
     assert block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table [B, max_blocks] int32"
     assert block_table.shape[1] == 0 or block_table.stride(1) == 1, "block_table rows must be unit-strided"
