@@ -80,7 +80,9 @@ FP8MLA_API int fp8mla_device_status(unsigned int* status, int reset, void* strea
 
 /*
  * Number of mbarrier try_wait calls after which a decode kernel's on-chip
- * wait gives up (and sets the device status word).  No reference counterpart.
+ * wait gives up (and sets the device status word); a 64th of it in the
+ * fp4_ds_mla kernels, whose calls suspend for longer.  No reference
+ * counterpart.
  */
 FP8MLA_API uint32_t fp8mla_wait_limit(void);
 
